@@ -51,6 +51,9 @@ typedef enum ltq_out_mode {
     LTQ_OUT_I32 = 2  /* acc itself: sum (a-z_a)(w-z_w) + bias, l-ten/math_fns.cpp:1469-1473 */
 } ltq_out_mode;
 
+/* Element type of floating-point tensors, for the operators that take more than float. */
+typedef enum ltq_dtype { LTQ_F32 = 0, LTQ_F16 = 1, LTQ_BF16 = 2 } ltq_dtype;
+
 /* Epilogue flags (bit-or). */
 #define LTQ_FLAG_RELU 1u     /* acc = max(acc,0) before scaling; no counterpart in the reference (its relu is float-only) */
 #define LTQ_FLAG_SATURATE 2u /* U8 cast clamps to [0,255]. Default (flag clear) reproduces the reference build's cast:
@@ -120,6 +123,27 @@ int ltq_row_sums_u8(const uint8_t *m_dev, uint64_t rows, uint64_t cols, int32_t 
  * part_row_bytes = (N / parts) * sizeof(element). */
 int ltq_interleave_column_blocks(const void *gathered_dev, void *out_dev, uint64_t parts, uint64_t M,
                                  uint64_t part_row_bytes, int device, void *stream);
+
+/* ---- parameters per token and per channel ------------------------------------------------------------------------
+ * The reference keeps one QuantizationParams per tensor (l-ten/layers.h:89-91).  The operators of this section and the two
+ * below keep one per matrix row instead: per token for activations, per output channel for weights, in the same uint8 codes
+ * and ltq_qparams, real = scale * (q - zero_point).  No counterpart in the reference. */
+
+/* GetMinMax + ComputeQuantizationParams + Quantize of every row on its own, in one pass: x_dev [tokens, features] of type
+ * x_dtype, rows ld_x elements apart -> q_dev uint8 [tokens, features] (dense), qp_dev [tokens] and, unless NULL, sums_dev
+ * int32 [tokens], the code sums that ltq_layer_forward_tokens needs.  Codes and parameters of a row are what the three
+ * per-tensor calls give for it.  Where those are undefined: a range below 255 * 2^-126 (a row of zeros) gets the scale
+ * 2^-126; a range that overflows gets max / 255 - min / 255; a row that holds an infinity or a NaN gets the scale NaN, zero
+ * point 0 and codes 0, so that what is computed from that token is NaN and other tokens are not touched.
+ * features <= 2^31 - 1. */
+int ltq_quantize_tokens_u8(const void *x_dev, int x_dtype, uint64_t tokens, uint64_t features, uint64_t ld_x, uint8_t *q_dev,
+                           ltq_qparams *qp_dev, int32_t *sums_dev, int device, void *stream);
+
+/* Its inverse: x_dev[i][k] = scale_i * (q[i][k] - zero_point_i), rounded to x_dtype; q_dev dense, x_dev rows ld_x apart.
+ * Also reads any other array of rows with parameters of their own, e.g. the codes of an ltq_kv_cache, whose rows are (block,
+ * head) pairs of block_tokens * head_dim codes. */
+int ltq_dequantize_tokens_u8(void *x_dev, int x_dtype, uint64_t ld_x, const uint8_t *q_dev, const ltq_qparams *qp_dev, uint64_t tokens,
+                             uint64_t features, int device, void *stream);
 
 /* ---- the reference kernel call, argument for argument ---------------------------------------------------------- */
 
@@ -219,6 +243,28 @@ int ltq_layer_set_clear_on_forward(ltq_layer *layer, int32_t *array_dev, uint64_
  * records next's weight pointer and shape as they are NOW; set it again after rebinding next's weights, and clear it
  * (next = NULL) before those weights are freed.  Both layers must be on the same device. */
 int ltq_layer_set_next(ltq_layer *layer, const ltq_layer *next);
+
+/* Parameters per output channel for the layer's weights: qp_channels_dev [out_features] (device; the layer borrows it) and an
+ * optional float bias [out_features].  Call after ltq_layer_set_weights (whose int32 bias and ltq_layer_set_qparams play no
+ * part in the two calls below) and again after every later ltq_layer_set_weights.  in_features <= 33025, so that no
+ * parameters can overflow the 32-bit sum: LTQ_ERR_UNSUPPORTED beyond.  When in_features is not a multiple of 16 the layer
+ * makes a padded copy of the weights here.  Synchronises `stream`; not for use inside a capture. */
+int ltq_layer_set_channel_qparams(ltq_layer *layer, const ltq_qparams *qp_channels_dev, const float *bias_dev, void *stream);
+
+/* Matrix product of 8-bit codes with parameters for each token and each channel:
+ *   out[i, j] = float(sum_k (x[i,k] - z_i) (w[j,k] - z_j)) * s_i * s_j (+ bias[j]), LTQ_FLAG_RELU on request,
+ * the sum exact, each float step rounded, the result rounded to out_dtype.  x_dev uint8 [M, in_features] (dense),
+ * qp_tokens_dev and asum_dev [M] as ltq_quantize_tokens_u8 leaves them, out_dev rows ld_out elements apart.  A scale of NaN
+ * makes its row (or column) NaN.  Nothing is allocated; may be captured.  LTQ_FLAG_FORCE_* as in ltq_layer_forward. */
+int ltq_layer_forward_tokens(ltq_layer *layer, const uint8_t *x_dev, const ltq_qparams *qp_tokens_dev, const int32_t *asum_dev, uint64_t M,
+                             int out_dtype, unsigned flags, void *out_dev, uint64_t ld_out, void *stream);
+
+/* ltq_quantize_tokens_u8 and the product in one call: x_dev [M, in_features] of x_dtype, rows ld_x elements apart.  The codes
+ * pass through workspace_dev, 16-byte aligned, of at least ltq_layer_float_workspace(layer, M) bytes; its contents mean
+ * nothing before or after the call.  Calls that may overlap on the GPU need workspaces of their own. */
+uint64_t ltq_layer_float_workspace(const ltq_layer *layer, uint64_t M);
+int ltq_layer_forward_float(ltq_layer *layer, const void *x_dev, int x_dtype, uint64_t ld_x, uint64_t M, int out_dtype, unsigned flags,
+                            void *out_dev, uint64_t ld_out, void *workspace_dev, uint64_t workspace_bytes, void *stream);
 
 /* ltq_layer_forward with the result written into several buffers at once, each holding rows of ld_out elements, at
  * column col_offset: element (i, j) of this layer's output goes to dests[d][i * ld_out + col_offset + j] for every d.
@@ -338,6 +384,59 @@ int ltq_comm_set_backend(const ltq_comm_backend *backend);
  * kernel ran out since the last check.  Synchronises `stream`. */
 int ltq_layer_check(ltq_layer *layer, void *stream);
 
+/* ---- keys and values of an attention layer in 8 bits ----------------------------------------------------------------
+ * A paged cache: K and V as uint8 codes [blocks][kv_heads][block_tokens][head_dim], each with one ltq_qparams per block and
+ * head [blocks][kv_heads].  The arrays are the caller's (16-byte aligned; the parameters 8-byte aligned); a block id names
+ * the same slot of all four.  block_tokens 16, 32, 64 or 128; head_dim 32, 64, 96, 128, 192 or 256.  No counterpart in the
+ * reference.
+ *
+ * Both calls below take a batch of `seqs` sequences described on the device, so that a captured call follows the values
+ * that these arrays hold when it is replayed:
+ *   lengths_dev int32 [seqs]      tokens of the sequence in all, those of this call included
+ *   offsets_dev int32 [seqs + 1]  sequence b's tokens of this call are rows offsets[b] .. offsets[b+1] - 1 of the row arrays
+ *   table_dev int32 [seqs][table_width]  block ids in the order of their tokens; token p is in block table[b][p / block_tokens]
+ *   max_new                       host bound on offsets[b+1] - offsets[b] (sizes the launch)
+ * The n tokens of this call are the sequence's last n: positions lengths[b] - n .. lengths[b] - 1.  Tokens whose position
+ * is negative (padding in front of a short sequence) are not stored, and their attention output is zero.  A sequence
+ * that contradicts the bounds (offsets that fall or leave [0, tokens], more than max_new tokens, a negative length or one beyond
+ * table_width * block_tokens) is left out - nothing stored, its output rows left as they were - and so is a block whose id
+ * is not in [0, blocks): its tokens are not stored and not attended to.  Either is reported by the next ltq_device_check as
+ * LTQ_ERR_INVALID_ARG. */
+typedef struct ltq_kv_cache {
+    uint8_t *k_dev;
+    ltq_qparams *k_qp_dev;
+    uint8_t *v_dev;
+    ltq_qparams *v_qp_dev;
+    uint64_t blocks;
+    uint32_t kv_heads;
+    uint32_t block_tokens;
+    uint32_t head_dim;
+} ltq_kv_cache;
+
+/* Quantises new keys and values into the cache.  k_dev, v_dev [tokens][kv_heads][head_dim] of `dtype`, tokens ld elements apart.
+ * The zero point is 128 throughout.  In a block that gets its first tokens, scale = max|x| / 127 over the block's new
+ * tokens of that head (at least 2^-126); in a block that already holds some, the scale grows to that where it is larger, and
+ * the codes already there become Quantize(Dequantize(code)) under the new scale.  An infinity or a NaN among the new values
+ * makes the block's scale NaN, for good.  Slots behind the last token keep their bytes.  Appending the same tokens again
+ * changes nothing.  Two sequences of one call must not append to the same block. */
+int ltq_cache_append(const ltq_kv_cache *cache, const void *k_dev, const void *v_dev, int dtype, uint64_t ld, uint64_t tokens,
+                     const int32_t *offsets_dev, const int32_t *lengths_dev, const int32_t *table_dev, uint64_t seqs, uint64_t table_width,
+                     uint64_t max_new, int device, void *stream);
+
+/* Causal attention of the new tokens over the cache (which holds them already): the token at position p attends positions
+ * 0 .. p of its sequence,  out = sum_j softmax_j(scale * q . k_j) v_j  over the dequantised keys and values.
+ * q_dev [tokens][q_heads][head_dim] of `dtype`, tokens ld_q elements apart; query head h reads key/value head
+ * h / (q_heads / kv_heads).  out_dev [tokens][q_heads][head_dim], same type, dense.  One token per sequence and many take the
+ * same call.  workspace_dev: 16-byte aligned, ltq_cache_attention_workspace bytes, contents meaningless before and after;
+ * calls that may overlap on the GPU need workspaces of their own.  q is taken to 22 significant bits (relative to its row's
+ * largest entry) and the probabilities to 11 bits - 22 for float output; sums are held in float. */
+uint64_t ltq_cache_attention_workspace(const ltq_kv_cache *cache, uint64_t tokens, uint32_t q_heads, uint64_t seqs, uint64_t table_width,
+                                       uint64_t max_new, int device);
+int ltq_cache_attention(const ltq_kv_cache *cache, const void *q_dev, int dtype, uint64_t ld_q, uint64_t tokens, uint32_t q_heads,
+                        const int32_t *offsets_dev, const int32_t *lengths_dev, const int32_t *table_dev, uint64_t seqs,
+                        uint64_t table_width, uint64_t max_new, float scale, void *out_dev, void *workspace_dev, uint64_t workspace_bytes,
+                        int device, void *stream);
+
 /* ---- quantized convolution: Conv2d_q (l-ten/layers.h:453-524, l-ten/conv2d.cpp:238-379) -------------------------
  * The reference runs this layer on the CPU only ("Conv2d_q only supports the CPU device type", conv2d.cpp:371); here
  * it is an im2col pass over the whole batch followed by one GEMM per image on the kernels of the linear path. */
@@ -388,7 +487,8 @@ int ltq_im2col_t_u8(const uint8_t *im_dev, uint64_t batches, uint64_t channels, 
                     uint64_t kernel_h, uint64_t kernel_w, uint64_t pad_h, uint64_t pad_w, uint64_t stride_h,
                     uint64_t stride_w, uint8_t *col_t_dev, uint64_t row_pitch, int device, void *stream);
 
-/* Same check for a device without a layer at hand (the stateless entry points share the device's status word). */
+/* Same check for a device without a layer at hand (the stateless entry points share the device's status word).
+ * LTQ_ERR_INVALID_ARG: a cache call met a sequence or block id outside its bounds since the last check. */
 int ltq_device_check(int device, void *stream);
 
 /* Failure-path self-test, no counterpart in the reference: launches one warp that waits on a barrier nothing will

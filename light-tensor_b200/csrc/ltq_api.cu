@@ -14,6 +14,7 @@
 #include "ltq_gemv.cuh"
 #include "ltq_conv_direct.cuh"
 #include "ltq_layer.cuh"
+#include "ltq_tokens.cuh"
 
 namespace ltq {
 
@@ -52,7 +53,8 @@ using DeviceState = GemmDevice;
 DeviceState g_dev[MAX_DEVICES] = {};
 std::mutex g_dev_mu;
 
-// Per-device constants and the status word, created on first use with that device current.
+}  // namespace
+
 int device_state(int device, DeviceState **out)
 {
     LTQ_REQUIRE(device >= 0 && device < MAX_DEVICES, LTQ_ERR_INVALID_ARG, "device index %d out of range", device);
@@ -74,6 +76,8 @@ int device_state(int device, DeviceState **out)
     *out = &d;
     return LTQ_OK;
 }
+
+namespace {
 
 enum Path { PATH_SIMT, PATH_TC, PATH_SKINNY };
 
@@ -212,6 +216,44 @@ int ltq_row_sums_u8(const uint8_t *m_dev, uint64_t rows, uint64_t cols, int32_t 
     if (rows == 0) return LTQ_OK;
     LTQ_ENTER_DEVICE(device);
     LTQ_CUDA_TRY(launch_row_sums(m_dev, rows, cols, sums_dev, (cudaStream_t)stream));
+    return LTQ_OK;
+}
+
+int ltq_quantize_tokens_u8(const void *x_dev, int x_dtype, uint64_t tokens, uint64_t features, uint64_t ld_x, uint8_t *q_dev,
+                           ltq_qparams *qp_dev, int32_t *sums_dev, int device, void *stream)
+{
+    LTQ_REQUIRE(x_dev && q_dev && qp_dev, LTQ_ERR_INVALID_ARG, "Invalid argument");
+    LTQ_REQUIRE(dtype_ok(x_dtype), LTQ_ERR_INVALID_ARG, "unknown element type %d", x_dtype);
+    LTQ_REQUIRE(features >= 1 && (ld_x >= features || tokens <= 1), LTQ_ERR_INVALID_ARG, "rows of %llu elements cannot be %llu apart",
+                (unsigned long long)features, (unsigned long long)ld_x);
+    LTQ_REQUIRE(features < (1ull << 31), LTQ_ERR_TOO_LARGE, "features must be below 2^31");
+    LTQ_REQUIRE(((uintptr_t)x_dev % dtype_size(x_dtype)) == 0 && ((uintptr_t)qp_dev & 3) == 0 && ((uintptr_t)sums_dev & 3) == 0,
+                LTQ_ERR_INVALID_ARG, "misaligned array");
+    if (tokens == 0) return LTQ_OK;
+    LTQ_ENTER_DEVICE(device);
+    DeviceState *dev;
+    int rc = device_state(device, &dev);
+    if (rc != LTQ_OK) return rc;
+    LTQ_CUDA_TRY(launch_quantize_tokens(x_dev, x_dtype, tokens, features, ld_x, q_dev, features, qp_dev, sums_dev, dev->sms,
+                                        (cudaStream_t)stream));
+    return LTQ_OK;
+}
+
+int ltq_dequantize_tokens_u8(void *x_dev, int x_dtype, uint64_t ld_x, const uint8_t *q_dev, const ltq_qparams *qp_dev, uint64_t tokens,
+                             uint64_t features, int device, void *stream)
+{
+    LTQ_REQUIRE(x_dev && q_dev && qp_dev, LTQ_ERR_INVALID_ARG, "Invalid argument");
+    LTQ_REQUIRE(dtype_ok(x_dtype), LTQ_ERR_INVALID_ARG, "unknown element type %d", x_dtype);
+    LTQ_REQUIRE(features >= 1 && (ld_x >= features || tokens <= 1), LTQ_ERR_INVALID_ARG, "rows of %llu elements cannot be %llu apart",
+                (unsigned long long)features, (unsigned long long)ld_x);
+    LTQ_REQUIRE(features < (1ull << 31), LTQ_ERR_TOO_LARGE, "features must be below 2^31");
+    LTQ_REQUIRE(((uintptr_t)x_dev % dtype_size(x_dtype)) == 0 && ((uintptr_t)qp_dev & 3) == 0, LTQ_ERR_INVALID_ARG, "misaligned array");
+    if (tokens == 0) return LTQ_OK;
+    LTQ_ENTER_DEVICE(device);
+    DeviceState *dev;
+    int rc = device_state(device, &dev);
+    if (rc != LTQ_OK) return rc;
+    LTQ_CUDA_TRY(launch_dequantize_tokens(x_dev, x_dtype, ld_x, q_dev, qp_dev, tokens, features, dev->sms, (cudaStream_t)stream));
     return LTQ_OK;
 }
 
@@ -384,6 +426,7 @@ int ltq_layer_destroy(ltq_layer *layer)
     LTQ_ENTER_DEVICE(layer->device);
     cudaFree(layer->wsum);
     cudaFree(layer->asum_ws);
+    cudaFree(layer->w_pad);
     delete layer;
     return LTQ_OK;
 }
@@ -394,6 +437,7 @@ int ltq_layer_set_weights(ltq_layer *layer, const uint8_t *w_dev, const int32_t 
     LTQ_ENTER_DEVICE(layer->device);
     layer->w = w_dev;
     layer->bias = bias_dev;
+    layer->qp_channels = nullptr;   // parameters per channel belong to the weights they were given for
     for (auto &m : layer->map_w) m = TcOperandMap();
     layer->map_w_gemv = GemvWeightMaps();
     LTQ_CUDA_TRY(launch_row_sums(w_dev, layer->N, layer->K, layer->wsum, (cudaStream_t)stream));
@@ -498,6 +542,99 @@ int ltq_layer_forward(ltq_layer *layer, const uint8_t *x_dev, const int32_t *asu
     LTQ_REQUIRE(out_dev, LTQ_ERR_INVALID_ARG, "Invalid argument");
     void *dests[1] = {out_dev};
     return layer_forward_impl(layer, x_dev, asum_dev, M, qp_in_dev, out_mode, flags, dests, 1, 0, 0, stream);
+}
+
+// ---- parameters per token and channel -----------------------------------------------------------------------------------
+int ltq_layer_set_channel_qparams(ltq_layer *layer, const ltq_qparams *qp_channels_dev, const float *bias_dev, void *stream)
+{
+    LTQ_REQUIRE(layer && qp_channels_dev, LTQ_ERR_INVALID_ARG, "Invalid argument");
+    LTQ_REQUIRE(layer->w, LTQ_ERR_INVALID_ARG, "ltq_layer_set_weights has not been called");
+    LTQ_REQUIRE(layer->K <= TOKENS_MAX_K, LTQ_ERR_UNSUPPORTED, "%llu input features: above %llu a sum of products may not fit 32 bits",
+                (unsigned long long)layer->K, (unsigned long long)TOKENS_MAX_K);
+    LTQ_REQUIRE(((uintptr_t)qp_channels_dev & 3) == 0 && ((uintptr_t)bias_dev & 3) == 0, LTQ_ERR_INVALID_ARG, "misaligned array");
+    LTQ_ENTER_DEVICE(layer->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    const uint64_t Kp = layer->padded_k();
+    if (Kp != layer->K) {
+        if (!layer->w_pad) {
+            cudaError_t e = cudaMalloc(&layer->w_pad, layer->N * Kp);
+            if (e != cudaSuccess) {
+                layer->w_pad = nullptr;
+                set_error("cudaMalloc of %llu bytes of padded weights failed: %s", (unsigned long long)(layer->N * Kp), cudaGetErrorString(e));
+                return LTQ_ERR_NO_MEMORY;
+            }
+        }
+        LTQ_CUDA_TRY(cudaMemsetAsync(layer->w_pad, 0, layer->N * Kp, st));
+        LTQ_CUDA_TRY(cudaMemcpy2DAsync(layer->w_pad, Kp, layer->w, layer->K, layer->K, layer->N, cudaMemcpyDeviceToDevice, st));
+    }
+    LTQ_CUDA_TRY(cudaStreamSynchronize(st));
+    layer->qp_channels = qp_channels_dev;
+    layer->fbias = bias_dev;
+    return LTQ_OK;
+}
+
+// Shared by the two forwards: x uint8 rows of Kx bytes (in_features, or the padded length with the padded weights).
+static int layer_product_tokens(ltq_layer *layer, const uint8_t *x, uint64_t Kx, const ltq_qparams *qp, const int32_t *asum, uint64_t M,
+                                int out_dtype, unsigned flags, void *out, uint64_t ld_out, cudaStream_t st)
+{
+    Epilogue epi = make_epilogue(layer->wsum, asum, nullptr, ltq_qparams{1.f, 0}, ltq_qparams{1.f, 0}, ltq_qparams{1.f, 0}, layer->K,
+                                 OUT_TOKENS + out_dtype, flags);
+    epi.qp_rows = qp;
+    epi.qp_cols = layer->qp_channels;
+    epi.fbias = layer->fbias;
+    epi.ldc = ld_out;
+    return run_fc_gemm(*layer->dev, M, layer->N, Kx, x, Kx == layer->K ? layer->w : layer->w_pad, epi, out, flags, layer, st);
+}
+
+static int check_tokens_call(const ltq_layer *layer, uint64_t M, int out_dtype, const void *out_dev, uint64_t ld_out)
+{
+    LTQ_REQUIRE(layer->w, LTQ_ERR_INVALID_ARG, "ltq_layer_set_weights has not been called");
+    LTQ_REQUIRE(layer->qp_channels, LTQ_ERR_INVALID_ARG, "ltq_layer_set_channel_qparams has not been called for these weights");
+    LTQ_REQUIRE(dtype_ok(out_dtype), LTQ_ERR_INVALID_ARG, "unknown element type %d", out_dtype);
+    LTQ_REQUIRE(M < (1ull << 31), LTQ_ERR_TOO_LARGE, "M must be below 2^31");
+    LTQ_REQUIRE(ld_out >= layer->N && ld_out < (1ull << 40), LTQ_ERR_INVALID_ARG, "rows of %llu elements cannot be %llu apart",
+                (unsigned long long)layer->N, (unsigned long long)ld_out);
+    LTQ_REQUIRE(((uintptr_t)out_dev % dtype_size(out_dtype)) == 0, LTQ_ERR_INVALID_ARG, "misaligned array");
+    return LTQ_OK;
+}
+
+int ltq_layer_forward_tokens(ltq_layer *layer, const uint8_t *x_dev, const ltq_qparams *qp_tokens_dev, const int32_t *asum_dev, uint64_t M,
+                             int out_dtype, unsigned flags, void *out_dev, uint64_t ld_out, void *stream)
+{
+    LTQ_REQUIRE(layer && x_dev && qp_tokens_dev && asum_dev && out_dev, LTQ_ERR_INVALID_ARG, "Invalid argument");
+    LTQ_REQUIRE(((uintptr_t)qp_tokens_dev & 3) == 0 && ((uintptr_t)asum_dev & 3) == 0, LTQ_ERR_INVALID_ARG, "misaligned array");
+    int rc = check_tokens_call(layer, M, out_dtype, out_dev, ld_out);
+    if (rc != LTQ_OK || M == 0) return rc;
+    LTQ_ENTER_DEVICE(layer->device);
+    return layer_product_tokens(layer, x_dev, layer->K, qp_tokens_dev, asum_dev, M, out_dtype, flags, out_dev, ld_out, (cudaStream_t)stream);
+}
+
+// Workspace of the float form: codes [M, padded K], parameters [M], sums [M].
+uint64_t ltq_layer_float_workspace(const ltq_layer *layer, uint64_t M)
+{
+    return layer ? M * (layer->padded_k() + sizeof(ltq_qparams) + sizeof(int32_t)) : 0;
+}
+
+int ltq_layer_forward_float(ltq_layer *layer, const void *x_dev, int x_dtype, uint64_t ld_x, uint64_t M, int out_dtype, unsigned flags,
+                            void *out_dev, uint64_t ld_out, void *workspace_dev, uint64_t workspace_bytes, void *stream)
+{
+    LTQ_REQUIRE(layer && (M == 0 || (x_dev && out_dev && workspace_dev)), LTQ_ERR_INVALID_ARG, "Invalid argument");
+    int rc = check_tokens_call(layer, M, out_dtype, out_dev, ld_out);
+    if (rc != LTQ_OK || M == 0) return rc;
+    LTQ_REQUIRE(dtype_ok(x_dtype), LTQ_ERR_INVALID_ARG, "unknown element type %d", x_dtype);
+    LTQ_REQUIRE(ld_x >= layer->K || M <= 1, LTQ_ERR_INVALID_ARG, "rows of %llu elements cannot be %llu apart", (unsigned long long)layer->K,
+                (unsigned long long)ld_x);
+    LTQ_REQUIRE(((uintptr_t)x_dev % dtype_size(x_dtype)) == 0 && ((uintptr_t)workspace_dev & 15) == 0, LTQ_ERR_INVALID_ARG, "misaligned array");
+    LTQ_REQUIRE(workspace_bytes >= ltq_layer_float_workspace(layer, M), LTQ_ERR_INVALID_ARG, "the workspace holds %llu bytes, %llu are needed",
+                (unsigned long long)workspace_bytes, (unsigned long long)ltq_layer_float_workspace(layer, M));
+    LTQ_ENTER_DEVICE(layer->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    const uint64_t Kp = layer->padded_k();
+    uint8_t *q = static_cast<uint8_t *>(workspace_dev);
+    ltq_qparams *qp = reinterpret_cast<ltq_qparams *>(q + M * Kp);
+    int32_t *asum = reinterpret_cast<int32_t *>(qp + M);
+    LTQ_CUDA_TRY(launch_quantize_tokens(x_dev, x_dtype, M, layer->K, ld_x, q, Kp, qp, asum, layer->dev->sms, st));
+    return layer_product_tokens(layer, q, Kp, qp, asum, M, out_dtype, flags, out_dev, ld_out, st);
 }
 
 int ltq_layer_forward_scatter(ltq_layer *layer, const uint8_t *x_dev, const int32_t *asum_dev, uint64_t M,
@@ -850,6 +987,11 @@ int ltq_device_check(int device, void *stream)
     LTQ_CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
     if (code) {
         LTQ_CUDA_TRY(cudaMemsetAsync(dev->status, 0, sizeof code, (cudaStream_t)stream));
+        if (code == STATUS_BAD_SEQUENCE || code == STATUS_BAD_BLOCK) {
+            set_error(code == STATUS_BAD_BLOCK ? "a cache call met a block id outside the cache"
+                                               : "a cache call met a sequence whose offsets or length contradict its bounds");
+            return LTQ_ERR_INVALID_ARG;
+        }
         set_error("a bounded device-side wait expired (code 0x%x: role %u, slot %u)", code, code >> 8, code & 0xFF);
         return LTQ_ERR_DEVICE_TIMEOUT;
     }

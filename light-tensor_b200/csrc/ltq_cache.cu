@@ -1,0 +1,291 @@
+// The 8-bit key/value cache: entry points (include/ltq.h) and the kernel that appends to it.  The attention kernels are in
+// ltq_cache_attention.cuh.
+#include "ltq_cache.cuh"
+#include "ltq_ptx.cuh"
+#include "ltq_quant.cuh"
+
+namespace ltq {
+
+namespace {
+
+constexpr int APPEND_THREADS = 128;
+constexpr float SMALLEST_SCALE = 1.17549435e-38f;   // 2^-126
+
+// Four neighbouring elements as floats.
+template <int DT>
+__device__ __forceinline__ float4 load4(const void *base, uint64_t at, bool vec)
+{
+    if (DT == LTQ_F32) {
+        const float *p = static_cast<const float *>(base) + at;
+        if (vec) return __ldg(reinterpret_cast<const float4 *>(p));
+        return make_float4(p[0], p[1], p[2], p[3]);
+    }
+    const uint16_t *p = static_cast<const uint16_t *>(base) + at;
+    uint32_t a, b;
+    if (vec) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
+        a = v.x;
+        b = v.y;
+    } else {
+        a = (uint32_t)p[0] | (uint32_t)p[1] << 16;
+        b = (uint32_t)p[2] | (uint32_t)p[3] << 16;
+    }
+    if (DT == LTQ_F16) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&a)), y = __half22float2(*reinterpret_cast<const __half2 *>(&b));
+        return make_float4(x.x, x.y, y.x, y.y);
+    }
+    return make_float4(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u), __uint_as_float(b << 16), __uint_as_float(b & 0xFFFF0000u));
+}
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+}  // namespace
+
+// One CTA per (block that a sequence touches, head, K or V): the largest magnitude of the block's new tokens fixes its scale,
+// older codes of the block follow if the scale grew, the new codes are written.  Bound by HBM at large sizes (element + 1
+// bytes per value; the second look at the new tokens hits L1 / L2), by launch latency for one token per sequence.
+// Grid: (2 * blocks per sequence, kv_heads, sequences).
+template <int DT>
+__global__ void __launch_bounds__(APPEND_THREADS)
+cache_append_kernel(const ltq_kv_cache cache, const CacheBatch bt, const void *__restrict__ k, const void *__restrict__ v, uint64_t ld, bool vec)
+{
+    griddep_launch_dependents();
+    griddep_wait();
+    const CacheSeq s = cache_seq(bt, blockIdx.z);
+    if (!s.ok || s.n == 0) return;
+    const bool is_v = blockIdx.x & 1;
+    const int bt_tokens = 1 << bt.log2_bt, start = s.len - s.n < 0 ? 0 : s.len - s.n;   // first position that is stored
+    const int64_t blk = (int64_t)(start >> bt.log2_bt) + (blockIdx.x >> 1);
+    const int64_t first = blk << bt.log2_bt;                                              // the block's first position
+    if (first >= s.len) return;
+    const int used = first >= start ? 0 : (int)(start - first);                           // tokens it holds already
+    const int end = s.len - first < bt_tokens ? (int)(s.len - first) : bt_tokens;
+    const int32_t page = bt.table[(uint64_t)blockIdx.z * bt.table_width + blk];
+    if ((uint32_t)page >= cache.blocks) {
+        if (threadIdx.x == 0) atomicCAS(bt.status, 0u, STATUS_BAD_BLOCK);
+        return;
+    }
+    const uint32_t D = cache.head_dim, h = blockIdx.y, per = D / 4;
+    const uint64_t slot = (uint64_t)(uint32_t)page * cache.kv_heads + h;
+    uint32_t *codes = reinterpret_cast<uint32_t *>((is_v ? cache.v_dev : cache.k_dev) + (slot << bt.log2_bt) * D);
+    ltq_qparams *qp = (is_v ? cache.v_qp_dev : cache.k_qp_dev) + slot;
+    const void *src = is_v ? v : k;
+    // row of the block's token i: the sequence's row of position p is off + p - (len - n)
+    const uint64_t row0 = (uint64_t)((int64_t)s.off + first - (s.len - s.n));
+    const uint32_t chunks = (uint32_t)(end - used) * per;
+
+    float most = 0.f;
+    for (uint32_t i = threadIdx.x; i < chunks; i += APPEND_THREADS) {
+        const uint32_t t = i / per, d = (i - t * per) * 4;
+        const float4 x = load4<DT>(src, (row0 + used + t) * ld + (uint64_t)h * D + d, vec);
+        most = max_nan(max_nan(most, max_nan(fabsf(x.x), fabsf(x.y))), max_nan(fabsf(x.z), fabsf(x.w)));
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+    __shared__ float s_most[APPEND_THREADS / 32];
+    if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
+    const float old = used ? qp->scale : 0.f;
+    __syncthreads();   // (also: everyone has read the old scale)
+#pragma unroll
+    for (int w = 0; w < APPEND_THREADS / 32; w++) most = max_nan(most, s_most[w]);
+    float scale = max_nan(fmaxf(__fdiv_rn(most, 127.f), SMALLEST_SCALE), old);
+    const bool finite = most < INFINITY && scale < INFINITY;   // false for NaN, a NaN that the block had before included
+    if (threadIdx.x == 0) {
+        const float stored = finite ? scale : __int_as_float(0x7FC00000);
+        if (((uintptr_t)qp & 7) == 0) *reinterpret_cast<uint2 *>(qp) = make_uint2(__float_as_uint(stored), 128u);
+    }
+    const float inv = quant_screen_inv(scale);
+    if (finite && used && scale > old) {
+        for (uint32_t i = threadIdx.x; i < (uint32_t)used * per; i += APPEND_THREADS) {
+            const uint32_t w = codes[i];
+            const float4 x = make_float4(__fmul_rn(old, (float)((int)(w & 0xFF) - 128)), __fmul_rn(old, (float)((int)((w >> 8) & 0xFF) - 128)),
+                                         __fmul_rn(old, (float)((int)((w >> 16) & 0xFF) - 128)), __fmul_rn(old, (float)((int)(w >> 24) - 128)));
+            codes[i] = quant4_u8(x, scale, 128.f, inv);
+        }
+    }
+    for (uint32_t i = threadIdx.x; i < chunks; i += APPEND_THREADS) {
+        const uint32_t t = i / per, d = (i - t * per) * 4;
+        uint32_t w = 0x80808080u;
+        if (finite) w = quant4_u8(load4<DT>(src, (row0 + used + t) * ld + (uint64_t)h * D + d, vec), scale, 128.f, inv);
+        codes[(uint32_t)used * per + i] = w;
+    }
+}
+
+cudaError_t launch_cache_append(const ltq_kv_cache &c, const CacheBatch &bt, const void *k, const void *v, int dtype, uint64_t ld,
+                                cudaStream_t stream)
+{
+    // n tokens from any offset touch at most (n + block_tokens - 2) / block_tokens + 1 blocks
+    const uint32_t bt_tokens = 1u << bt.log2_bt, blocks = (bt.max_new + bt_tokens - 2) / bt_tokens + 1;
+    const dim3 grid(2 * blocks, c.kv_heads, bt.seqs);
+    const uint64_t e4 = 4 * dtype_size(dtype);
+    const bool vec = ld % 4 == 0 && (((uintptr_t)k | (uintptr_t)v) % e4) == 0;
+    count_launch();
+    if (dtype == LTQ_F32) return launch_chained(cache_append_kernel<LTQ_F32>, grid, dim3(APPEND_THREADS), 0, stream, c, bt, k, v, ld, vec);
+    if (dtype == LTQ_F16) return launch_chained(cache_append_kernel<LTQ_F16>, grid, dim3(APPEND_THREADS), 0, stream, c, bt, k, v, ld, vec);
+    return launch_chained(cache_append_kernel<LTQ_BF16>, grid, dim3(APPEND_THREADS), 0, stream, c, bt, k, v, ld, vec);
+}
+
+uint32_t attn_rows_per_tile(int dtype, uint32_t head_dim, uint64_t rows)
+{
+    // sixteen rows share the conversion of the keys where the registers allow it
+    return rows > 8 && head_dim * (dtype == LTQ_F32 ? 2 : 1) <= 128 ? 16 : 8;
+}
+
+namespace {
+
+// CTAs that share one sequence's keys: enough to fill the device (about three CTAs fit an SM), but none with less than
+// four 16-key steps for each of its warps.
+uint32_t attn_splits(uint32_t kv_heads, uint64_t row_tiles, uint64_t seqs, uint64_t max_keys, int sms)
+{
+    const uint64_t items = kv_heads * row_tiles * seqs, target = (uint64_t)sms * 3, steps = (max_keys + 15) / 16;
+    uint64_t s = (target + items - 1) / items;
+    if (s > steps / 16) s = steps / 16;
+    return (uint32_t)(s < 1 ? 1 : (s > 64 ? 64 : s));
+}
+
+int check_cache(const ltq_kv_cache *c)
+{
+    LTQ_REQUIRE(c && c->k_dev && c->v_dev && c->k_qp_dev && c->v_qp_dev, LTQ_ERR_INVALID_ARG, "Invalid argument");
+    LTQ_REQUIRE(c->blocks >= 1 && c->blocks < (1ull << 31) && c->kv_heads >= 1 && c->kv_heads <= 65535, LTQ_ERR_INVALID_ARG,
+                "a cache of %llu blocks with %u heads", (unsigned long long)c->blocks, c->kv_heads);
+    LTQ_REQUIRE(c->block_tokens == 16 || c->block_tokens == 32 || c->block_tokens == 64 || c->block_tokens == 128, LTQ_ERR_UNSUPPORTED,
+                "block_tokens must be 16, 32, 64 or 128, not %u", c->block_tokens);
+    const uint32_t d = c->head_dim;
+    LTQ_REQUIRE(d == 32 || d == 64 || d == 96 || d == 128 || d == 192 || d == 256, LTQ_ERR_UNSUPPORTED,
+                "head_dim must be 32, 64, 96, 128, 192 or 256, not %u", d);
+    LTQ_REQUIRE((((uintptr_t)c->k_dev | (uintptr_t)c->v_dev) & 15) == 0 && (((uintptr_t)c->k_qp_dev | (uintptr_t)c->v_qp_dev) & 7) == 0,
+                LTQ_ERR_INVALID_ARG, "misaligned cache arrays");
+    return LTQ_OK;
+}
+
+int check_batch(const ltq_kv_cache *c, const void *offsets, const void *lengths, const void *table, uint64_t tokens, uint64_t seqs,
+                uint64_t table_width, uint64_t max_new)
+{
+    LTQ_REQUIRE(offsets && lengths && (table || table_width == 0), LTQ_ERR_INVALID_ARG, "Invalid argument");
+    LTQ_REQUIRE((((uintptr_t)offsets | (uintptr_t)lengths | (uintptr_t)table) & 3) == 0, LTQ_ERR_INVALID_ARG, "misaligned array");
+    LTQ_REQUIRE(seqs <= 65535, LTQ_ERR_TOO_LARGE, "%llu sequences: at most 65535", (unsigned long long)seqs);
+    LTQ_REQUIRE(tokens < (1ull << 31) && max_new <= tokens && table_width * c->block_tokens < (1ull << 31), LTQ_ERR_INVALID_ARG,
+                "%llu tokens, at most %llu per sequence, tables of %llu blocks", (unsigned long long)tokens, (unsigned long long)max_new,
+                (unsigned long long)table_width);
+    return LTQ_OK;
+}
+
+CacheBatch make_batch(const ltq_kv_cache *c, const int32_t *offsets, const int32_t *lengths, const int32_t *table, uint64_t tokens,
+                      uint64_t seqs, uint64_t table_width, uint64_t max_new, uint32_t *status)
+{
+    CacheBatch bt;
+    bt.offsets = offsets;
+    bt.lengths = lengths;
+    bt.table = table;
+    bt.tokens = tokens;
+    bt.seqs = (uint32_t)seqs;
+    bt.table_width = (uint32_t)table_width;
+    bt.max_new = (uint32_t)max_new;
+    bt.log2_bt = c->block_tokens == 16 ? 4 : (c->block_tokens == 32 ? 5 : (c->block_tokens == 64 ? 6 : 7));
+    bt.status = status;
+    return bt;
+}
+
+uint32_t attn_plan(const ltq_kv_cache *c, int dtype, uint32_t q_heads, uint64_t seqs, uint64_t table_width, uint64_t max_new, int sms)
+{
+    const uint64_t rows = max_new * (q_heads / c->kv_heads), per = attn_rows_per_tile(dtype, c->head_dim, rows);
+    return attn_splits(c->kv_heads, (rows + per - 1) / per, seqs, table_width * c->block_tokens, sms);
+}
+
+}  // namespace
+}  // namespace ltq
+
+using namespace ltq;
+
+extern "C" {
+
+int ltq_cache_append(const ltq_kv_cache *cache, const void *k_dev, const void *v_dev, int dtype, uint64_t ld, uint64_t tokens,
+                     const int32_t *offsets_dev, const int32_t *lengths_dev, const int32_t *table_dev, uint64_t seqs, uint64_t table_width,
+                     uint64_t max_new, int device, void *stream)
+{
+    int rc = check_cache(cache);
+    if (rc != LTQ_OK) return rc;
+    LTQ_REQUIRE(dtype_ok(dtype), LTQ_ERR_INVALID_ARG, "unknown element type %d", dtype);
+    if (tokens == 0 || seqs == 0 || max_new == 0) return LTQ_OK;
+    LTQ_REQUIRE(k_dev && v_dev, LTQ_ERR_INVALID_ARG, "Invalid argument");
+    rc = check_batch(cache, offsets_dev, lengths_dev, table_dev, tokens, seqs, table_width, max_new);
+    if (rc != LTQ_OK) return rc;
+    const uint64_t row = (uint64_t)cache->kv_heads * cache->head_dim;
+    LTQ_REQUIRE(ld >= row && ld < (1ull << 31), LTQ_ERR_INVALID_ARG, "tokens of %llu elements cannot be %llu apart", (unsigned long long)row,
+                (unsigned long long)ld);
+    LTQ_REQUIRE((((uintptr_t)k_dev | (uintptr_t)v_dev) % dtype_size(dtype)) == 0, LTQ_ERR_INVALID_ARG, "misaligned array");
+    LTQ_ENTER_DEVICE(device);
+    GemmDevice *dev;
+    rc = device_state(device, &dev);
+    if (rc != LTQ_OK) return rc;
+    LTQ_CUDA_TRY(launch_cache_append(*cache, make_batch(cache, offsets_dev, lengths_dev, table_dev, tokens, seqs, table_width, max_new, dev->status),
+                                     k_dev, v_dev, dtype, ld, (cudaStream_t)stream));
+    return LTQ_OK;
+}
+
+// Partial results of every split: head_dim sums and {maximum, sum} per row.  The float form has the fewest rows per tile, so its
+// split count, the smallest or equal, is not the bound: take the larger of the two.
+uint64_t ltq_cache_attention_workspace(const ltq_kv_cache *cache, uint64_t tokens, uint32_t q_heads, uint64_t seqs, uint64_t table_width,
+                                       uint64_t max_new, int device)
+{
+    if (check_cache(cache) != LTQ_OK || q_heads == 0 || q_heads % cache->kv_heads != 0 || tokens == 0 || seqs == 0 || max_new == 0) return 0;
+    DeviceGuard guard(device);
+    GemmDevice *dev;
+    if (guard.err != cudaSuccess || device_state(device, &dev) != LTQ_OK) return 0;
+    const uint32_t a = attn_plan(cache, LTQ_F32, q_heads, seqs, table_width, max_new, dev->sms);
+    const uint32_t b = attn_plan(cache, LTQ_BF16, q_heads, seqs, table_width, max_new, dev->sms);
+    const uint64_t s = a > b ? a : b;
+    return s == 1 ? 16 : s * tokens * q_heads * (cache->head_dim + 2) * sizeof(float);
+}
+
+int ltq_cache_attention(const ltq_kv_cache *cache, const void *q_dev, int dtype, uint64_t ld_q, uint64_t tokens, uint32_t q_heads,
+                        const int32_t *offsets_dev, const int32_t *lengths_dev, const int32_t *table_dev, uint64_t seqs,
+                        uint64_t table_width, uint64_t max_new, float scale, void *out_dev, void *workspace_dev, uint64_t workspace_bytes,
+                        int device, void *stream)
+{
+    int rc = check_cache(cache);
+    if (rc != LTQ_OK) return rc;
+    LTQ_REQUIRE(dtype_ok(dtype), LTQ_ERR_INVALID_ARG, "unknown element type %d", dtype);
+    LTQ_REQUIRE(q_heads >= 1 && q_heads % cache->kv_heads == 0 && q_heads / cache->kv_heads <= 1024, LTQ_ERR_INVALID_ARG,
+                "%u query heads do not divide over %u key/value heads", q_heads, cache->kv_heads);
+    if (tokens == 0 || seqs == 0 || max_new == 0) return LTQ_OK;
+    LTQ_REQUIRE(q_dev && out_dev && workspace_dev, LTQ_ERR_INVALID_ARG, "Invalid argument");
+    rc = check_batch(cache, offsets_dev, lengths_dev, table_dev, tokens, seqs, table_width, max_new);
+    if (rc != LTQ_OK) return rc;
+    const uint64_t row = (uint64_t)q_heads * cache->head_dim;
+    LTQ_REQUIRE(ld_q >= row && ld_q < (1ull << 31), LTQ_ERR_INVALID_ARG, "tokens of %llu elements cannot be %llu apart", (unsigned long long)row,
+                (unsigned long long)ld_q);
+    LTQ_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev) % dtype_size(dtype)) == 0 && ((uintptr_t)workspace_dev & 15) == 0, LTQ_ERR_INVALID_ARG,
+                "misaligned array");
+    LTQ_REQUIRE(scale - scale == 0.f, LTQ_ERR_INVALID_ARG, "the softmax scale must be finite");
+    LTQ_REQUIRE(max_new * q_heads < (1ull << 31), LTQ_ERR_TOO_LARGE, "max_new * q_heads must be below 2^31");
+    LTQ_ENTER_DEVICE(device);
+    GemmDevice *dev;
+    rc = device_state(device, &dev);
+    if (rc != LTQ_OK) return rc;
+    AttnArgs a;
+    a.cache = *cache;
+    a.bt = make_batch(cache, offsets_dev, lengths_dev, table_dev, tokens, seqs, table_width, max_new, dev->status);
+    a.q = q_dev;
+    a.out = out_dev;
+    a.ld_q = ld_q;
+    a.q_heads = q_heads;
+    a.group = q_heads / cache->kv_heads;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.splits = attn_plan(cache, dtype, q_heads, seqs, table_width, max_new, dev->sms);
+    const uint64_t rows = a.splits * tokens * q_heads;
+    LTQ_REQUIRE(a.splits == 1 || workspace_bytes >= rows * (cache->head_dim + 2) * sizeof(float), LTQ_ERR_INVALID_ARG,
+                "the workspace holds %llu bytes, %llu are needed", (unsigned long long)workspace_bytes,
+                (unsigned long long)(rows * (cache->head_dim + 2) * sizeof(float)));
+    a.part_o = static_cast<float *>(workspace_dev);
+    a.part_ml = reinterpret_cast<float2 *>(a.part_o + rows * cache->head_dim);
+    cudaStream_t st = (cudaStream_t)stream;
+    LTQ_CUDA_TRY(dtype == LTQ_F32 ? launch_attention_f32(a, st) : (dtype == LTQ_F16 ? launch_attention_f16(a, st) : launch_attention_bf16(a, st)));
+    return LTQ_OK;
+}
+
+}  // extern "C"

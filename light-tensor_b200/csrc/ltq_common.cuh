@@ -17,7 +17,11 @@ extern std::atomic<uint64_t> g_launches;
 inline void count_launch(uint64_t n = 1) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 // Name (with template arguments) of the GEMM kernel the calling thread launched last, for ltq_last_kernel().
 void note_kernel(const char *fmt, ...);
-inline const char *out_mode_name(int out_mode) { return out_mode == LTQ_OUT_U8 ? "u8" : (out_mode == LTQ_OUT_F32 ? "f32" : "i32"); }
+inline const char *out_mode_name(int out_mode)
+{
+    static const char *const names[] = {"u8", "f32", "i32", "tokens-f32", "tokens-f16", "tokens-bf16"};
+    return names[out_mode];
+}
 
 #define LTQ_CUDA_TRY(expr)                                                                                   \
     do {                                                                                                     \
@@ -121,6 +125,10 @@ struct Epilogue {
     // needed).  Nothing in this launch may use that array.
     int32_t *clear_ptr;
     uint32_t clear_count;
+    // Output modes OUT_TOKENS + ltq_dtype (ltq_tokens.cuh): parameters per row of A and per column, float bias per column.
+    const ltq_qparams *qp_rows;   // [M]
+    const ltq_qparams *qp_cols;   // [N]
+    const float *fbias;           // [N] or nullptr
 };
 
 // The epilogue of a plain call: one dense [M, N] destination, no chain hooks.  Callers switch further fields on.
@@ -141,6 +149,9 @@ __host__ __device__ inline Epilogue make_epilogue(const int32_t *bsum, const int
     e.out_rowsum = nullptr;
     e.clear_ptr = nullptr;
     e.clear_count = 0;
+    e.qp_rows = nullptr;
+    e.qp_cols = nullptr;
+    e.fbias = nullptr;
     for (auto &m : e.more_out) m = nullptr;
     e.qpA_dev = nullptr;
     e.sA = qa.scale;
@@ -420,6 +431,10 @@ struct GemmDevice {
     int sms;
     uint32_t *status;
 };
+// Codes of the status word that are not expired waits: what the cache kernels found in their device-side arguments.
+constexpr uint32_t STATUS_BAD_SEQUENCE = 0xA01u, STATUS_BAD_BLOCK = 0xA02u;
+// Per-device constants and the status word, created on first use with that device current.
+int device_state(int device, GemmDevice **out);
 }  // namespace ltq
 struct ltq_layer;
 namespace ltq {

@@ -7,6 +7,7 @@
 // 64x64 output tile per 256-thread CTA, 32-deep K slices staged in shared memory as packed 4-byte K groups, each
 // thread owning a 4x4 register tile (16 dp4a per 8 shared loads).
 #include "ltq_common.cuh"
+#include "ltq_tokens.cuh"
 
 namespace ltq {
 
@@ -70,6 +71,26 @@ __global__ void __launch_bounds__(256) gemm_simt_kernel(bool a_kc, bool b_kc, ui
         __syncthreads();
     }
 
+    if (out_is_tokens(epi.out_mode)) {
+        const bool relu = epi.flags & LTQ_FLAG_RELU;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint64_t row = m0 + ty + 16 * i;
+            if (row >= M) continue;
+            const TokenRow tr = token_row(epi, row);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint64_t col = n0 + tx + 16 * j;
+                if (col >= N) continue;
+                const float y = token_value((uint32_t)acc[i][j], tr, token_col(epi, col), relu);
+                const uint64_t o = row * epilogue_pitch(epi, N) + col;
+                if (epi.out_mode == OUT_TOKENS + LTQ_F32) static_cast<float *>(out)[o] = y;
+                else if (epi.out_mode == OUT_TOKENS + LTQ_F16) static_cast<uint16_t *>(out)[o] = (uint16_t)token_bits<LTQ_F16>(y);
+                else static_cast<uint16_t *>(out)[o] = (uint16_t)token_bits<LTQ_BF16>(y);
+            }
+        }
+        return;
+    }
     const EpilogueConsts c = epilogue_consts(epi);
     const bool relu = epi.flags & LTQ_FLAG_RELU, sat = epi.flags & LTQ_FLAG_SATURATE;
 #pragma unroll

@@ -21,6 +21,7 @@
 #include "ltq_common.cuh"
 #include "ltq_gemm_tc.cuh"
 #include "ltq_tcgen05.cuh"
+#include "ltq_tokens.cuh"
 
 namespace ltq {
 
@@ -31,34 +32,37 @@ constexpr int BK = 128;          // bytes (= elements) of K per smem stage: one 
 constexpr int UMMA_K = 32;       // kind::i8
 constexpr int NUM_THREADS = 192;
 
-template <int BN>
+// Bytes of column terms per output column in shared memory: one correction word, or the 16 bytes of token_col.
+__host__ __device__ constexpr int col_bytes(int out) { return out_is_tokens(out) ? 16 : 4; }
+
+template <int BN, int OUT>
 struct Cfg {
     static constexpr int STAGES = (BN == 256) ? 4 : (BN == 128 ? 6 : 8);
     static constexpr int A_BYTES = BM * BK;
     static constexpr int B_BYTES = BN * BK;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int TMEM_COLS = (2 * BN < 32) ? 32 : 2 * BN;  // power of two >= 32
-    // ring + 1024 B alignment slack + column terms (2 x BN x 4) + barriers
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 2 * BN * 4 + 256;
+    // ring + 1024 B alignment slack + column terms (two tiles) + barriers
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 2 * BN * col_bytes(OUT) + 256;
 };
 
 }  // namespace
 
-// OUT: 0 = uint8, 1 = float, 2 = int32 (ltq_out_mode).
+// OUT: 0 = uint8, 1 = float, 2 = int32 (ltq_out_mode), OUT_TOKENS + ltq_dtype = parameters per token and channel.
 template <int BN, int OUT>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, uint32_t M,
                uint32_t N, uint32_t K, Epilogue epi, void *__restrict__ out, uint32_t *status)
 {
     griddep_launch_dependents();
-    using C = Cfg<BN>;
+    using C = Cfg<BN, OUT>;
     extern __shared__ uint8_t smem_raw[];
     // 128B-swizzled tiles need a 1024-byte aligned base.
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;
     uint8_t *after = smem_raw + (ring - raw) + C::STAGES * C::STAGE_BYTES;
     uint32_t *s_col = reinterpret_cast<uint32_t *>(after);                 // [2][BN] column terms
-    uint64_t *bars = reinterpret_cast<uint64_t *>(after + 2 * BN * 4);     // full[S] empty[S] tfull[2] tempty[2]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(after + 2 * BN * col_bytes(OUT));  // full[S] empty[S] tfull[2] tempty[2]
     uint32_t *s_misc = reinterpret_cast<uint32_t *>(bars + 2 * C::STAGES + 4);  // [0] tmem base, [1] abort flag
     volatile uint32_t *abort_flag = s_misc + 1;
 
@@ -152,6 +156,42 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         // ---------------- epilogue (warps 2..5 = 128 threads) ----------------
         const uint32_t q = (uint32_t)warp & 3u;       // TMEM lane quarter this warp may read
         const uint32_t et = threadIdx.x - 64;         // 0..127
+        if constexpr (out_is_tokens(OUT)) {
+            const bool relu = epi.flags & LTQ_FLAG_RELU;
+            const uint64_t ldc = epilogue_pitch(epi, N);
+            const bool vec_ok = epilogue_vec_ok(epi, out, N, OUT == OUT_TOKENS + LTQ_F32 ? 4 : 2);
+            uint32_t as = 0, aph = 0;
+            bool ok = true;
+            for (uint32_t t = blockIdx.x; t < num_tiles; t += gridDim.x) {
+                const uint32_t m0 = (t / tiles_n) * BM, n0 = (t % tiles_n) * BN;
+                uint4 *col = reinterpret_cast<uint4 *>(s_col) + as * BN;
+                for (uint32_t j = et; j < (uint32_t)BN; j += 128) {
+                    const uint32_t gj = n0 + j;
+                    col[j] = gj < N ? token_col(epi, gj) : make_uint4(0, 0, 0, 0);
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                const uint32_t row = m0 + q * 32 + lane;
+                const TokenRow tr = row < M ? token_row(epi, row) : TokenRow{0, 0, 0.f};
+                if (ok) ok = mbar_wait(tfull0 + 8 * as, aph, abort_flag, status, 0x400u | as);
+                if (ok) {
+                    tc_fence_after();
+                    const uint32_t taddr = tmem_base + ((q * 32u) << 16) + as * BN;
+#pragma unroll 1
+                    for (int ch = 0; ch < BN / 32; ch++) {
+                        uint32_t v[32];
+                        tmem_ld32(taddr + ch * 32, v);
+                        tmem_ld_wait();
+                        const uint32_t c0 = n0 + ch * 32;
+                        if (row < M && c0 < N)
+                            token_chunk<OUT, 32>(v, tr, col + ch * 32, relu, out, row * ldc + c0, vec_ok, (N - c0) < 32u ? (int)(N - c0) : 32);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(tempty0 + 8 * as);
+                }
+                if (++as == 2) { as = 0; aph ^= 1; }
+            }
+        } else {
         const EpilogueConsts c = epilogue_consts(epi);
         const bool relu = epi.flags & LTQ_FLAG_RELU, sat = epi.flags & LTQ_FLAG_SATURATE;
         using OutT = typename std::conditional<OUT == 0, uint8_t, typename std::conditional<OUT == 1, float, int32_t>::type>::type;
@@ -193,6 +233,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 if (lane == 0) mbar_arrive(tempty0 + 8 * as);
             }
             if (++as == 2) { as = 0; aph ^= 1; }
+        }
         }
     }
 
@@ -241,11 +282,11 @@ constexpr int P_BN = 256;               // widest tile
 constexpr int P_A_BYTES = BM * BK;
 constexpr int P_B_BYTES = (P_BN / 2) * BK;  // room for this CTA's half of the widest tile's B rows
 constexpr int P_STAGE_BYTES = P_A_BYTES + P_B_BYTES;
-constexpr int P_TAIL_BYTES = 1024 + 2 * P_BN * 4 + 256;  // alignment slack + column terms + barriers
 constexpr int P_PEER_STAGE_BYTES = 8 * PeerStage::BYTES_PER_WARP;
-inline size_t pair_smem_bytes(int stages, bool peer_stage)
+inline size_t pair_smem_bytes(int stages, bool peer_stage, int out)
 {
-    return (size_t)stages * P_STAGE_BYTES + P_TAIL_BYTES + (peer_stage ? P_PEER_STAGE_BYTES : 0);
+    // ring + alignment slack + column terms + barriers
+    return (size_t)stages * P_STAGE_BYTES + 1024 + 2 * P_BN * col_bytes(out) + 256 + (peer_stage ? P_PEER_STAGE_BYTES : 0);
 }
 
 struct PairTile {
@@ -287,10 +328,10 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     const uint32_t ring = (raw + 1023u) & ~1023u;
     uint8_t *after = smem_raw + (ring - raw) + stages * P_STAGE_BYTES;
     uint32_t *s_col = reinterpret_cast<uint32_t *>(after);                  // [2][P_BN] column terms
-    uint64_t *bars = reinterpret_cast<uint64_t *>(after + 2 * P_BN * 4);    // full[S] empty[S] tfull[2] tempty[2]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(after + 2 * P_BN * col_bytes(OUT));    // full[S] empty[S] tfull[2] tempty[2]
     uint32_t *s_misc = reinterpret_cast<uint32_t *>(bars + 2 * P_MAX_STAGES + 4);  // [0] tmem base, [1] abort flag
     volatile uint32_t *abort_flag = s_misc + 1;
-    uint8_t *s_stage = after + 2 * P_BN * 4 + 256;    // [8 warps][32 rows][128 B], only allocated when epi.staged
+    uint8_t *s_stage = after + 2 * P_BN * col_bytes(OUT) + 256;    // [8 warps][32 rows][128 B], only allocated when epi.staged
 
     const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * P_MAX_STAGES;
     const uint32_t tfull0 = empty0 + 8 * P_MAX_STAGES, tempty0 = tfull0 + 16;
@@ -398,6 +439,57 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         const uint32_t q = (uint32_t)warp & 3u;            // TMEM lane quarter this warp may read
         const uint32_t h = (uint32_t)(warp - 2) >> 2;      // 0: lower column range of the tile, 1: upper
         const uint32_t et = threadIdx.x - 64;              // 0..255
+        if constexpr (out_is_tokens(OUT)) {
+            const bool relu = epi.flags & LTQ_FLAG_RELU;
+            const uint64_t ldc = epilogue_pitch(epi, N);
+            const bool vec_ok = epilogue_vec_ok(epi, out, N, OUT == OUT_TOKENS + LTQ_F32 ? 4 : 2);
+            uint32_t as = 0, aph = 0;
+            bool ok = true;
+            for (uint32_t t = pair; t < num_tiles; t += num_pairs) {
+                const PairTile pt = pair_tile(tl, t);
+                const uint32_t m0 = pt.m0 + rank * BM, n0 = pt.n0;
+                const int width = (int)pt.width;
+                const int split = ((width / 2 + 15) / 16) * 16;
+                uint4 *col = reinterpret_cast<uint4 *>(s_col) + as * P_BN;
+                for (uint32_t j = et; j < (uint32_t)width; j += 256) {
+                    const uint32_t gj = n0 + j;
+                    col[j] = gj < N ? token_col(epi, gj) : make_uint4(0, 0, 0, 0);
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                const uint32_t row = m0 + q * 32 + lane;
+                const TokenRow tr = row < M ? token_row(epi, row) : TokenRow{0, 0, 0.f};
+                if (ok) ok = mbar_wait(tfull0 + 8 * as, aph, abort_flag, status, 0x400u | as);
+                if (ok) {
+                    tc_fence_after();
+                    const uint32_t taddr = tmem_base + ((q * 32u) << 16) + as * P_BN;
+                    int cc = h ? split : 0;
+                    const int ce = h ? width : split;
+                    auto chunk = [&](auto &v) {
+                        constexpr int CW = (int)(sizeof(v) / sizeof(uint32_t));
+                        const uint32_t c0 = n0 + cc;
+                        if (row < M && c0 < N)
+                            token_chunk<OUT, CW>(v, tr, col + cc, relu, out, row * ldc + c0, vec_ok, (N - c0) < (uint32_t)CW ? (int)(N - c0) : CW);
+                    };
+#pragma unroll 1
+                    for (; cc + 32 <= ce; cc += 32) {
+                        uint32_t v[32];
+                        tmem_ld32(taddr + cc, v);
+                        tmem_ld_wait();
+                        chunk(v);
+                    }
+                    if (cc < ce) {
+                        uint32_t v[16];
+                        tmem_ld16(taddr + cc, v);
+                        tmem_ld_wait();
+                        chunk(v);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_remote(in_leader_cta(tempty0 + 8 * as));
+                }
+                if (++as == 2) { as = 0; aph ^= 1; }
+            }
+        } else {
         const EpilogueConsts c = epilogue_consts(epi);
         const bool relu = epi.flags & LTQ_FLAG_RELU, sat = epi.flags & LTQ_FLAG_SATURATE;
         using OutT = typename std::conditional<OUT == 0, uint8_t, typename std::conditional<OUT == 1, float, int32_t>::type>::type;
@@ -476,6 +568,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             }
             if (++as == 2) { as = 0; aph ^= 1; }
         }
+        }
     }
 
     // Teardown.  The leader's MMAs read the peer's shared memory and both CTAs' barriers receive remote arrivals, so
@@ -521,7 +614,7 @@ template <int BN, int OUT>
 cudaError_t launch_cfg(const CUtensorMap &ma, const CUtensorMap &mb, uint64_t M, uint64_t N, uint64_t K,
                        const Epilogue &epi, void *out, uint32_t *status, int sms, cudaStream_t stream)
 {
-    using C = Cfg<BN>;
+    using C = Cfg<BN, OUT>;
     static bool attr_done[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -547,6 +640,9 @@ cudaError_t launch_out(const CUtensorMap &ma, const CUtensorMap &mb, uint64_t M,
     switch (epi.out_mode) {
         case LTQ_OUT_U8: return launch_cfg<BN, 0>(ma, mb, M, N, K, epi, out, status, sms, stream);
         case LTQ_OUT_F32: return launch_cfg<BN, 1>(ma, mb, M, N, K, epi, out, status, sms, stream);
+        case OUT_TOKENS + LTQ_F32: return launch_cfg<BN, OUT_TOKENS + LTQ_F32>(ma, mb, M, N, K, epi, out, status, sms, stream);
+        case OUT_TOKENS + LTQ_F16: return launch_cfg<BN, OUT_TOKENS + LTQ_F16>(ma, mb, M, N, K, epi, out, status, sms, stream);
+        case OUT_TOKENS + LTQ_BF16: return launch_cfg<BN, OUT_TOKENS + LTQ_BF16>(ma, mb, M, N, K, epi, out, status, sms, stream);
         default: return launch_cfg<BN, 2>(ma, mb, M, N, K, epi, out, status, sms, stream);
     }
 }
@@ -564,7 +660,7 @@ cudaError_t launch_pair(const CUtensorMap &ma, const CUtensorMap *const mb[4], c
     cudaGetDevice(&dev);
     if (dev >= 0 && dev < 64 && !attr_done[dev]) {
         cudaError_t e = cudaFuncSetAttribute(gemm_tc_pair_kernel<OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)pair_smem_bytes(P_MAX_STAGES, false));
+                                             (int)pair_smem_bytes(P_MAX_STAGES, false, OUT));
         if (e != cudaSuccess) return e;
         attr_done[dev] = true;
     }
@@ -575,7 +671,7 @@ cudaError_t launch_pair(const CUtensorMap &ma, const CUtensorMap *const mb[4], c
     Epilogue epi_l = epi;
     epi_l.staged = (epi.n_more > 0 || epi.mc) ? 1 : 0;
     uint32_t stages = epi_l.staged ? P_MAX_STAGES - 1 : P_MAX_STAGES;
-    const size_t smem = pair_smem_bytes((int)stages, epi_l.staged != 0);
+    const size_t smem = pair_smem_bytes((int)stages, epi_l.staged != 0, OUT);
     cudaError_t e = launch_chained(gemm_tc_pair_kernel<OUT>, dim3((unsigned)(2 * pairs)), dim3(P_THREADS), smem, stream, ma,
                                    *mb[0], *mb[1], *mb[2], *mb[3], tl, (uint32_t)M, (uint32_t)N, (uint32_t)K, stages,
                                    epi_l, out, status);
@@ -660,6 +756,9 @@ cudaError_t launch_gemm_tc_pair(const TcOperandMap &map_a, const TcOperandMap *c
     switch (epi.out_mode) {
         case LTQ_OUT_U8: return launch_pair<0>(ma, mb, tl, M, N, K, epi, out, status, sms, stream);
         case LTQ_OUT_F32: return launch_pair<1>(ma, mb, tl, M, N, K, epi, out, status, sms, stream);
+        case OUT_TOKENS + LTQ_F32: return launch_pair<OUT_TOKENS + LTQ_F32>(ma, mb, tl, M, N, K, epi, out, status, sms, stream);
+        case OUT_TOKENS + LTQ_F16: return launch_pair<OUT_TOKENS + LTQ_F16>(ma, mb, tl, M, N, K, epi, out, status, sms, stream);
+        case OUT_TOKENS + LTQ_BF16: return launch_pair<OUT_TOKENS + LTQ_BF16>(ma, mb, tl, M, N, K, epi, out, status, sms, stream);
         default: return launch_pair<2>(ma, mb, tl, M, N, K, epi, out, status, sms, stream);
     }
 }

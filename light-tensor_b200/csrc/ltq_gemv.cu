@@ -37,6 +37,7 @@
 #include "ltq_common.cuh"
 #include "ltq_gemv.cuh"
 #include "ltq_tcgen05.cuh"
+#include "ltq_tokens.cuh"
 
 namespace ltq {
 
@@ -122,7 +123,7 @@ struct NextBand {
 
 }  // namespace
 
-// OUT: 0 = uint8, 1 = float, 2 = int32 (ltq_out_mode).
+// OUT: 0 = uint8, 1 = float, 2 = int32 (ltq_out_mode), OUT_TOKENS + ltq_dtype = parameters per token and channel.
 template <int OUT>
 __global__ void __launch_bounds__(THREADS, 2)
 gemv_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w_lo,
@@ -307,6 +308,50 @@ gemv_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         griddep_wait();  // the activation row sums (and device-side qparams) come from the previous kernel
         if (blockIdx.x == 0 && epi.clear_ptr)  // chain housekeeping, see Epilogue::clear_ptr (128 epilogue threads)
             for (uint32_t i = threadIdx.x - 64; i < epi.clear_count; i += 128) epi.clear_ptr[i] = 0;
+        if constexpr (out_is_tokens(OUT)) {
+            // One weight row and its parameters per thread; the tokens' parameters sit in lanes 0..15 of every warp and
+            // are broadcast one token at a time (48 registers otherwise).
+            constexpr int DT = OUT - OUT_TOKENS;
+            using OutT = typename std::conditional<DT == LTQ_F32, uint32_t, uint16_t>::type;
+            OutT *o = static_cast<OutT *>(out);
+            const bool relu = epi.flags & LTQ_FLAG_RELU;
+            const uint64_t ldc = epilogue_pitch(epi, N);
+            const TokenRow mine = (uint32_t)lane < M ? token_row(epi, (uint64_t)lane) : TokenRow{0, 0, 0.f};
+            uint32_t as = 0, aph = 0;
+            bool ok = true;
+            for (uint32_t t = t_begin; t < t_end; t++) {
+                const uint32_t o0 = (uint32_t)(((uint64_t)t * octs) / tiles), o1 = (uint32_t)(((uint64_t)(t + 1) * octs) / tiles);
+                const uint32_t n = o0 * 8 + q * 32 + lane;
+                const bool valid = (q * 32 + lane) < (o1 - o0) * 8 && n < N;
+                const uint4 tc = valid ? token_col(epi, n) : make_uint4(0, 0, 0, 0);
+                if (ok) ok = __all_sync(0xFFFFFFFFu, mbar_wait(tfull0 + 8 * as, aph, abort_flag, status, 0x400u | as));
+                if (ok) {
+                    tc_fence_after();
+                    uint32_t v[XROWS], w1[XROWS], w2[XROWS], w3[XROWS];
+                    const uint32_t tacc = tmem_base + ((q * 32u) << 16) + as * (NACC * XROWS);
+                    tmem_ld16(tacc, v);
+                    tmem_ld16(tacc + XROWS, w1);
+                    tmem_ld16(tacc + 2 * XROWS, w2);
+                    tmem_ld16(tacc + 3 * XROWS, w3);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int m = 0; m < XROWS; m++) v[m] += w1[m] + w2[m] + w3[m];
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(tempty0 + 8 * as);
+#pragma unroll
+                    for (int m = 0; m < XROWS; m++) {
+                        if ((uint32_t)m < M) {
+                            const TokenRow tr{__shfl_sync(0xFFFFFFFFu, mine.za, m), __shfl_sync(0xFFFFFFFFu, mine.neg_asum, m),
+                                              __shfl_sync(0xFFFFFFFFu, mine.sa, m)};
+                            const float y = token_value(v[m], tr, tc, relu);
+                            if (valid) o[(size_t)m * ldc + n] = (OutT)token_bits<DT>(y);
+                        }
+                    }
+                }
+                if (++as == 2) { as = 0; aph ^= 1; }
+            }
+        } else {
         const EpilogueConsts c = epilogue_consts(epi);
         const bool relu = epi.flags & LTQ_FLAG_RELU, sat = epi.flags & LTQ_FLAG_SATURATE;
         using OutT = typename std::conditional<OUT == 0, uint8_t, typename std::conditional<OUT == 1, float, int32_t>::type>::type;
@@ -378,6 +423,7 @@ gemv_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
                 }
             }
             if (++as == 2) { as = 0; aph ^= 1; }
+        }
         }
     }
 
@@ -501,6 +547,9 @@ cudaError_t launch_gemv(const uint8_t *x, const uint8_t *W, uint64_t M, uint64_t
     }
     switch (epi.out_mode) {
         case LTQ_OUT_U8: return launch_t<0>(mx, wm->lo, wm->hi, p, M, N, K, epi, out, status, stream, early_weights, *nlo, *nhi, nx);
+        case OUT_TOKENS + LTQ_F32: return launch_t<OUT_TOKENS + LTQ_F32>(mx, wm->lo, wm->hi, p, M, N, K, epi, out, status, stream, early_weights, *nlo, *nhi, nx);
+        case OUT_TOKENS + LTQ_F16: return launch_t<OUT_TOKENS + LTQ_F16>(mx, wm->lo, wm->hi, p, M, N, K, epi, out, status, stream, early_weights, *nlo, *nhi, nx);
+        case OUT_TOKENS + LTQ_BF16: return launch_t<OUT_TOKENS + LTQ_BF16>(mx, wm->lo, wm->hi, p, M, N, K, epi, out, status, stream, early_weights, *nlo, *nhi, nx);
         case LTQ_OUT_F32: return launch_t<1>(mx, wm->lo, wm->hi, p, M, N, K, epi, out, status, stream, early_weights, *nlo, *nhi, nx);
         default: return launch_t<2>(mx, wm->lo, wm->hi, p, M, N, K, epi, out, status, stream, early_weights, *nlo, *nhi, nx);
     }

@@ -19,6 +19,12 @@ struct ltq_layer {
     int32_t *rowsum_out = nullptr; // optional: receives the row sums of uint8 outputs (ltq_layer_set_rowsum_output)
     int32_t *clear_ptr = nullptr;  // optional: array cleared by every forward (ltq_layer_set_clear_on_forward)
     uint32_t clear_count = 0;
+    // Parameters per output channel (ltq_layer_set_channel_qparams) with their float bias; a copy of the weights whose rows
+    // are padded with zeros to a multiple of 16 bytes when in_features is not one (what the tensor copies need).
+    const ltq_qparams *qp_channels = nullptr;
+    const float *fbias = nullptr;
+    uint8_t *w_pad = nullptr;
+    uint64_t padded_k() const { return (K + 15) / 16 * 16; }
     ltq::TcOperandMap map_w[LAYER_MAPS];  // weight tensor maps of the tensor-core kernels, one per box height, built on demand
     int map_w_next = 0;
     ltq::GemvWeightMaps map_w_gemv;     // weight tensor maps of the skinny kernel

@@ -20,7 +20,14 @@ class QParams(C.Structure):
         return f"QParams(scale={self.scale!r}, zero_point={self.zero_point})"
 
 
+class KVCacheDesc(C.Structure):
+    """``ltq_kv_cache``: device arrays and shape of a paged 8-bit key/value cache."""
+    _fields_ = [("k_dev", C.c_void_p), ("k_qp_dev", C.c_void_p), ("v_dev", C.c_void_p), ("v_qp_dev", C.c_void_p),
+                ("blocks", C.c_uint64), ("kv_heads", C.c_uint32), ("block_tokens", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
 OUT_U8, OUT_F32, OUT_I32 = 0, 1, 2
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2   # ltq_dtype
 MAX_DESTS = 8
 FLAG_RELU, FLAG_SATURATE, FLAG_BIAS_PER_CHANNEL = 1, 2, 4
 FLAG_FORCE_SIMT, FLAG_FORCE_TC, FLAG_FORCE_SKINNY = 0x100, 0x200, 0x400
@@ -30,6 +37,7 @@ FLAG_NHWC_IN, FLAG_NHWC_OUT = 0x4000, 0x8000
 
 _u64, _vp, _int = C.c_uint64, C.c_void_p, C.c_int
 _qp = C.POINTER(QParams)
+_kv = C.POINTER(KVCacheDesc)
 
 # name -> (restype, argtypes); one entry per declaration in include/ltq.h
 _SIGNATURES = {
@@ -60,6 +68,16 @@ _SIGNATURES = {
     "ltq_layer_set_qparams": (_int, [_vp, _qp, _qp, _qp]),
     "ltq_layer_forward": (_int, [_vp, _vp, _vp, _u64, _vp, _int, C.c_uint, _vp, _vp]),
     "ltq_layer_check": (_int, [_vp, _vp]),
+    "ltq_quantize_tokens_u8": (_int, [_vp, _int, _u64, _u64, _u64, _vp, _vp, _vp, _int, _vp]),
+    "ltq_dequantize_tokens_u8": (_int, [_vp, _int, _u64, _vp, _vp, _u64, _u64, _int, _vp]),
+    "ltq_layer_set_channel_qparams": (_int, [_vp, _vp, _vp, _vp]),
+    "ltq_layer_forward_tokens": (_int, [_vp, _vp, _vp, _vp, _u64, _int, C.c_uint, _vp, _u64, _vp]),
+    "ltq_layer_float_workspace": (_u64, [_vp, _u64]),
+    "ltq_layer_forward_float": (_int, [_vp, _vp, _int, _u64, _u64, _int, C.c_uint, _vp, _u64, _vp, _u64, _vp]),
+    "ltq_cache_append": (_int, [_kv, _vp, _vp, _int, _u64, _u64, _vp, _vp, _vp, _u64, _u64, _u64, _int, _vp]),
+    "ltq_cache_attention_workspace": (_u64, [_kv, _u64, C.c_uint32, _u64, _u64, _u64, _int]),
+    "ltq_cache_attention": (_int, [_kv, _vp, _int, _u64, _u64, C.c_uint32, _vp, _vp, _vp, _u64, _u64, _u64, C.c_float, _vp, _vp, _u64,
+                                   _int, _vp]),
     "ltq_layer_set_rowsum_output": (_int, [_vp, _vp]),
     "ltq_layer_set_clear_on_forward": (_int, [_vp, _vp, _u64]),
     "ltq_layer_set_next": (_int, [_vp, _vp]),

@@ -4,6 +4,7 @@ import ctypes as C
 
 import torch
 
+from . import tokens as _tokens
 from ._binding import (OUT_F32, OUT_I32, OUT_U8, FLAG_BIAS_PER_CHANNEL, FLAG_NHWC_IN, FLAG_NHWC_OUT, FLAG_RELU, FLAG_SATURATE, QParams, check,
                        lib)
 
@@ -75,6 +76,54 @@ class LayerHandle:
         Results are unchanged.  Set it again after ``nxt.set_weights``; pass None before ``nxt``'s weights are freed."""
         self._next = nxt  # keeps the weights it points at alive
         check(lib().ltq_layer_set_next(self._h, None if nxt is None else nxt._h))
+
+    def set_channel_qparams(self, qparams, bias=None):
+        """Parameters per output channel: uint8 CUDA tensor [N, 8] of QParams (``quantize_tokens`` of the weight matrix gives
+        one), optional float32 bias [N].  Call after set_weights, and again after every later set_weights."""
+        _tokens.check_qparams(qparams, self.N, self.device_index)
+        if bias is not None and not (bias.is_cuda and bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == self.N):
+            raise ValueError("bias must be a contiguous float32 CUDA tensor with one value per output feature")
+        self._keep_channels = (qparams, bias)  # the library borrows these pointers
+        check(lib().ltq_layer_set_channel_qparams(self._h, qparams.data_ptr(), None if bias is None else bias.data_ptr(), self._stream()))
+
+    def forward_tokens(self, x, qparams, sums, dtype=torch.float32, flags=0, out=None):
+        """Product of codes x uint8 [M, K] that have parameters per token (``quantize_tokens`` returns all three) with this
+        layer's weights under their parameters per channel.  Returns [M, N] of `dtype`; ``out`` may have strided rows."""
+        if not (x.is_cuda and x.dtype == torch.uint8 and x.is_contiguous() and x.dim() == 2 and x.shape[1] == self.K):
+            raise ValueError(f"x must be a contiguous uint8 CUDA tensor [tokens, {self.K}]")
+        M = x.shape[0]
+        _tokens.check_qparams(qparams, M, self.device_index)
+        if not (sums.is_cuda and sums.dtype == torch.int32 and sums.is_contiguous() and sums.numel() == M):
+            raise ValueError("sums must be a contiguous int32 CUDA tensor with one value per token")
+        out = self._tokens_out(out, M, dtype, x.device)
+        if M:
+            check(lib().ltq_layer_forward_tokens(self._h, x.data_ptr(), qparams.data_ptr(), sums.data_ptr(), M, _tokens.dtype_code(dtype), flags,
+                                                 out.data_ptr(), out.stride(0), self._stream()))
+        return out
+
+    def forward_float(self, x, dtype=None, flags=0, out=None):
+        """quantize_tokens and forward_tokens in one call: x float32 / float16 / bfloat16 [M, K] (rows may be strided).  Returns
+        [M, N] of `dtype` (default: x's)."""
+        if not (x.is_cuda and x.dim() == 2 and x.shape[1] == self.K and x.device.index == self.device_index):
+            raise ValueError(f"x must be a CUDA tensor [tokens, {self.K}] on device {self.device_index}")
+        code, ld = _tokens.dtype_code(x.dtype), _tokens.row_stride(x)
+        M = x.shape[0]
+        out = self._tokens_out(out, M, dtype or x.dtype, x.device)
+        if M:
+            need = lib().ltq_layer_float_workspace(self._h, M)
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+            check(lib().ltq_layer_forward_float(self._h, x.data_ptr(), code, ld, M, _tokens.dtype_code(out.dtype), flags, out.data_ptr(),
+                                                out.stride(0), ws.data_ptr(), need, self._stream()))
+        return out
+
+    def _tokens_out(self, out, M, dtype, device):
+        if out is None:
+            return torch.empty((M, self.N), dtype=dtype, device=device)
+        if not (out.is_cuda and out.device == device and out.dtype == dtype and out.shape == (M, self.N) and (out.stride(1) == 1 or self.N == 1)):
+            raise ValueError(f"out must be a CUDA tensor [{M}, {self.N}] of {dtype} with contiguous rows")
+        if M > 1 and out.stride(0) < self.N:
+            raise ValueError("out's rows overlap")
+        return out
 
     def forward_scatter(self, x, dest_ptrs, ld_out, col_offset, out_mode=OUT_U8, flags=0, asum=None, qp_in_dev=None):
         """Like forward, but element (i, j) goes to ``dest_ptrs[d] + (i * ld_out + col_offset + j) * itemsize`` for
@@ -227,6 +276,56 @@ class FullyConnected_q:
         out = self._handle.forward(x.view(-1, self.input_features_), self._out_mode, self._flags, asum=asum,
                                    qp_in_dev=qp_in_dev)
         return out.view(*input.shape[:-1], self.output_features_)
+
+
+class FullyConnected_t:
+    """Linear layer for transformer blocks: y = x w^T + b in x's own type, x quantised per token (row) on the fly, w held in
+    8 bits with parameters per output channel.  ``weight`` uint8 CUDA [N, K], ``weight_qparams`` uint8 CUDA [N, 8] (a QParams
+    per row), ``bias`` float32 CUDA [N] or None; ``from_float`` quantises a float weight matrix.  No counterpart in the
+    reference, whose FullyConnected_q has one set of parameters per tensor and uint8 in and out."""
+
+    def __init__(self, weight, weight_qparams, bias=None):
+        if not (weight.is_cuda and weight.dtype == torch.uint8 and weight.dim() == 2 and weight.is_contiguous()):
+            raise ValueError("weight must be a contiguous uint8 CUDA tensor [output features, input features]")
+        self.output_features_, self.input_features_ = weight.shape
+        self.weight_ptr_, self.weight_qparams_, self.bias_ptr_ = weight, weight_qparams, bias
+        self._flags = 0
+        self._handle = LayerHandle(weight.device.index, self.input_features_, self.output_features_)
+        self._handle.set_weights(weight)
+        self._handle.set_channel_qparams(weight_qparams, bias)
+
+    @classmethod
+    def from_float(cls, weight, bias=None):
+        """weight: float32 / float16 / bfloat16 CUDA [N, K]; quantised per output channel."""
+        codes, qparams, _ = _tokens.quantize_tokens(weight)
+        return cls(codes, qparams, None if bias is None else bias.float().contiguous())
+
+    def get_weights(self):
+        return self.weight_ptr_
+
+    def get_bias(self):
+        return self.bias_ptr_
+
+    def is_using_bias(self):
+        return self.bias_ptr_ is not None
+
+    def set_output(self, relu=False):
+        self._flags = FLAG_RELU if relu else 0
+
+    def forward(self, input, out=None):
+        """input [..., K] float32 / float16 / bfloat16 on the layer's device -> [..., N] of the same type."""
+        if input.dim() == 0 or input.shape[-1] != self.input_features_:
+            raise ValueError("Last dimension must be equal to the number of input features")
+        if input.device != self.weight_ptr_.device:
+            raise ValueError("Input tensor device type is not the same as this layer's parameters")
+        x = input if input.dim() == 2 else input.reshape(-1, self.input_features_)
+        if out is not None:
+            if out.shape != (*input.shape[:-1], self.output_features_):
+                raise ValueError("out has another shape")
+            self._handle.forward_float(x, None, self._flags, out.view(-1, self.output_features_))
+            return out
+        y = self._handle.forward_float(x, None, self._flags)
+        return y if input.dim() == 2 else y.view(*input.shape[:-1], self.output_features_)
 
 
 class ConvHandle:
