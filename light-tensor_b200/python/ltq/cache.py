@@ -26,9 +26,11 @@ class KVCache:
         for t in (k_qparams, v_qparams):
             _tokens.check_qparams(t, self.blocks * self.kv_heads, k.device.index)
         self.k, self.k_qparams, self.v, self.v_qparams = k, k_qparams, v, v_qparams
-        self.device = k.device
+        self.device, self._index = k.device, k.device.index
         self._desc = KVCacheDesc(k.data_ptr(), k_qparams.data_ptr(), v.data_ptr(), v_qparams.data_ptr(), self.blocks, self.kv_heads,
                                  self.block_tokens, self.head_dim)
+        self._ref = C.byref(self._desc)
+        self._as_rows = tuple((t.view(self.blocks * self.kv_heads, self.block_tokens * self.head_dim), p.view(-1, 8)) for t, p in ((k, k_qparams), (v, v_qparams)))
 
     @classmethod
     def empty(cls, blocks, kv_heads, block_tokens, head_dim, device="cuda"):
@@ -40,69 +42,66 @@ class KVCache:
         return cls(codes[0], qparams[0], codes[1], qparams[1])
 
     def _batch(self, table, lengths, offsets):
-        if not (table.dtype == lengths.dtype == offsets.dtype == torch.int32 and table.device == lengths.device == offsets.device == self.device):
+        dev, i32 = self._index, torch.int32
+        if not (table.dtype is i32 and lengths.dtype is i32 and offsets.dtype is i32 and
+                table.get_device() == dev and lengths.get_device() == dev and offsets.get_device() == dev):
             raise ValueError(f"table, lengths and offsets must be int32 tensors on {self.device}")
         if not (table.is_contiguous() and lengths.is_contiguous() and offsets.is_contiguous()):
             raise ValueError("table, lengths and offsets must be contiguous")
-        seqs = lengths.shape[0]
-        if not (table.dim() == 2 and table.shape[0] == seqs and lengths.dim() == 1 and offsets.shape == (seqs + 1,)):
+        seqs = lengths.numel()
+        if not (table.dim() == 2 and table.shape[0] == seqs and lengths.dim() == 1 and offsets.dim() == 1 and offsets.numel() == seqs + 1):
             raise ValueError("table [seqs, width], lengths [seqs] and offsets [seqs + 1] are expected")
         return seqs, table.shape[1]
 
     def _rows(self, t, heads, what):
-        """Elements between the tokens of a [tokens, heads, head_dim] tensor whose tokens are contiguous."""
-        if not (t.device == self.device and t.dim() == 3 and t.shape[2] == self.head_dim and (heads is None or t.shape[1] == heads)):
+        """(tokens, heads, elements between the tokens) of a [tokens, heads, head_dim] tensor whose tokens are contiguous."""
+        if not (t.get_device() == self._index and t.dim() == 3 and t.shape[2] == self.head_dim and (heads is None or t.shape[1] == heads)):
             raise ValueError(f"{what} must be a tensor [tokens, heads, {self.head_dim}] on {self.device}")
-        n = t.shape[1] * self.head_dim
-        if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != self.head_dim) or (t.shape[0] > 1 and t.stride(0) < n):
+        tokens, heads, D = t.shape
+        pitch, between, step = t.stride()
+        n = heads * D
+        if step != 1 or (heads > 1 and between != D) or (tokens > 1 and pitch < n):
             raise ValueError(f"the heads of a token of {what} must be contiguous")
-        return t.stride(0) if t.shape[0] > 1 else n
-
-    def _stream(self):
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+        return tokens, heads, pitch if tokens > 1 else n
 
     def append(self, k, v, table, lengths, offsets, max_new):
         """Quantises new keys and values [tokens, kv_heads, head_dim] (float32 / float16 / bfloat16; token stride free) into the
         cache.  See ltq_cache_append for the scales."""
-        ld = self._rows(k, self.kv_heads, "k")
-        if v.dtype != k.dtype or v.shape != k.shape or self._rows(v, self.kv_heads, "v") != ld:
+        tokens, _, ld = self._rows(k, self.kv_heads, "k")
+        if v.dtype is not k.dtype or self._rows(v, self.kv_heads, "v") != (tokens, self.kv_heads, ld):
             raise ValueError("k and v must have the same type, shape and strides")
         seqs, width = self._batch(table, lengths, offsets)
-        check(lib().ltq_cache_append(C.byref(self._desc), k.data_ptr(), v.data_ptr(), _tokens.dtype_code(k.dtype), ld, k.shape[0],
-                                     offsets.data_ptr(), lengths.data_ptr(), table.data_ptr(), seqs, width, max_new, self.device.index,
-                                     self._stream()))
+        check(lib().ltq_cache_append(self._ref, k.data_ptr(), v.data_ptr(), _tokens.dtype_code(k.dtype), ld, tokens, offsets.data_ptr(),
+                                     lengths.data_ptr(), table.data_ptr(), seqs, width, max_new, self._index, _tokens.raw_stream(self._index)))
 
     def attention(self, q, table, lengths, offsets, max_new, scale=None, out=None, workspace=None):
         """Causal attention of the new tokens' queries [tokens, q_heads, head_dim] over the cache, which holds their keys already.
         Returns the same shape and type (`out`, contiguous, if given).  scale: default head_dim ** -0.5.  workspace: uint8
         CUDA tensor of at least ``attention_workspace`` bytes; made here if not given."""
-        ld = self._rows(q, None, "q")
+        tokens, heads, ld = self._rows(q, None, "q")
         code = _tokens.dtype_code(q.dtype)
         seqs, width = self._batch(table, lengths, offsets)
-        tokens, heads = q.shape[0], q.shape[1]
         if out is None:
-            out = torch.empty((tokens, heads, self.head_dim), dtype=q.dtype, device=q.device)
-        elif not (out.device == q.device and out.dtype == q.dtype and out.shape == q.shape and out.is_contiguous()):
+            out = q.new_empty((tokens, heads, self.head_dim))
+        elif not (out.get_device() == self._index and out.dtype is q.dtype and out.shape == q.shape and out.is_contiguous()):
             raise ValueError("out must be a contiguous tensor of q's shape, type and device")
         if workspace is None:
-            workspace = torch.empty(self.attention_workspace(tokens, heads, seqs, width, max_new), dtype=torch.uint8, device=q.device)
-        elif not (workspace.device == q.device and workspace.dtype == torch.uint8 and workspace.is_contiguous()):
+            workspace = q.new_empty(self.attention_workspace(tokens, heads, seqs, width, max_new), dtype=torch.uint8)
+        elif not (workspace.get_device() == self._index and workspace.dtype is torch.uint8 and workspace.is_contiguous()):
             raise ValueError("workspace must be a contiguous uint8 tensor on q's device")
-        check(lib().ltq_cache_attention(C.byref(self._desc), q.data_ptr(), code, ld, tokens, heads, offsets.data_ptr(), lengths.data_ptr(),
+        check(lib().ltq_cache_attention(self._ref, q.data_ptr(), code, ld, tokens, heads, offsets.data_ptr(), lengths.data_ptr(),
                                         table.data_ptr(), seqs, width, max_new, self.head_dim ** -0.5 if scale is None else scale,
-                                        out.data_ptr(), workspace.data_ptr(), workspace.numel(), self.device.index, self._stream()))
+                                        out.data_ptr(), workspace.data_ptr(), workspace.numel(), self._index, _tokens.raw_stream(self._index)))
         return out
 
     def attention_workspace(self, tokens, q_heads, seqs, width, max_new):
         """Bytes of workspace that ``attention`` needs for these sizes."""
-        return lib().ltq_cache_attention_workspace(C.byref(self._desc), tokens, q_heads, seqs, width, max_new, self.device.index)
+        return lib().ltq_cache_attention_workspace(self._ref, tokens, q_heads, seqs, width, max_new, self._index)
 
     def values(self, dtype=torch.float32):
         """Keys and values of all slots as numbers: two tensors [blocks, kv_heads, block_tokens, head_dim] of `dtype`."""
-        rows = (self.blocks * self.kv_heads, self.block_tokens * self.head_dim)
-        return tuple(_tokens.dequantize_tokens(t.view(rows), p.view(-1, 8), dtype).view(t.shape)
-                     for t, p in ((self.k, self.k_qparams), (self.v, self.v_qparams)))
+        return tuple(_tokens.dequantize_tokens(t, p, dtype).view(self.k.shape) for t, p in self._as_rows)
 
     def check(self):
         """Waits for the stream and raises if a cache call met a sequence or block id outside its bounds since the last check."""
-        check(lib().ltq_device_check(self.device.index, self._stream()))
+        check(lib().ltq_device_check(self._index, _tokens.raw_stream(self._index)))

@@ -18,6 +18,7 @@ class LayerHandle:
         self._h = C.c_void_p()
         self.device_index = device_index
         self.K, self.N = in_features, out_features
+        self._row_workspace = 0
         check(lib().ltq_layer_create(C.byref(self._h), device_index, in_features, out_features))
 
     def close(self):
@@ -85,6 +86,7 @@ class LayerHandle:
             raise ValueError("bias must be a contiguous float32 CUDA tensor with one value per output feature")
         self._keep_channels = (qparams, bias)  # the library borrows these pointers
         check(lib().ltq_layer_set_channel_qparams(self._h, qparams.data_ptr(), None if bias is None else bias.data_ptr(), self._stream()))
+        self._row_workspace = lib().ltq_layer_float_workspace(self._h, 1)   # bytes per token, see forward_float
 
     def forward_tokens(self, x, qparams, sums, dtype=torch.float32, flags=0, out=None):
         """Product of codes x uint8 [M, K] that have parameters per token (``quantize_tokens`` returns all three) with this
@@ -104,16 +106,21 @@ class LayerHandle:
     def forward_float(self, x, dtype=None, flags=0, out=None):
         """quantize_tokens and forward_tokens in one call: x float32 / float16 / bfloat16 [M, K] (rows may be strided).  Returns
         [M, N] of `dtype` (default: x's)."""
-        if not (x.is_cuda and x.dim() == 2 and x.shape[1] == self.K and x.device.index == self.device_index):
-            raise ValueError(f"x must be a CUDA tensor [tokens, {self.K}] on device {self.device_index}")
+        dev = self.device_index
+        if not (x.get_device() == dev and x.dim() == 2 and x.shape[1] == self.K):
+            raise ValueError(f"x must be a CUDA tensor [tokens, {self.K}] on device {dev}")
         code, ld = _tokens.dtype_code(x.dtype), _tokens.row_stride(x)
         M = x.shape[0]
-        out = self._tokens_out(out, M, dtype or x.dtype, x.device)
+        out_code = code if dtype is None else _tokens.dtype_code(dtype)
+        if out is None:
+            out, ld_out = x.new_empty((M, self.N), dtype=dtype), self.N
+        else:
+            out, ld_out = self._tokens_out(out, M, dtype or x.dtype, x.device), out.stride(0)
         if M:
-            need = lib().ltq_layer_float_workspace(self._h, M)
-            ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-            check(lib().ltq_layer_forward_float(self._h, x.data_ptr(), code, ld, M, _tokens.dtype_code(out.dtype), flags, out.data_ptr(),
-                                                out.stride(0), ws.data_ptr(), need, self._stream()))
+            need = M * self._row_workspace
+            ws = x.new_empty(need, dtype=torch.uint8)
+            check(lib().ltq_layer_forward_float(self._h, x.data_ptr(), code, ld, M, out_code, flags, out.data_ptr(), ld_out, ws.data_ptr(), need,
+                                                _tokens.raw_stream(dev)))
         return out
 
     def _tokens_out(self, out, M, dtype, device):
@@ -314,18 +321,17 @@ class FullyConnected_t:
 
     def forward(self, input, out=None):
         """input [..., K] float32 / float16 / bfloat16 on the layer's device -> [..., N] of the same type."""
+        if input.dim() == 2 and out is None:
+            return self._handle.forward_float(input, None, self._flags)
         if input.dim() == 0 or input.shape[-1] != self.input_features_:
             raise ValueError("Last dimension must be equal to the number of input features")
-        if input.device != self.weight_ptr_.device:
-            raise ValueError("Input tensor device type is not the same as this layer's parameters")
-        x = input if input.dim() == 2 else input.reshape(-1, self.input_features_)
-        if out is not None:
-            if out.shape != (*input.shape[:-1], self.output_features_):
-                raise ValueError("out has another shape")
-            self._handle.forward_float(x, None, self._flags, out.view(-1, self.output_features_))
-            return out
-        y = self._handle.forward_float(x, None, self._flags)
-        return y if input.dim() == 2 else y.view(*input.shape[:-1], self.output_features_)
+        x = input.reshape(-1, self.input_features_)
+        if out is None:
+            return self._handle.forward_float(x, None, self._flags).view(*input.shape[:-1], self.output_features_)
+        if out.shape != (*input.shape[:-1], self.output_features_):
+            raise ValueError("out has another shape")
+        self._handle.forward_float(x, None, self._flags, out.view(-1, self.output_features_))
+        return out
 
 
 class ConvHandle:
