@@ -56,6 +56,7 @@ cache_append_kernel(const ltq_kv_cache cache, const CacheBatch bt, const void *_
     griddep_launch_dependents();
     griddep_wait();
     const CacheSeq s = cache_seq(bt, blockIdx.z);
+    if (!s.ok && threadIdx.x == 0) atomicCAS(bt.status, 0u, STATUS_BAD_SEQUENCE);
     if (!s.ok || s.n == 0) return;
     const bool is_v = blockIdx.x & 1;
     const int bt_tokens = 1 << bt.log2_bt, start = s.len - s.n < 0 ? 0 : s.len - s.n;   // first position that is stored
@@ -134,18 +135,12 @@ uint32_t attn_rows_per_tile(int dtype, uint32_t head_dim, uint64_t rows)
     // sixteen rows share the conversion of the keys where the registers allow it
     return rows > 8 && head_dim * (dtype == LTQ_F32 ? 2 : 1) <= 128 ? 16 : 8;
 }
+uint32_t attn_ctas_per_sm(int dtype, uint32_t head_dim, uint32_t rows_per_tile)
+{
+    return head_dim * (rows_per_tile / 8) * (dtype == LTQ_F32 ? 2 : 1) <= 128 ? 3 : 2;
+}
 
 namespace {
-
-// CTAs that share one sequence's keys: enough to fill the device (about three CTAs fit an SM), but none with less than
-// four 16-key steps for each of its warps.
-uint32_t attn_splits(uint32_t kv_heads, uint64_t row_tiles, uint64_t seqs, uint64_t max_keys, int sms)
-{
-    const uint64_t items = kv_heads * row_tiles * seqs, target = (uint64_t)sms * 3, steps = (max_keys + 15) / 16;
-    uint64_t s = (target + items - 1) / items;
-    if (s > steps / 16) s = steps / 16;
-    return (uint32_t)(s < 1 ? 1 : (s > 64 ? 64 : s));
-}
 
 int check_cache(const ltq_kv_cache *c)
 {
@@ -190,10 +185,26 @@ CacheBatch make_batch(const ltq_kv_cache *c, const int32_t *offsets, const int32
     return bt;
 }
 
-uint32_t attn_plan(const ltq_kv_cache *c, int dtype, uint32_t q_heads, uint64_t seqs, uint64_t table_width, uint64_t max_new, int sms)
+// How the attention call is laid out: CTAs, row tiles per sequence, and the workspace behind them.
+struct AttnPlan {
+    uint32_t rows_per_tile, row_tiles, ctas;
+    uint64_t o_floats, ml, items, bytes;
+};
+AttnPlan attn_plan(const ltq_kv_cache *c, int dtype, uint32_t q_heads, uint64_t seqs, uint64_t table_width, uint64_t max_new, int sms)
 {
-    const uint64_t rows = max_new * (q_heads / c->kv_heads), per = attn_rows_per_tile(dtype, c->head_dim, rows);
-    return attn_splits(c->kv_heads, (rows + per - 1) / per, seqs, table_width * c->block_tokens, sms);
+    AttnPlan p;
+    const uint64_t rows = max_new * (q_heads / c->kv_heads);
+    p.rows_per_tile = attn_rows_per_tile(dtype, c->head_dim, rows);
+    p.row_tiles = (uint32_t)((rows + p.rows_per_tile - 1) / p.rows_per_tile);
+    const uint64_t steps = table_width * c->block_tokens / 16;
+    const uint64_t most = (seqs * p.row_tiles * c->kv_heads * (steps ? steps : 1) + ATTN_MIN_STEPS - 1) / ATTN_MIN_STEPS;
+    const uint64_t fit = (uint64_t)sms * attn_ctas_per_sm(dtype, c->head_dim, p.rows_per_tile);
+    p.ctas = (uint32_t)(most < fit ? most : fit);
+    p.ml = (uint64_t)2 * ATTN_WARPS * p.ctas * p.rows_per_tile;
+    p.o_floats = p.ml * c->head_dim;
+    p.items = seqs * p.row_tiles * c->kv_heads;
+    p.bytes = p.o_floats * sizeof(float) + p.ml * sizeof(float2) + p.items * sizeof(int2);
+    return p;
 }
 
 }  // namespace
@@ -227,8 +238,6 @@ int ltq_cache_append(const ltq_kv_cache *cache, const void *k_dev, const void *v
     return LTQ_OK;
 }
 
-// Partial results of every split: head_dim sums and {maximum, sum} per row.  The float form has the fewest rows per tile, so its
-// split count, the smallest or equal, is not the bound: take the larger of the two.
 uint64_t ltq_cache_attention_workspace(const ltq_kv_cache *cache, uint64_t tokens, uint32_t q_heads, uint64_t seqs, uint64_t table_width,
                                        uint64_t max_new, int device)
 {
@@ -236,10 +245,9 @@ uint64_t ltq_cache_attention_workspace(const ltq_kv_cache *cache, uint64_t token
     DeviceGuard guard(device);
     GemmDevice *dev;
     if (guard.err != cudaSuccess || device_state(device, &dev) != LTQ_OK) return 0;
-    const uint32_t a = attn_plan(cache, LTQ_F32, q_heads, seqs, table_width, max_new, dev->sms);
-    const uint32_t b = attn_plan(cache, LTQ_BF16, q_heads, seqs, table_width, max_new, dev->sms);
-    const uint64_t s = a > b ? a : b;
-    return s == 1 ? 16 : s * tokens * q_heads * (cache->head_dim + 2) * sizeof(float);
+    const uint64_t a = attn_plan(cache, LTQ_F32, q_heads, seqs, table_width, max_new, dev->sms).bytes;
+    const uint64_t b = attn_plan(cache, LTQ_BF16, q_heads, seqs, table_width, max_new, dev->sms).bytes;
+    return a > b ? a : b;   // the type of q is not known here
 }
 
 int ltq_cache_attention(const ltq_kv_cache *cache, const void *q_dev, int dtype, uint64_t ld_q, uint64_t tokens, uint32_t q_heads,
@@ -276,13 +284,16 @@ int ltq_cache_attention(const ltq_kv_cache *cache, const void *q_dev, int dtype,
     a.q_heads = q_heads;
     a.group = q_heads / cache->kv_heads;
     a.scale_log2 = scale * 1.4426950408889634f;
-    a.splits = attn_plan(cache, dtype, q_heads, seqs, table_width, max_new, dev->sms);
-    const uint64_t rows = a.splits * tokens * q_heads;
-    LTQ_REQUIRE(a.splits == 1 || workspace_bytes >= rows * (cache->head_dim + 2) * sizeof(float), LTQ_ERR_INVALID_ARG,
-                "the workspace holds %llu bytes, %llu are needed", (unsigned long long)workspace_bytes,
-                (unsigned long long)(rows * (cache->head_dim + 2) * sizeof(float)));
+    const AttnPlan p = attn_plan(cache, dtype, q_heads, seqs, table_width, max_new, dev->sms);
+    LTQ_REQUIRE(workspace_bytes >= p.bytes, LTQ_ERR_INVALID_ARG, "the workspace holds %llu bytes, %llu are needed",
+                (unsigned long long)workspace_bytes, (unsigned long long)p.bytes);
+    a.q_vec = ld_q % 4 == 0 && ((uintptr_t)q_dev % (4 * dtype_size(dtype))) == 0;
+    a.out_vec = ((uintptr_t)out_dev % (4 * dtype_size(dtype))) == 0;
+    a.ctas = p.ctas;
+    a.row_tiles = p.row_tiles;
     a.part_o = static_cast<float *>(workspace_dev);
-    a.part_ml = reinterpret_cast<float2 *>(a.part_o + rows * cache->head_dim);
+    a.part_ml = reinterpret_cast<float2 *>(a.part_o + p.o_floats);
+    a.item = reinterpret_cast<int2 *>(a.part_ml + p.ml);
     cudaStream_t st = (cudaStream_t)stream;
     LTQ_CUDA_TRY(dtype == LTQ_F32 ? launch_attention_f32(a, st) : (dtype == LTQ_F16 ? launch_attention_f16(a, st) : launch_attention_bf16(a, st)));
     return LTQ_OK;

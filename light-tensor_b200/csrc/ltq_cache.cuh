@@ -18,7 +18,7 @@ struct CacheSeq {
     int32_t off, n, len;    // first row, tokens of this call, tokens in all
     bool ok;
 };
-// Reads and checks sequence b; every CTA that meets a bad one reports it.
+// Reads and checks sequence b.
 __device__ __forceinline__ CacheSeq cache_seq(const CacheBatch &bt, uint32_t b)
 {
     CacheSeq s;
@@ -28,7 +28,6 @@ __device__ __forceinline__ CacheSeq cache_seq(const CacheBatch &bt, uint32_t b)
     s.n = e - a;
     s.ok = a >= 0 && e >= a && (uint64_t)e <= bt.tokens && (uint32_t)s.n <= bt.max_new && s.len >= 0 &&
            (uint64_t)s.len <= ((uint64_t)bt.table_width << bt.log2_bt);
-    if (!s.ok && threadIdx.x == 0) atomicCAS(bt.status, 0u, STATUS_BAD_SEQUENCE);
     return s;
 }
 
@@ -43,12 +42,20 @@ struct AttnArgs {
     uint64_t ld_q;
     uint32_t q_heads, group;       // group = q_heads / kv_heads
     float scale_log2;              // softmax scale * log2(e)
-    uint32_t splits;               // CTAs that share one sequence's keys
-    float *part_o;                 // [splits][tokens][q_heads][head_dim]
-    float2 *part_ml;               // [splits][tokens][q_heads]: running maximum (base 2), sum
+    bool q_vec, out_vec;           // rows start aligned to four elements
+    // Workspace: what warps leave of (row tile, head) items that they share with other warps, see ltq_cache_attention.cuh.
+    float *part_o;                 // [2 * warps][rows per tile][head_dim]
+    float2 *part_ml;               // [2 * warps][rows per tile]: running maximum (base 2), sum
+    int2 *item;                    // [seqs][row tiles][kv_heads]: first slot, last warp
+    uint32_t ctas, row_tiles;
 };
+constexpr uint32_t ATTN_WARPS = 4;             // per CTA
+constexpr uint32_t ATTN_MIN_STEPS = 4;         // fewer 16-key steps than this are not worth a warp of their own
+constexpr uint64_t ATTN_FEW_ROWS = 1184;       // eight CTAs on each of 148 SMs
 // Rows of (token, head of the group) that one CTA of the attention kernel takes.
 uint32_t attn_rows_per_tile(int dtype, uint32_t head_dim, uint64_t rows);
+// CTAs of it that fit an SM at once.
+uint32_t attn_ctas_per_sm(int dtype, uint32_t head_dim, uint32_t rows_per_tile);
 cudaError_t launch_attention_f32(const AttnArgs &a, cudaStream_t stream);
 cudaError_t launch_attention_f16(const AttnArgs &a, cudaStream_t stream);
 cudaError_t launch_attention_bf16(const AttnArgs &a, cudaStream_t stream);

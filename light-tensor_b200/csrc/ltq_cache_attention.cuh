@@ -13,12 +13,23 @@
 // lane (g = lane / 4, c = lane % 4) takes 16 neighbouring bytes of keys g and g + 8 for K and of keys 2c, 2c+1, 2c+8,
 // 2c+9 for V: wide loads, whole sectors.  P^T leaves the accumulators transposed and is turned with movmatrix.
 //
-// A code b becomes the half 1024 + b by putting 0x64 above it (a byte permute) and (code - zero point) by one exact
-// subtraction; block scales multiply the float results.  q is scaled by a power of two per row so that halves hold it;
-// float q is split into two halves (22 bits), and so are the probabilities then.
+// The next step's bytes are on their way into registers while a step is computed (4 KB per warp at head_dim 128, 48 KB per SM).
 //
-// Softmax keeps its running maximum only approximately: the reference value m moves when some score exceeds it by more
-// than 8 (in base 2), so that probabilities stay below 2^8 and almost every step does without a reduction over lanes.
+// Work is divided evenly whatever the lengths are: the steps of all (sequence, row tile, head) items in a row are cut into
+// equal ranges, one per resident warp.  A warp finishes the items that lie inside its range and leaves its part of the one
+// or two that reach beyond it in the workspace, for the join kernel.  Warps never wait for one another, so that the start and
+// end of one's range passes under the others' reading.  (Ranges per CTA, its warps joined in shared memory: 27 us of the
+// 126 us of 64 sequences of 2048 to 8192 tokens went there.)
+//
+// Past that the kernel is bound by instruction issue, so a step is kept short:
+//  * a code b with a zero byte above it IS a half, the subnormal b * 2^-24, which the tensor core multiplies exactly: one byte
+//    permute per two codes.  Zero points come off the sums: q . (k - z) = q . k - z * sum(q), and p . (v - z) = p . v - z * sum(p)
+//    with p as rounded for the MMA;
+//  * q is scaled by a power of two per row so that halves hold it (float q: split into two halves, 22 bits, and so are
+//    the probabilities then);
+//  * V's block scales go into the probabilities as a ratio to the largest one so far, so that one accumulator serves all;
+//  * the running maximum is kept only approximately: the reference m moves when a score exceeds it by more than 8 (base 2), so
+//    that probabilities stay below 2^8 and almost every step does without a reduction over lanes.
 #include <cuda_fp16.h>
 
 #include "ltq_cache.cuh"
@@ -30,15 +41,14 @@ namespace {
 
 constexpr int DT = LTQ_ATTN_DT;
 constexpr int TERMS = DT == LTQ_F32 ? 2 : 1;
-constexpr int WARPS = 4;
+constexpr int WARPS = ATTN_WARPS;
+constexpr float SMALLEST_SCALE = 1.17549435e-38f;   // 2^-126
+#ifndef AHEAD
+constexpr uint32_t AHEAD = 2;     // steps beyond the one on its way into registers that are asked into L2
+#endif
 constexpr float MAX_STEP = 8.f;   // how far a score may exceed the reference maximum before it moves
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
-__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b)
-{
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
-    return *reinterpret_cast<const uint32_t *>(&r);
-}
 __device__ __forceinline__ uint32_t pack2(float lo, float hi)
 {
     const __half2 r = __floats2half2_rn(lo, hi);
@@ -88,62 +98,90 @@ struct Geo {
     }
 };
 
-// `n` words starting at p, in the widest loads that the geometry guarantees (see k_dim / v_dim).
-__device__ __forceinline__ void load_words(uint32_t *w, const uint8_t *p, int n)
-{
-    if (n == 4) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
-        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-    } else if (n == 2) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
-        w[0] = v.x; w[1] = v.y;
-    } else {
-        w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
-    }
-}
+// The pieces (16, 8 and 4 bytes) that a lane holds of one key, for K and for V.
+template <int D>
+struct Piece {
+    static constexpr int K16 = D / 64, K8 = (D % 64) / 32;
+    static constexpr int V16 = D / 128, V8 = (D % 128) >= 64, V4 = (D % 64) / 32;
+};
 
-// What a lane holds of 16 keys.
+// Byte offsets of a lane's first piece of each size within 16 keys, the rest lies at constant distances from them.
+template <int D>
+struct LaneOffsets {
+    uint32_t k16, k8, v16, v8, v4;
+    __device__ __forceinline__ LaneOffsets(int lane)
+    {
+        const int g = lane >> 2, c = lane & 3;
+        k16 = g * D + Geo<D>::k_dim(0, c);
+        k8 = g * D + Geo<D>::k_dim(Geo<D>::KW - 1, c) - 4;
+        v16 = 2 * c * D + Geo<D>::v_dim(0, g);
+        v8 = 2 * c * D + Geo<D>::v_dim(4 * Piece<D>::V16, g);
+        v4 = 2 * c * D + Geo<D>::v_dim(Geo<D>::VW - 1, g);
+    }
+};
+
+// What a lane holds of 16 keys, and their block's parameters.
 template <int D>
 struct Keys {
     uint32_t k[2][Geo<D>::KW];   // keys g, g + 8
     uint32_t v[4][Geo<D>::VW];   // keys 2c, 2c+1, 2c+8, 2c+9
-    float ks, vs;
-    uint32_t kz, vz;             // 1024 + zero point as a pair of halves
+    uint2 k_par, v_par;          // scale, zero point
     bool bad;                    // the block id is out of range: none of these keys exists
 };
 
+__device__ __forceinline__ void load16(uint32_t *w, const uint8_t *p)
+{
+    const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p));
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+}
+__device__ __forceinline__ void load8(uint32_t *w, const uint8_t *p)
+{
+    const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
+    w[0] = x.x; w[1] = x.y;
+}
+
 template <int D>
-__device__ __forceinline__ void load_keys(Keys<D> &t, const AttnArgs &a, int32_t page, uint32_t h, uint32_t key_in_block, int g, int c)
+__device__ __forceinline__ void fetch_keys(Keys<D> &t, const AttnArgs &a, const LaneOffsets<D> &at, int32_t page, uint32_t h, uint32_t key_in_block)
 {
     t.bad = (uint32_t)page >= a.cache.blocks;
     if (t.bad) {
         page = 0;
         if (threadIdx.x % 32 == 0) atomicCAS(a.bt.status, 0u, STATUS_BAD_BLOCK);
     }
-    const uint64_t slot = (uint64_t)(uint32_t)page * a.cache.kv_heads + h;
-    const uint2 kq = __ldg(reinterpret_cast<const uint2 *>(a.cache.k_qp_dev + slot)), vq = __ldg(reinterpret_cast<const uint2 *>(a.cache.v_qp_dev + slot));
-    t.ks = __uint_as_float(kq.x);
-    t.vs = __uint_as_float(vq.x);
-    t.kz = pack2(1024.f + (float)(kq.y & 0xFF), 1024.f + (float)(kq.y & 0xFF));
-    t.vz = pack2(1024.f + (float)(vq.y & 0xFF), 1024.f + (float)(vq.y & 0xFF));
-    const uint64_t base = ((slot << a.bt.log2_bt) + key_in_block) * D;
+    const uint64_t slot = (uint64_t)(uint32_t)page * a.cache.kv_heads + h, base = ((slot << a.bt.log2_bt) + key_in_block) * D;
+    t.k_par = __ldg(reinterpret_cast<const uint2 *>(a.cache.k_qp_dev + slot));
+    t.v_par = __ldg(reinterpret_cast<const uint2 *>(a.cache.v_qp_dev + slot));
+    const uint8_t *k = a.cache.k_dev + base, *v = a.cache.v_dev + base;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        const uint8_t *p = a.cache.k_dev + base + (uint64_t)(g + 8 * i) * D;
 #pragma unroll
-        for (int w = 0; w < Geo<D>::KW; w += 4) {
-            constexpr int KW = Geo<D>::KW;
-            load_words(t.k[i] + w, p + Geo<D>::k_dim(w, c), KW - w >= 4 ? 4 : KW - w);
-        }
+        for (int j = 0; j < Piece<D>::K16; j++) load16(t.k[i] + 4 * j, k + at.k16 + (8 * i * D + 64 * j));
+        if (Piece<D>::K8) load8(t.k[i] + 4 * Piece<D>::K16, k + at.k8 + 8 * i * D);
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const uint8_t *p = a.cache.v_dev + base + (uint64_t)(2 * c + (i & 1) + 8 * (i >> 1)) * D;
-        constexpr int P = D / 128, REST = D - P * 128;
+        const int key = ((i & 1) + 8 * (i >> 1)) * D;
 #pragma unroll
-        for (int w = 0; w < 4 * P; w += 4) load_words(t.v[i] + w, p + Geo<D>::v_dim(w, g), 4);
-        if (REST >= 64) load_words(t.v[i] + 4 * P, p + Geo<D>::v_dim(4 * P, g), 2);
-        if (REST == 32 || REST == 96) load_words(t.v[i] + Geo<D>::VW - 1, p + Geo<D>::v_dim(Geo<D>::VW - 1, g), 1);
+        for (int j = 0; j < Piece<D>::V16; j++) load16(t.v[i] + 4 * j, v + at.v16 + (key + 128 * j));
+        if (Piece<D>::V8) load8(t.v[i] + 4 * Piece<D>::V16, v + at.v8 + key);
+        if (Piece<D>::V4) t.v[i][Geo<D>::VW - 1] = __ldg(reinterpret_cast<const uint32_t *>(v + at.v4 + key));
+    }
+}
+
+// Asks 16 keys of a block into L2: one line per lane and round.
+template <int D>
+__device__ __forceinline__ void ask_keys(const AttnArgs &a, int32_t page, uint32_t h, uint32_t key_in_block, int lane)
+{
+    if ((uint32_t)page >= a.cache.blocks) return;
+    const uint64_t base = ((((uint64_t)(uint32_t)page * a.cache.kv_heads + h) << a.bt.log2_bt) + key_in_block) * D;
+    constexpr int LINES = 16 * D / 128;   // of K, and of V
+#pragma unroll
+    for (int i = 0; i < (2 * LINES + 31) / 32; i++) {
+        const int line = i * 32 + lane;
+        if (line < 2 * LINES) {
+            const uint8_t *p = (line < LINES ? a.cache.k_dev + base + line * 128 : a.cache.v_dev + base + (line - LINES) * 128);
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+        }
     }
 }
 
@@ -151,15 +189,21 @@ template <int D, int NT>
 struct Rows {
     uint32_t q[TERMS][NT][D / 16][2];   // Q^T operand
     float scale[NT][2];                 // softmax scale (base 2) over q's power of two, rows 2c and 2c + 1 of each tile
-    int pos[NT][2];                     // position of those rows' tokens; -1: no such row
+    float q_sum[NT][2];                 // sum of the row's q, as the operand holds it
+    int pos[NT][2];                     // position of those rows' tokens (rows that do not exist see everything, with q = 0)
+    int first_pos;                      // the smallest of the warp's
     float m[NT][2], l[NT][2];
-    float o[D / 16][NT][4];
+    float o[D / 16][NT][4];             // 2^-24 * sum of probability * V scale / v_ref * code
+    float zp[NT][2];                    // sum of probability * V scale / v_ref * zero point
+    float v_ref, v_inv;                 // largest V scale so far and its inverse
 };
+constexpr float CODE = 16777216.f;      // 2^24: a code's half is the code over this
 
 template <int D, int NT>
 __device__ __forceinline__ void load_rows(Rows<D, NT> &r, const AttnArgs &a, const CacheSeq &s, uint32_t h, uint32_t row0, int g, int c)
 {
     using T = typename std::conditional<DT == LTQ_F32, float, uint16_t>::type;
+    using Four = typename std::conditional<DT == LTQ_F32, float4, uint2>::type;
     const T *q = static_cast<const T *>(a.q);
     const uint32_t rows = (uint32_t)s.n * a.group;
 #pragma unroll
@@ -173,15 +217,21 @@ __device__ __forceinline__ void load_rows(Rows<D, NT> &r, const AttnArgs &a, con
 #pragma unroll
         for (int w = 0; w < D / 16; w++) {
             const int d = Geo<D>::k_dim(w, c);
+            T raw[4] = {0, 0, 0, 0};
+            if (real) {
+                if (a.q_vec) {
+                    *reinterpret_cast<Four *>(raw) = __ldg(reinterpret_cast<const Four *>(p + d));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) raw[i] = p[d + i];
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                float v = 0.f;
-                if (real) {
-                    const T raw = p[d + i];
-                    if constexpr (DT == LTQ_F32) v = raw;
-                    else if constexpr (DT == LTQ_F16) v = __half2float(__ushort_as_half(raw));
-                    else v = __uint_as_float((uint32_t)raw << 16);
-                }
+                float v;
+                if constexpr (DT == LTQ_F32) v = raw[i];
+                else if constexpr (DT == LTQ_F16) v = __half2float(__ushort_as_half(raw[i]));
+                else v = __uint_as_float((uint32_t)raw[i] << 16);
                 x[w][i] = v;
                 finite = finite && fabsf(v) < INFINITY;
                 most = fmaxf(most, fabsf(v));
@@ -199,24 +249,33 @@ __device__ __forceinline__ void load_rows(Rows<D, NT> &r, const AttnArgs &a, con
             e = e > 100 ? 100 : e;
         }
         const float f = ldexpf(1.f, e);
-        float sc = finite ? a.scale_log2 * ldexpf(1.f, -e) : __int_as_float(0x7FC00000);   // an infinity or NaN: the row becomes NaN
+        const float sc = finite ? a.scale_log2 * ldexpf(1.f, -e) : __int_as_float(0x7FC00000);   // an infinity or NaN: the row becomes NaN
+        float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < D / 16; w++) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const float u = finite ? x[w][2 * i] * f : 0.f, v = finite ? x[w][2 * i + 1] * f : 0.f;
                 const uint32_t hi = pack2(u, v);
+                const float2 b = unpack2(hi);
                 r.q[0][nt][w][i] = hi;
+                sum += b.x + b.y;
                 if (TERMS == 2) {
-                    const float2 b = unpack2(hi);
-                    r.q[TERMS - 1][nt][w][i] = pack2(u - b.x, v - b.y);
+                    const uint32_t lo = pack2(u - b.x, v - b.y);
+                    const float2 d = unpack2(lo);
+                    r.q[TERMS - 1][nt][w][i] = lo;
+                    sum += d.x + d.y;
                 }
             }
         }
-        const int pos = real ? s.len - s.n + (int)t : -1;
+#pragma unroll
+        for (int o = 1; o <= 2; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        const int pos = real ? s.len - s.n + (int)t : 0x7FFFFFFF;
 #pragma unroll
         for (int j = 0; j < 2; j++) {   // rows 2c + j live in lanes with g = 2c + j
             r.scale[nt][j] = __shfl_sync(0xFFFFFFFFu, sc, (2 * c + j) * 4);
+            r.q_sum[nt][j] = __shfl_sync(0xFFFFFFFFu, sum, (2 * c + j) * 4);
+            r.zp[nt][j] = 0.f;
             r.pos[nt][j] = __shfl_sync(0xFFFFFFFFu, pos, (2 * c + j) * 4);
             r.m[nt][j] = -INFINITY;
             r.l[nt][j] = 0.f;
@@ -228,48 +287,87 @@ __device__ __forceinline__ void load_rows(Rows<D, NT> &r, const AttnArgs &a, con
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int j = 0; j < 4; j++) r.o[i][nt][j] = 0.f;
+    int first = 0x7FFFFFFF;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) first = min(first, min(r.pos[nt][0], r.pos[nt][1]));
+    r.first_pos = __reduce_min_sync(0xFFFFFFFFu, first);
+    r.v_ref = SMALLEST_SCALE;
+    r.v_inv = 1.f / SMALLEST_SCALE;
 }
 
 // Scores, softmax and accumulation for 16 keys, the first at position key0.
 template <int D, int NT>
-__device__ __forceinline__ void take_keys(Rows<D, NT> &r, const Keys<D> &t, int key0, int g)
+__device__ __forceinline__ void take_keys(Rows<D, NT> &r, const Keys<D> &keys, int key0, int g)
 {
-    const uint32_t magic = 0x64646464u;
-    float s[NT][4];
+    const float k_scale = __uint_as_float(keys.k_par.x), v_scale = __uint_as_float(keys.v_par.x);
+    const float k_zero = (float)(keys.k_par.y & 0xFF), v_zero = (float)(keys.v_par.y & 0xFF);
+    const bool bad = keys.bad;
+    float acc[NT][2][4];   // two chains: an MMA waits for the one before it on the same accumulator
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) s[nt][j] = 0.f;
+        for (int j = 0; j < 4; j++) acc[nt][0][j] = acc[nt][1][j] = 0.f;
 #pragma unroll
     for (int w = 0; w < D / 16; w++) {
-        const uint32_t a0 = sub2(prmt(t.k[0][w], magic, 0x4140), t.kz), a2 = sub2(prmt(t.k[0][w], magic, 0x4342), t.kz);
-        const uint32_t a1 = sub2(prmt(t.k[1][w], magic, 0x4140), t.kz), a3 = sub2(prmt(t.k[1][w], magic, 0x4342), t.kz);
+        const uint32_t a0 = prmt(keys.k[0][w], 0, 0x4140), a2 = prmt(keys.k[0][w], 0, 0x4342);
+        const uint32_t a1 = prmt(keys.k[1][w], 0, 0x4140), a3 = prmt(keys.k[1][w], 0, 0x4342);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int i = 0; i < TERMS; i++) mma16816(s[nt], a0, a1, a2, a3, r.q[i][nt][w][0], r.q[i][nt][w][1]);
+            for (int i = 0; i < TERMS; i++) mma16816(acc[nt][w & 1], a0, a1, a2, a3, r.q[i][nt][w][0], r.q[i][nt][w][1]);
     }
-    bool up = false;
+
+    // t = score - m.  Of element j: row 2c + (j & 1), key g + 8 * (j >> 1).
+    float t[NT][4], sc[NT][2], zo[NT][2];
+    const bool masked = bad || key0 + 15 > r.first_pos;
+    float top = -INFINITY;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const float x = r.scale[nt][j] * k_scale;
+            sc[nt][j] = x * CODE;
+            zo[nt][j] = x * (k_zero * r.q_sum[nt][j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            acc[nt][0][j] += acc[nt][1][j];
+            t[nt][j] = fmaf(acc[nt][0][j], sc[nt][j & 1], -(zo[nt][j & 1] + r.m[nt][j & 1]));
+        }
+    }
+    auto mask = [&](float (&x)[NT][4]) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (bad || key0 + g + 8 * (j >> 1) > r.pos[nt][j & 1]) x[nt][j] = -INFINITY;
+    };
+    if (masked) mask(t);
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {   // j & 1: row 2c + (j & 1); j >> 1: key g or g + 8
-            const int key = key0 + g + 8 * (j >> 1);
-            s[nt][j] = (key <= r.pos[nt][j & 1] && !t.bad) ? s[nt][j] * (r.scale[nt][j & 1] * t.ks) : -INFINITY;
-            up = up || s[nt][j] > r.m[nt][j & 1] + MAX_STEP;
-        }
-    if (__any_sync(0xFFFFFFFFu, up)) {
+        for (int j = 0; j < 4; j++) top = fmaxf(top, t[nt][j]);
+    if (__any_sync(0xFFFFFFFFu, top > MAX_STEP)) {   // (also the first time: m is -inf, t +inf)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) t[nt][j] = fmaf(acc[nt][0][j], sc[nt][j & 1], -zo[nt][j & 1]);
+        if (masked) mask(t);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                float mx = fmaxf(s[nt][j], s[nt][j + 2]);
+                float mx = fmaxf(t[nt][j], t[nt][j + 2]);
 #pragma unroll
                 for (int o = 4; o <= 16; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
                 mx = fmaxf(mx, r.m[nt][j]);
                 const float alpha = r.m[nt][j] == mx ? 1.f : exp2_fast(r.m[nt][j] - mx);   // (both -inf: nothing there yet)
+                const float m = mx == -INFINITY ? 0.f : mx;
+                t[nt][j] -= m;
+                t[nt][j + 2] -= m;
                 r.m[nt][j] = mx;
                 r.l[nt][j] *= alpha;
+                r.zp[nt][j] *= alpha;
 #pragma unroll
                 for (int i = 0; i < D / 16; i++) {
                     r.o[i][nt][j] *= alpha;
@@ -277,179 +375,319 @@ __device__ __forceinline__ void take_keys(Rows<D, NT> &r, const Keys<D> &t, int 
                 }
             }
     }
+    if (v_scale > r.v_ref) {   // the same in all lanes
+        const float f = r.v_ref * __fdividef(1.f, v_scale);
+        r.v_ref = v_scale;
+        r.v_inv = __fdiv_rn(1.f, v_scale);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) r.zp[nt][j] *= f;
+#pragma unroll
+            for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) r.o[i][nt][j] *= f;
+        }
+    }
+    const float ratio = v_scale * r.v_inv;
     uint32_t p[TERMS][NT][2];
-    float vs[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const float m = r.m[nt][j & 1];
-            s[nt][j] = exp2_fast(s[nt][j] - (m == -INFINITY ? 0.f : m));
-            r.l[nt][j & 1] += s[nt][j];
+            t[nt][j] = exp2_fast(t[nt][j]);
+            r.l[nt][j & 1] += t[nt][j];
+        }
+        float f0 = ratio, f1 = ratio;
+        if (ratio != ratio) {   // a block whose scale is NaN must not reach rows that see none of its keys (0 * NaN)
+            f0 = key0 <= r.pos[nt][0] && !bad ? ratio : 0.f;
+            f1 = key0 <= r.pos[nt][1] && !bad ? ratio : 0.f;
         }
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const uint32_t hi = pack2(s[nt][2 * i], s[nt][2 * i + 1]);
+            const float x = t[nt][2 * i] * f0, y = t[nt][2 * i + 1] * f1;
+            const uint32_t hi = pack2(x, y);
+            float2 b = unpack2(hi);
             p[0][nt][i] = movmatrix(hi);
             if (TERMS == 2) {
-                const float2 b = unpack2(hi);
-                p[TERMS - 1][nt][i] = movmatrix(pack2(s[nt][2 * i] - b.x, s[nt][2 * i + 1] - b.y));
+                const uint32_t lo = pack2(x - b.x, y - b.y);
+                const float2 d = unpack2(lo);
+                p[TERMS - 1][nt][i] = movmatrix(lo);
+                b.x += d.x;
+                b.y += d.y;
             }
+            r.zp[nt][0] = fmaf(v_zero, b.x, r.zp[nt][0]);
+            r.zp[nt][1] = fmaf(v_zero, b.y, r.zp[nt][1]);
         }
-        // a block whose scale is NaN must not reach rows that see none of its keys (0 * NaN)
-#pragma unroll
-        for (int j = 0; j < 2; j++) vs[nt][j] = (t.vs == t.vs || (key0 <= r.pos[nt][j] && !t.bad)) ? t.vs : 0.f;
     }
 #pragma unroll
     for (int w = 0; w < D / 32; w++) {
 #pragma unroll
         for (int half = 0; half < 2; half++) {
             const uint32_t sel = half ? 0x7362 : 0x5140;
-            const uint32_t x = prmt(t.v[0][w], t.v[1][w], sel), y = prmt(t.v[2][w], t.v[3][w], sel);
-            const uint32_t a0 = sub2(prmt(x, magic, 0x4140), t.vz), a1 = sub2(prmt(x, magic, 0x4342), t.vz);
-            const uint32_t a2 = sub2(prmt(y, magic, 0x4140), t.vz), a3 = sub2(prmt(y, magic, 0x4342), t.vz);
+            const uint32_t x = prmt(keys.v[0][w], keys.v[1][w], sel), y = prmt(keys.v[2][w], keys.v[3][w], sel);
+            const uint32_t a0 = prmt(x, 0, 0x4140), a1 = prmt(x, 0, 0x4342), a2 = prmt(y, 0, 0x4140), a3 = prmt(y, 0, 0x4342);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int i = 0; i < TERMS; i++) mma16816(d, a0, a1, a2, a3, p[i][nt][0], p[i][nt][1]);
-#pragma unroll
-                for (int j = 0; j < 4; j++) r.o[2 * w + half][nt][j] = fmaf(vs[nt][j & 1], d[j], r.o[2 * w + half][nt][j]);
-            }
+                for (int i = 0; i < TERMS; i++) mma16816(r.o[2 * w + half][nt], a0, a1, a2, a3, p[i][nt][0], p[i][nt][1]);
         }
     }
 }
 
-template <int D, int NT>
-struct Shared {
-    float o[WARPS][8 * NT][D + 4];   // + 4: rows start in different banks
-    float m[WARPS][8 * NT], l[WARPS][8 * NT];
-};
-
-// Grid: (splits * row tiles, kv_heads, sequences).  The keys that a row tile can see are cut into `splits` equal runs of 16-key
-// steps, a run into four for the warps; the four results meet in shared memory.
-template <int D, int NT>
-__global__ void __launch_bounds__(32 * WARPS)
-cache_attention_kernel(const AttnArgs a, uint32_t row_tiles)
+// Steps of one (row tile, head) of a sequence: 16 keys each, by its longest row tile, and at least one (rows without keys get
+// their zeros that way).  Row tiles of a long run of new tokens see fewer keys than the last one does; their surplus is empty.
+__device__ __forceinline__ uint32_t item_steps(const CacheSeq &s) { return s.len > 16 ? ((uint32_t)s.len + 15) / 16 : 1u; }
+__device__ __forceinline__ unsigned long long seq_steps(const AttnArgs &a, const CacheSeq &s, uint32_t rows_per_tile)
 {
-    griddep_launch_dependents();
-    griddep_wait();
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    Shared<D, NT> &sh = *reinterpret_cast<Shared<D, NT> *>(smem_raw);
-    const uint32_t b = blockIdx.z, h = blockIdx.y, split = blockIdx.x / row_tiles, row0 = (blockIdx.x - split * row_tiles) * 8 * NT;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const CacheSeq s = cache_seq(a.bt, b);
-    const uint32_t rows = s.ok ? (uint32_t)s.n * a.group : 0u;
-    if (row0 >= rows) return;
+    if (!s.ok || s.n == 0) return 0;
+    return (unsigned long long)item_steps(s) * (((uint32_t)s.n * a.group + rows_per_tile - 1) / rows_per_tile) * a.cache.kv_heads;
+}
+// How many warps take part: none with fewer than MIN_STEPS steps.
+__device__ __forceinline__ unsigned long long active_warps(const AttnArgs &a, unsigned long long total)
+{
+    const unsigned long long most = (total + ATTN_MIN_STEPS - 1) / ATTN_MIN_STEPS, there = (unsigned long long)a.ctas * WARPS;
+    return most < there ? most : there;
+}
+
+template <int D>
+__device__ __forceinline__ void store4(const AttnArgs &a, uint64_t row, int d, float x, float y, float z, float w)
+{
+    if constexpr (DT == LTQ_F32) {
+        float *p = static_cast<float *>(a.out) + row * D + d;
+        if (a.out_vec) *reinterpret_cast<float4 *>(p) = make_float4(x, y, z, w);
+        else p[0] = x, p[1] = y, p[2] = z, p[3] = w;
+    } else {
+        uint16_t *p = static_cast<uint16_t *>(a.out) + row * D + d;
+        const uint32_t lo = token_bits2<DT>(x, y), hi = token_bits2<DT>(z, w);
+        if (a.out_vec) *reinterpret_cast<uint2 *>(p) = make_uint2(lo, hi);
+        else p[0] = (uint16_t)lo, p[1] = (uint16_t)(lo >> 16), p[2] = (uint16_t)hi, p[3] = (uint16_t)(hi >> 16);
+    }
+}
+
+// One warp's part [first, end) of the steps of one item; the result goes to `out` if the part is the whole item, to workspace
+// slot `slot` otherwise.
+template <int D, int NT>
+__device__ __forceinline__ void do_segment(const AttnArgs &a, uint32_t b, const CacheSeq &s, uint32_t h, uint32_t row0, uint32_t first,
+                                           uint32_t end, bool whole, uint32_t slot)
+{
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const uint32_t rows = (uint32_t)s.n * a.group;
     const uint32_t last = row0 + 8 * NT < rows ? row0 + 8 * NT - 1 : rows - 1;
     const int keys = s.len - s.n + (int)(last / a.group) + 1;             // what the tile's last row sees
-    const uint32_t steps = keys > 0 ? ((uint32_t)keys + 15) / 16 : 0u;
-    const uint32_t c0 = (uint32_t)((uint64_t)steps * split / a.splits), c1 = (uint32_t)((uint64_t)steps * (split + 1) / a.splits);
-    const uint32_t w0 = c0 + (c1 - c0) * warp / WARPS, w1 = c0 + (c1 - c0) * (warp + 1) / WARPS;
+    const uint32_t seen = keys > 0 ? ((uint32_t)keys + 15) / 16 : 0u, w0 = first, w1 = end < seen ? end : seen;
 
+    const int32_t *table = a.bt.table + (uint64_t)b * a.bt.table_width;
+    const int sh16 = a.bt.log2_bt - 4;                                    // steps per block, log2
+    const uint32_t in_block = (1u << sh16) - 1;
+    const LaneOffsets<D> at(lane);
     Rows<D, NT> r;
-    load_rows<D, NT>(r, a, s, h, row0, g, c);
-    if (w0 < w1) {
-        const int32_t *table = a.bt.table + (uint64_t)b * a.bt.table_width;
-        const int sh16 = a.bt.log2_bt - 4;                    // steps per block, log2
-        const uint32_t in_block = (1u << sh16) - 1;
-        Keys<D> cur, nxt;
-        load_keys<D>(cur, a, __ldg(table + (w0 >> sh16)), h, (w0 & in_block) * 16, g, c);
-        int32_t page = w0 + 1 < w1 ? __ldg(table + ((w0 + 1) >> sh16)) : 0;
-        for (uint32_t st = w0; st < w1; st++) {
-            if (st + 1 < w1) load_keys<D>(nxt, a, page, h, ((st + 1) & in_block) * 16, g, c);
-            if (st + 2 < w1) page = __ldg(table + ((st + 2) >> sh16));
-            take_keys<D, NT>(r, cur, (int)(st * 16), g);
-            cur = nxt;
+    Keys<D> even, odd;
+    int32_t page = 0, page_ahead = 0;   // blocks of the steps to be fetched, and to be asked into L2, next
+    auto fetch = [&](Keys<D> &into, uint32_t st) {
+        if (st < w1) {
+            fetch_keys<D>(into, a, at, page, h, (st & in_block) * 16);
+            if (st + 1 < w1) page = __ldg(table + ((st + 1) >> sh16));
         }
+    };
+    auto ask = [&](uint32_t st) {
+        if (st < w1) {
+            ask_keys<D>(a, page_ahead, h, (st & in_block) * 16, lane);
+            if (st + 1 < w1) page_ahead = __ldg(table + ((st + 1) >> sh16));
+        }
+    };
+    if (w0 < w1) page = __ldg(table + (w0 >> sh16));
+    if (w0 + 1 < w1) page_ahead = __ldg(table + ((w0 + 1) >> sh16));
+    fetch(even, w0);
+    for (uint32_t i = 1; i <= AHEAD; i++) ask(w0 + i);
+    load_rows<D, NT>(r, a, s, h, row0, g, c);
+    for (uint32_t st = w0; st < w1; st += 2) {
+        fetch(odd, st + 1);
+        ask(st + 1 + AHEAD);
+        take_keys<D, NT>(r, even, (int)(st * 16), g);
+        if (st + 1 >= w1) break;
+        fetch(even, st + 2);
+        ask(st + 2 + AHEAD);
+        take_keys<D, NT>(r, odd, (int)(st * 16) + 16, g);
     }
-    // this warp's share -> shared memory
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            float l = r.l[nt][j];
+        for (int j = 0; j < 2; j++) {   // row 2c + j of the tile: its lanes are those with the same c
+            float l = r.l[nt][j], zp = r.zp[nt][j];
 #pragma unroll
-            for (int o = 4; o <= 16; o <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
-            if (g == 0) {
-                sh.m[warp][nt * 8 + 2 * c + j] = r.m[nt][j];
-                sh.l[warp][nt * 8 + 2 * c + j] = l;
+            for (int o = 4; o <= 16; o <<= 1) {
+                l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+                zp += __shfl_xor_sync(0xFFFFFFFFu, zp, o);
             }
+            const uint32_t rr = nt * 8 + 2 * c + j, row = row0 + rr;
+            if (row >= rows) continue;
+            const uint32_t t = row / a.group;
+            const uint64_t out_row = ((uint64_t)s.off + t) * a.q_heads + h * a.group + (row - t * a.group);
+            const uint64_t place = (uint64_t)slot * 8 * NT + rr;
+            const float f = whole ? (l == 0.f ? 0.f : __fdiv_rn(r.v_ref, l)) : r.v_ref;   // (a row that sees nothing: zeros)
 #pragma unroll
             for (int w = 0; w < D / 32; w++) {
-                const float4 v = make_float4(r.o[2 * w][nt][j], r.o[2 * w][nt][j + 2], r.o[2 * w + 1][nt][j], r.o[2 * w + 1][nt][j + 2]);
-                *reinterpret_cast<float4 *>(&sh.o[warp][nt * 8 + 2 * c + j][Geo<D>::v_dim(w, g)]) = v;
+                auto real = [&](float x) { return fmaf(x, CODE, -zp) * f; };
+                const float x0 = real(r.o[2 * w][nt][j]), x1 = real(r.o[2 * w][nt][j + 2]);
+                const float x2 = real(r.o[2 * w + 1][nt][j]), x3 = real(r.o[2 * w + 1][nt][j + 2]);
+                const int d = Geo<D>::v_dim(w, g);
+                if (whole) store4<D>(a, out_row, d, x0, x1, x2, x3);
+                else *reinterpret_cast<float4 *>(a.part_o + place * D + d) = make_float4(x0, x1, x2, x3);
             }
+            if (!whole && g == 0) a.part_ml[place] = make_float2(r.m[nt][j], l);
         }
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(32 * WARPS, (D * NT * TERMS <= 128 ? 3 : 2))
+cache_attention_kernel(const __grid_constant__ AttnArgs a)
+{
+    griddep_launch_dependents();
+    griddep_wait();
+    __shared__ unsigned long long before[32 * WARPS], s_total;   // prefix sums of the sequences' steps
+    constexpr uint32_t ROWS = 8 * NT;
+    // Where this warp's range begins: every thread adds up a run of sequences, the run with the beginning is then walked.
+    const uint32_t run = (a.bt.seqs + 32 * WARPS - 1) / (32 * WARPS), b0 = threadIdx.x * run;
+    unsigned long long mine = 0;
+    for (uint32_t b = b0; b < b0 + run && b < a.bt.seqs; b++) {
+        const CacheSeq s = cache_seq(a.bt, b);
+        if (!s.ok) atomicCAS(a.bt.status, 0u, STATUS_BAD_SEQUENCE);
+        mine += seq_steps(a, s, ROWS);
+    }
+    before[threadIdx.x] = mine;
     __syncthreads();
-    using T = typename std::conditional<DT == LTQ_F32, float, uint16_t>::type;
-    T *out = static_cast<T *>(a.out);
-    for (uint32_t i = threadIdx.x; i < 8 * NT * (D / 4); i += 32 * WARPS) {
-        const uint32_t rr = i / (D / 4), d = (i - rr * (D / 4)) * 4, row = row0 + rr;
-        if (row >= rows) break;
-        float m = -INFINITY, l = 0.f;
+    if (threadIdx.x < 32) {
+        unsigned long long v[WARPS], sum = 0;
 #pragma unroll
-        for (int w = 0; w < WARPS; w++) m = fmaxf(m, sh.m[w][rr]);
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < WARPS; w++) {
-            const float mw = sh.m[w][rr], f = mw == m ? 1.f : exp2_fast(mw - m);
-            const float4 v = *reinterpret_cast<const float4 *>(&sh.o[w][rr][d]);
-            l = fmaf(f, sh.l[w][rr], l);
-            o.x = fmaf(f, v.x, o.x);
-            o.y = fmaf(f, v.y, o.y);
-            o.z = fmaf(f, v.z, o.z);
-            o.w = fmaf(f, v.w, o.w);
+        for (int k = 0; k < WARPS; k++) {
+            v[k] = before[threadIdx.x * WARPS + k];
+            sum += v[k];
         }
-        const uint32_t t = row / a.group;
-        const uint64_t at = ((uint64_t)s.off + t) * a.q_heads + h * a.group + (row - t * a.group);
-        if (a.splits > 1) {
-            const uint64_t slot = (uint64_t)split * a.bt.tokens * a.q_heads + at;
-            *reinterpret_cast<float4 *>(a.part_o + slot * D + d) = o;
-            if (d == 0) a.part_ml[slot] = make_float2(m, l);
-        } else {
-            const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);   // a row that sees nothing: zeros
-            T *p = out + at * D + d;
-            const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+        unsigned long long incl = sum;
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                if constexpr (DT == LTQ_F32) p[k] = y[k];
-                else p[k] = (T)token_bits<DT>(y[k]);
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+            if ((int)threadIdx.x >= o) incl += up;
+        }
+        if (threadIdx.x == 31) s_total = incl;
+        unsigned long long excl = incl - sum;
+#pragma unroll
+        for (int k = 0; k < WARPS; k++) {
+            before[threadIdx.x * WARPS + k] = excl;
+            excl += v[k];
+        }
+    }
+    __syncthreads();
+    // warps are numbered across the CTAs first: a small call spreads over the SMs
+    const unsigned long long total = s_total, warps = active_warps(a, total), me = (unsigned long long)(threadIdx.x >> 5) * gridDim.x + blockIdx.x;
+    if (me >= warps) return;
+    unsigned long long u = me * total / warps;
+    const unsigned long long end = (me + 1) * total / warps;
+    int lo = 0, hi = 32 * WARPS - 1;   // last run that begins at or before u (runs without steps share their beginning)
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (before[mid] <= u) lo = mid;
+        else hi = mid - 1;
+    }
+    uint32_t b = (uint32_t)lo * run;
+    unsigned long long base = before[lo];   // first step of sequence b
+    bool first_segment = true;
+    while (u < end) {
+        const CacheSeq s = cache_seq(a.bt, b);
+        const unsigned long long steps_b = seq_steps(a, s, ROWS);
+        if (u >= base + steps_b) {
+            base += steps_b;
+            b++;
+            continue;
+        }
+        const uint32_t steps = item_steps(s);
+        while (u < end && u < base + steps_b) {
+            const uint64_t item = (u - base) / steps;
+            const unsigned long long item0 = base + item * steps;
+            const uint32_t tile = (uint32_t)(item / a.cache.kv_heads), h = (uint32_t)(item - (uint64_t)tile * a.cache.kv_heads);
+            const uint32_t from = (uint32_t)(u - item0), to = end - item0 < steps ? (uint32_t)(end - item0) : steps;
+            const bool whole = from == 0 && to == steps;
+            const uint32_t slot = (uint32_t)me * 2 + (first_segment ? 0 : 1);   // a shared item is a warp's first or its last
+            if (from == 0 && (threadIdx.x & 31) == 0) {
+                // the last warp with a part of the item: the one whose range holds its last step
+                const unsigned long long last = ((item0 + steps) * warps + total - 1) / total - 1;
+                a.item[((uint64_t)b * a.row_tiles + tile) * a.cache.kv_heads + h] = make_int2((int)slot, (int)last);
             }
+            do_segment<D, NT>(a, b, s, h, tile * ROWS, from, to, whole, slot);
+            u = item0 + to;
+            first_segment = false;
         }
     }
 }
 
-// Joins the splits: one warp per (new token, query head).
-template <int D>
+// Joins the parts of shared items.  WPR warps share a row (new token and query head): one where there are many rows, eight
+// where there are few and a row may have hundreds of parts.
+template <int D, int WPR>
 __global__ void __launch_bounds__(256)
-cache_attention_join_kernel(const AttnArgs a)
+cache_attention_join_kernel(const __grid_constant__ AttnArgs a, uint32_t rows_per_tile)
 {
     griddep_launch_dependents();
     griddep_wait();
-    const int lane = threadIdx.x & 31;
+    constexpr int V = D / 32;   // values per lane
+    const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) % WPR;
     const CacheSeq s = cache_seq(a.bt, blockIdx.y);
-    const uint32_t i = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (!s.ok || i >= (uint32_t)s.n * a.q_heads) return;
-    const uint64_t at = (uint64_t)s.off * a.q_heads + i, pitch = a.bt.tokens * a.q_heads;
-    float m = -INFINITY;
-    for (uint32_t k = 0; k < a.splits; k++) m = fmaxf(m, a.part_ml[k * pitch + at].x);
-    float l = 0.f;
-    float o[(D + 31) / 32];
+    const uint32_t i = blockIdx.x * (8 / WPR) + (threadIdx.x >> 5) / WPR;
+    if (!s.ok || i >= (uint32_t)s.n * a.q_heads) return;   // (with WPR = 8 the whole CTA)
+    const uint32_t t = i / a.q_heads, head = i - t * a.q_heads, h = head / a.group;
+    const uint32_t row = t * a.group + (head - h * a.group), tile = row / rows_per_tile, rr = row - tile * rows_per_tile;
+    const int2 it = a.item[((uint64_t)blockIdx.y * a.row_tiles + tile) * a.cache.kv_heads + h];
+    const int first = it.x >> 1;
+    if (first == it.y) return;   // one warp had it all
+    // the first warp's part lies in slot it.x, those of the warps behind it in their first slots
+    float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
-    for (int j = 0; j < D / 32; j++) o[j] = 0.f;
-    for (uint32_t k = 0; k < a.splits; k++) {
-        const float2 ml = a.part_ml[k * pitch + at];
-        const float f = ml.x == m ? 1.f : exp2_fast(ml.x - m);
-        l = fmaf(f, ml.y, l);
+    for (int j = 0; j < V; j++) o[j] = 0.f;
+    constexpr int BATCH = 4;     // parts loaded before the first is used
+    for (int k0 = first + w * BATCH; k0 <= it.y; k0 += WPR * BATCH) {
+        float2 ml[BATCH];
+        float part[BATCH][V];
 #pragma unroll
-        for (int j = 0; j < D / 32; j++) o[j] = fmaf(f, a.part_o[(k * pitch + at) * D + 32 * j + lane], o[j]);
+        for (int e = 0; e < BATCH; e++) {
+            const int k = k0 + e;
+            const uint64_t place = (uint64_t)(k == first ? it.x : 2 * k) * rows_per_tile + rr;
+            ml[e] = k <= it.y ? a.part_ml[place] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int j = 0; j < V; j++) part[e][j] = k <= it.y ? a.part_o[place * D + 32 * j + lane] : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < BATCH; e++) {
+            const float mx = fmaxf(m, ml[e].x), f0 = m == mx ? 1.f : exp2_fast(m - mx), f1 = ml[e].x == mx ? 1.f : exp2_fast(ml[e].x - mx);
+            m = mx;
+            l = fmaf(f0, l, f1 * ml[e].y);
+#pragma unroll
+            for (int j = 0; j < V; j++) o[j] = fmaf(f0, o[j], f1 * part[e][j]);
+        }
+    }
+    if (WPR > 1) {
+        __shared__ float s_o[WPR][D], s_m[WPR], s_l[WPR];
+        if (lane == 0) {
+            s_m[w] = m;
+            s_l[w] = l;
+        }
+#pragma unroll
+        for (int j = 0; j < V; j++) s_o[w][32 * j + lane] = o[j];
+        __syncthreads();
+        if (w != 0) return;
+#pragma unroll
+        for (int k = 1; k < WPR; k++) {
+            const float mx = fmaxf(m, s_m[k]), f0 = m == mx ? 1.f : exp2_fast(m - mx), f1 = s_m[k] == mx ? 1.f : exp2_fast(s_m[k] - mx);
+            m = mx;
+            l = fmaf(f0, l, f1 * s_l[k]);
+#pragma unroll
+            for (int j = 0; j < V; j++) o[j] = fmaf(f0, o[j], f1 * s_o[k][32 * j + lane]);
+        }
     }
     const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
     using T = typename std::conditional<DT == LTQ_F32, float, uint16_t>::type;
-    T *p = static_cast<T *>(a.out) + at * D;
+    T *p = static_cast<T *>(a.out) + ((uint64_t)s.off * a.q_heads + i) * D;
 #pragma unroll
-    for (int j = 0; j < D / 32; j++) {
+    for (int j = 0; j < V; j++) {
         if constexpr (DT == LTQ_F32) p[32 * j + lane] = o[j] * inv;
         else p[32 * j + lane] = (T)token_bits<DT>(o[j] * inv);
     }
@@ -458,22 +696,15 @@ cache_attention_join_kernel(const AttnArgs a)
 template <int D, int NT>
 cudaError_t launch_nt(const AttnArgs &a, cudaStream_t stream)
 {
-    constexpr size_t smem = sizeof(Shared<D, NT>);
-    static bool attr_done[64] = {false};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (smem > 48 * 1024 && dev >= 0 && dev < 64 && !attr_done[dev]) {
-        e = cudaFuncSetAttribute(cache_attention_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-        attr_done[dev] = true;
-    }
-    const uint32_t row_tiles = (a.bt.max_new * a.group + 8 * NT - 1) / (8 * NT);
-    e = launch_chained(cache_attention_kernel<D, NT>, dim3(a.splits * row_tiles, a.cache.kv_heads, a.bt.seqs), dim3(32 * WARPS), smem, stream, a,
-                       row_tiles);
+    cudaError_t e = launch_chained(cache_attention_kernel<D, NT>, dim3(a.ctas), dim3(32 * WARPS), 0, stream, a);
     count_launch();
-    if (e != cudaSuccess || a.splits == 1) return e;
-    e = launch_chained(cache_attention_join_kernel<D>, dim3((a.bt.max_new * a.q_heads + 7) / 8, a.bt.seqs), dim3(256), 0, stream, a);
+    if (e != cudaSuccess) return e;
+    const uint64_t rows = (uint64_t)a.bt.max_new * a.q_heads;   // of one sequence
+    if (rows * a.bt.seqs <= ATTN_FEW_ROWS) {
+        e = launch_chained(cache_attention_join_kernel<D, 8>, dim3((unsigned)rows, a.bt.seqs), dim3(256), 0, stream, a, 8u * NT);
+    } else {
+        e = launch_chained(cache_attention_join_kernel<D, 1>, dim3((unsigned)((rows + 7) / 8), a.bt.seqs), dim3(256), 0, stream, a, 8u * NT);
+    }
     count_launch();
     return e;
 }
