@@ -187,7 +187,7 @@ CacheBatch make_batch(const ltq_kv_cache *c, const int32_t *offsets, const int32
 
 // How the attention call is laid out: CTAs, row tiles per sequence, and the workspace behind them.
 struct AttnPlan {
-    uint32_t rows_per_tile, row_tiles, ctas;
+    uint32_t rows_per_tile, row_tiles, ctas, cluster;
     uint64_t o_floats, ml, items, bytes;
 };
 AttnPlan attn_plan(const ltq_kv_cache *c, int dtype, uint32_t q_heads, uint64_t seqs, uint64_t table_width, uint64_t max_new, int sms)
@@ -197,13 +197,18 @@ AttnPlan attn_plan(const ltq_kv_cache *c, int dtype, uint32_t q_heads, uint64_t 
     p.rows_per_tile = attn_rows_per_tile(dtype, c->head_dim, rows);
     p.row_tiles = (uint32_t)((rows + p.rows_per_tile - 1) / p.rows_per_tile);
     const uint64_t steps = table_width * c->block_tokens / 16;
+    // Few keys: a cluster per item (see cache_attention_cluster_kernel), as many CTAs as the device holds at once, up to eight
+    const uint64_t items = seqs * p.row_tiles * c->kv_heads, slots = (uint64_t)sms * attn_ctas_per_sm(dtype, c->head_dim, p.rows_per_tile);
+    p.cluster = 8;
+    while (p.cluster > 1 && items * p.cluster > slots) p.cluster /= 2;
+    if (steps > (uint64_t)p.cluster * ATTN_WARPS * ATTN_CLUSTER_STEPS) p.cluster = 0;
     const uint64_t most = (seqs * p.row_tiles * c->kv_heads * (steps ? steps : 1) + ATTN_MIN_STEPS - 1) / ATTN_MIN_STEPS;
     const uint64_t fit = (uint64_t)sms * attn_ctas_per_sm(dtype, c->head_dim, p.rows_per_tile);
     p.ctas = (uint32_t)(most < fit ? most : fit);
     p.ml = (uint64_t)2 * ATTN_WARPS * p.ctas * p.rows_per_tile;
     p.o_floats = p.ml * c->head_dim;
-    p.items = seqs * p.row_tiles * c->kv_heads;
-    p.bytes = p.o_floats * sizeof(float) + p.ml * sizeof(float2) + p.items * sizeof(int2);
+    p.items = items;
+    p.bytes = p.cluster ? 16 : p.o_floats * sizeof(float) + p.ml * sizeof(float2) + p.items * sizeof(int2);
     return p;
 }
 
@@ -289,6 +294,7 @@ int ltq_cache_attention(const ltq_kv_cache *cache, const void *q_dev, int dtype,
                 (unsigned long long)workspace_bytes, (unsigned long long)p.bytes);
     a.q_vec = ld_q % 4 == 0 && ((uintptr_t)q_dev % (4 * dtype_size(dtype))) == 0;
     a.out_vec = ((uintptr_t)out_dev % (4 * dtype_size(dtype))) == 0;
+    a.cluster = p.cluster;
     a.ctas = p.ctas;
     a.row_tiles = p.row_tiles;
     a.part_o = static_cast<float *>(workspace_dev);

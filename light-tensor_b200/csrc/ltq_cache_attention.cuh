@@ -30,6 +30,7 @@
 //  * V's block scales go into the probabilities as a ratio to the largest one so far, so that one accumulator serves all;
 //  * the running maximum is kept only approximately: the reference m moves when a score exceeds it by more than 8 (base 2), so
 //    that probabilities stay below 2^8 and almost every step does without a reduction over lanes.
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include "ltq_cache.cuh"
@@ -43,9 +44,7 @@ constexpr int DT = LTQ_ATTN_DT;
 constexpr int TERMS = DT == LTQ_F32 ? 2 : 1;
 constexpr int WARPS = ATTN_WARPS;
 constexpr float SMALLEST_SCALE = 1.17549435e-38f;   // 2^-126
-#ifndef AHEAD
 constexpr uint32_t AHEAD = 2;     // steps beyond the one on its way into registers that are asked into L2
-#endif
 constexpr float MAX_STEP = 8.f;   // how far a score may exceed the reference maximum before it moves
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
@@ -465,23 +464,24 @@ __device__ __forceinline__ void store4(const AttnArgs &a, uint64_t row, int d, f
     }
 }
 
-// One warp's part [first, end) of the steps of one item; the result goes to `out` if the part is the whole item, to workspace
-// slot `slot` otherwise.
+// What a row tile's last row sees, in steps.
+__device__ __forceinline__ uint32_t seen_steps(const AttnArgs &a, const CacheSeq &s, uint32_t row0, uint32_t rows_per_tile)
+{
+    const uint32_t rows = (uint32_t)s.n * a.group, last = row0 + rows_per_tile < rows ? row0 + rows_per_tile - 1 : rows - 1;
+    const int keys = s.len - s.n + (int)(last / a.group) + 1;
+    return keys > 0 ? ((uint32_t)keys + 15) / 16 : 0u;
+}
+
+// One warp takes steps [w0, w1) of one item into `r`.
 template <int D, int NT>
-__device__ __forceinline__ void do_segment(const AttnArgs &a, uint32_t b, const CacheSeq &s, uint32_t h, uint32_t row0, uint32_t first,
-                                           uint32_t end, bool whole, uint32_t slot)
+__device__ __forceinline__ void take_steps(Rows<D, NT> &r, const AttnArgs &a, uint32_t b, const CacheSeq &s, uint32_t h, uint32_t row0,
+                                           uint32_t w0, uint32_t w1)
 {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const uint32_t rows = (uint32_t)s.n * a.group;
-    const uint32_t last = row0 + 8 * NT < rows ? row0 + 8 * NT - 1 : rows - 1;
-    const int keys = s.len - s.n + (int)(last / a.group) + 1;             // what the tile's last row sees
-    const uint32_t seen = keys > 0 ? ((uint32_t)keys + 15) / 16 : 0u, w0 = first, w1 = end < seen ? end : seen;
-
     const int32_t *table = a.bt.table + (uint64_t)b * a.bt.table_width;
     const int sh16 = a.bt.log2_bt - 4;                                    // steps per block, log2
     const uint32_t in_block = (1u << sh16) - 1;
     const LaneOffsets<D> at(lane);
-    Rows<D, NT> r;
     Keys<D> even, odd;
     int32_t page = 0, page_ahead = 0;   // blocks of the steps to be fetched, and to be asked into L2, next
     auto fetch = [&](Keys<D> &into, uint32_t st) {
@@ -510,6 +510,18 @@ __device__ __forceinline__ void do_segment(const AttnArgs &a, uint32_t b, const 
         ask(st + 2 + AHEAD);
         take_keys<D, NT>(r, odd, (int)(st * 16) + 16, g);
     }
+}
+
+// One warp's part [first, end) of the steps of one item; the result goes to `out` if the part is the whole item, to workspace
+// slot `slot` otherwise.
+template <int D, int NT>
+__device__ __forceinline__ void do_segment(const AttnArgs &a, uint32_t b, const CacheSeq &s, uint32_t h, uint32_t row0, uint32_t first,
+                                           uint32_t end, bool whole, uint32_t slot)
+{
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const uint32_t rows = (uint32_t)s.n * a.group, seen = seen_steps(a, s, row0, 8 * NT);
+    Rows<D, NT> r;
+    take_steps<D, NT>(r, a, b, s, h, row0, first, end < seen ? end : seen);
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -643,7 +655,7 @@ cache_attention_join_kernel(const __grid_constant__ AttnArgs a, uint32_t rows_pe
     float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
     for (int j = 0; j < V; j++) o[j] = 0.f;
-    constexpr int BATCH = 4;     // parts loaded before the first is used
+    constexpr int BATCH = WPR == 1 || V > 4 ? 4 : 8;   // parts loaded before the first is used
     for (int k0 = first + w * BATCH; k0 <= it.y; k0 += WPR * BATCH) {
         float2 ml[BATCH];
         float part[BATCH][V];
@@ -693,9 +705,129 @@ cache_attention_join_kernel(const __grid_constant__ AttnArgs a, uint32_t rows_pe
     }
 }
 
+// The same for calls of few items and at most a thousand keys or so per CTA: one launch, no workspace.  A cluster of CTAs takes an
+// item (row tiles along grid.x, heads grid.y, sequences grid.z), every warp an equal part of its steps; the parts meet in
+// shared memory, the CTAs' results through distributed shared memory, each CTA finishing some of the rows.
+template <int D, int NT>
+__global__ void __launch_bounds__(32 * WARPS, (D * NT * TERMS <= 128 ? 3 : 2))
+cache_attention_cluster_kernel(const __grid_constant__ AttnArgs a)
+{
+    griddep_launch_dependents();
+    griddep_wait();
+    constexpr uint32_t ROWS = 8 * NT;
+    __shared__ __align__(16) float s_o[ROWS][D], s_part[WARPS][ROWS][2];
+    __shared__ float s_m[ROWS], s_l[ROWS];
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t rank = cluster.block_rank(), size = cluster.num_blocks();
+    const uint32_t h = blockIdx.y, b = blockIdx.z, row0 = blockIdx.x / size * ROWS;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const CacheSeq s = cache_seq(a.bt, b);
+    if (!s.ok && threadIdx.x == 0) atomicCAS(a.bt.status, 0u, STATUS_BAD_SEQUENCE);
+    const uint32_t rows = s.ok ? (uint32_t)s.n * a.group : 0u;
+    if (row0 >= rows) return;   // the whole cluster
+    const uint32_t steps = seen_steps(a, s, row0, ROWS), parts = size * WARPS, me = rank * WARPS + warp;
+    Rows<D, NT> r;
+    take_steps<D, NT>(r, a, b, s, h, row0, (uint32_t)((uint64_t)steps * me / parts), (uint32_t)((uint64_t)steps * (me + 1) / parts));
+    // the warps' maxima and sums, then their rows one warp after the other into the CTA's
+    float l[NT][2], zp[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            l[nt][j] = r.l[nt][j];
+            zp[nt][j] = r.zp[nt][j];
+#pragma unroll
+            for (int o = 4; o <= 16; o <<= 1) {
+                l[nt][j] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][j], o);
+                zp[nt][j] += __shfl_xor_sync(0xFFFFFFFFu, zp[nt][j], o);
+            }
+            if (g == 0) {
+                s_part[warp][nt * 8 + 2 * c + j][0] = r.m[nt][j];
+                s_part[warp][nt * 8 + 2 * c + j][1] = l[nt][j];
+            }
+        }
+    __syncthreads();
+    float f[NT][2];   // this warp's weight in the CTA's row
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int rr = nt * 8 + 2 * c + j;
+            float m = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) m = fmaxf(m, s_part[w][rr][0]);
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) sum = fmaf(s_part[w][rr][0] == m ? 1.f : exp2_fast(s_part[w][rr][0] - m), s_part[w][rr][1], sum);
+            f[nt][j] = r.m[nt][j] == m ? 1.f : exp2_fast(r.m[nt][j] - m);
+            if (warp == 0 && g == 0) {
+                s_m[rr] = m;
+                s_l[rr] = sum;
+            }
+        }
+    for (int w = 0; w < WARPS; w++) {
+        if (warp == w) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float k = f[nt][j] * r.v_ref;
+#pragma unroll
+                    for (int i = 0; i < D / 32; i++) {
+                        float4 *at = reinterpret_cast<float4 *>(&s_o[nt * 8 + 2 * c + j][Geo<D>::v_dim(i, g)]);
+                        float4 v = w == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *at;
+                        v.x = fmaf(fmaf(r.o[2 * i][nt][j], CODE, -zp[nt][j]), k, v.x);
+                        v.y = fmaf(fmaf(r.o[2 * i][nt][j + 2], CODE, -zp[nt][j]), k, v.y);
+                        v.z = fmaf(fmaf(r.o[2 * i + 1][nt][j], CODE, -zp[nt][j]), k, v.z);
+                        v.w = fmaf(fmaf(r.o[2 * i + 1][nt][j + 2], CODE, -zp[nt][j]), k, v.w);
+                        *at = v;
+                    }
+                }
+        }
+        __syncthreads();
+    }
+    if (size > 1) cluster.sync();   // every CTA's rows are there
+    for (uint32_t k = threadIdx.x; k < ROWS * (D / 4); k += 32 * WARPS) {
+        const uint32_t rr = k / (D / 4), d = (k - rr * (D / 4)) * 4, row = row0 + rr;
+        if (rr % size != rank || row >= rows) continue;
+        float m = -INFINITY, sum = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t q = 0; q < size; q++) m = fmaxf(m, *cluster.map_shared_rank(&s_m[rr], q));
+        for (uint32_t q = 0; q < size; q++) {
+            const float mq = *cluster.map_shared_rank(&s_m[rr], q), w = mq == m ? 1.f : exp2_fast(mq - m);
+            const float4 v = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(&s_o[rr][d], q));
+            sum = fmaf(w, *cluster.map_shared_rank(&s_l[rr], q), sum);
+            o.x = fmaf(w, v.x, o.x);
+            o.y = fmaf(w, v.y, o.y);
+            o.z = fmaf(w, v.z, o.z);
+            o.w = fmaf(w, v.w, o.w);
+        }
+        const uint32_t t = row / a.group;
+        const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);   // a row that sees nothing: zeros
+        store4<D>(a, ((uint64_t)s.off + t) * a.q_heads + h * a.group + (row - t * a.group), d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    }
+    if (size > 1) cluster.sync();   // nobody leaves while its shared memory may still be read
+}
+
 template <int D, int NT>
 cudaError_t launch_nt(const AttnArgs &a, cudaStream_t stream)
 {
+    if (a.cluster) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(a.cluster * a.row_tiles, a.cache.kv_heads, a.bt.seqs);
+        cfg.blockDim = dim3(32 * WARPS);
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = a.cluster;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = chained_launches_enabled() ? 2 : 1;
+        count_launch();
+        return cudaLaunchKernelEx(&cfg, cache_attention_cluster_kernel<D, NT>, a);
+    }
     cudaError_t e = launch_chained(cache_attention_kernel<D, NT>, dim3(a.ctas), dim3(32 * WARPS), 0, stream, a);
     count_launch();
     if (e != cudaSuccess) return e;

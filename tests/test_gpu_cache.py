@@ -69,13 +69,14 @@ def ints(torch, v):
     return torch.tensor(v, dtype=torch.int32, device="cuda")
 
 
-def batch(torch, seed, spans, bt, spare=2):
-    """offsets, lengths, block table of sequences with (new, length) tokens; blocks in random order."""
+def batch(torch, seed, spans, bt, spare=2, wide=0):
+    """offsets, lengths, block table of sequences with (new, length) tokens; blocks in random order.  `wide`: that many more
+    table columns (the launch is sized by the table's width)."""
     g = torch.Generator().manual_seed(seed)
     per = [-(-max(length, 0) // bt) for _, length in spans]
     blocks = sum(per) + spare
     order = torch.randperm(blocks, generator=g).tolist()
-    table = [[order.pop() for _ in range(n)] + [-7] * (max(per + [1]) - n) for n in per]   # unused entries are never read
+    table = [[order.pop() for _ in range(n)] + [-7] * (max(per + [1]) + wide - n) for n in per]   # unused entries are never read
     offsets = [0]
     for n, _ in spans:
         offsets.append(offsets[-1] + n)
@@ -249,11 +250,13 @@ CASES = [  # spans, block_tokens, head_dim, kv_heads, group
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("case", range(len(CASES)))
-def test_attention(cuda, dtype, case):
+@pytest.mark.parametrize("wide", [0, 20000])
+def test_attention(cuda, dtype, case, wide):
+    """Tables as wide as the sequences need (few keys: one launch) and far wider (work divided on the device, parts joined)."""
     import ltq
     torch = cuda
     spans, bt, D, heads, group = CASES[case]
-    b = batch(torch, case, spans, bt)
+    b = batch(torch, case, spans, bt, wide=wide // bt)
     cache = random_cache(torch, ltq, case, b["blocks"], heads, bt, D)
     q = torch.randn(b["tokens"], heads * group, D, generator=torch.Generator().manual_seed(case)).to(getattr(torch, dtype)).cuda()
     got = cache.attention(q, ints(torch, b["table"]), ints(torch, b["lengths"]), ints(torch, b["offsets"]), b["max_new"])
