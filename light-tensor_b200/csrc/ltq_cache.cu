@@ -188,6 +188,7 @@ CacheBatch make_batch(const ltq_kv_cache *c, const int32_t *offsets, const int32
 // How the attention call is laid out: CTAs, row tiles per sequence, and the workspace behind them.
 struct AttnPlan {
     uint32_t rows_per_tile, row_tiles, ctas, cluster;
+    bool tc;
     uint64_t o_floats, ml, items, bytes;
 };
 AttnPlan attn_plan(const ltq_kv_cache *c, int dtype, uint32_t q_heads, uint64_t seqs, uint64_t table_width, uint64_t max_new, int sms)
@@ -208,7 +209,8 @@ AttnPlan attn_plan(const ltq_kv_cache *c, int dtype, uint32_t q_heads, uint64_t 
     p.ml = (uint64_t)2 * ATTN_WARPS * p.ctas * p.rows_per_tile;
     p.o_floats = p.ml * c->head_dim;
     p.items = items;
-    p.bytes = p.cluster ? 16 : p.o_floats * sizeof(float) + p.ml * sizeof(float2) + p.items * sizeof(int2);
+    p.tc = dtype != LTQ_F32 && rows >= ATTN_TC_ROWS && rows <= (uint64_t)65535 * 128;
+    p.bytes = p.cluster || p.tc ? 16 : p.o_floats * sizeof(float) + p.ml * sizeof(float2) + p.items * sizeof(int2);
     return p;
 }
 
@@ -293,6 +295,8 @@ int ltq_cache_attention(const ltq_kv_cache *cache, const void *q_dev, int dtype,
     LTQ_REQUIRE(workspace_bytes >= p.bytes, LTQ_ERR_INVALID_ARG, "the workspace holds %llu bytes, %llu are needed",
                 (unsigned long long)workspace_bytes, (unsigned long long)p.bytes);
     a.q_vec = ld_q % 4 == 0 && ((uintptr_t)q_dev % (4 * dtype_size(dtype))) == 0;
+    a.q_vec8 = (ld_q * dtype_size(dtype)) % 16 == 0 && ((uintptr_t)q_dev & 15) == 0;
+    a.out_vec8 = ((uintptr_t)out_dev & 15) == 0;
     a.out_vec = ((uintptr_t)out_dev % (4 * dtype_size(dtype))) == 0;
     a.cluster = p.cluster;
     a.ctas = p.ctas;
@@ -301,6 +305,10 @@ int ltq_cache_attention(const ltq_kv_cache *cache, const void *q_dev, int dtype,
     a.part_ml = reinterpret_cast<float2 *>(a.part_o + p.o_floats);
     a.item = reinterpret_cast<int2 *>(a.part_ml + p.ml);
     cudaStream_t st = (cudaStream_t)stream;
+    if (p.tc) {
+        LTQ_CUDA_TRY(launch_attention_tc(a, dtype, st));
+        return LTQ_OK;
+    }
     LTQ_CUDA_TRY(dtype == LTQ_F32 ? launch_attention_f32(a, st) : (dtype == LTQ_F16 ? launch_attention_f16(a, st) : launch_attention_bf16(a, st)));
     return LTQ_OK;
 }

@@ -43,6 +43,7 @@ struct AttnArgs {
     uint32_t q_heads, group;       // group = q_heads / kv_heads
     float scale_log2;              // softmax scale * log2(e)
     bool q_vec, out_vec;           // rows start aligned to four elements
+    bool q_vec8, out_vec8;         // to 16 bytes
     // Workspace: what warps leave of (row tile, head) items that they share with other warps, see ltq_cache_attention.cuh.
     float *part_o;                 // [2 * warps][rows per tile][head_dim]
     float2 *part_ml;               // [2 * warps][rows per tile]: running maximum (base 2), sum
@@ -61,5 +62,8 @@ uint32_t attn_ctas_per_sm(int dtype, uint32_t head_dim, uint32_t rows_per_tile);
 cudaError_t launch_attention_f32(const AttnArgs &a, cudaStream_t stream);
 cudaError_t launch_attention_f16(const AttnArgs &a, cudaStream_t stream);
 cudaError_t launch_attention_bf16(const AttnArgs &a, cudaStream_t stream);
+// The tensor-core form for many new tokens (half and bfloat16 queries), ltq_cache_attention_tc.cu.
+cudaError_t launch_attention_tc(const AttnArgs &a, int dtype, cudaStream_t stream);
+constexpr uint64_t ATTN_TC_ROWS = 64;          // rows (new tokens x group) of a sequence from which it is faster
 
 }  // namespace ltq

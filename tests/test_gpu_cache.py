@@ -245,7 +245,9 @@ CASES = [  # spans, block_tokens, head_dim, kv_heads, group
     ([(1, 1)], 16, 128, 1, 1), ([(1, 15), (1, 16), (1, 17)], 16, 64, 2, 4), ([(1, 100), (1, 333), (1, 1)], 32, 128, 2, 8),
     ([(1, 700)], 64, 128, 1, 12), ([(1, 2000), (1, 5)], 128, 96, 1, 7), ([(3, 40), (1, 129), (5, 5)], 16, 32, 2, 3),
     ([(33, 100), (2, 260)], 64, 64, 2, 2), ([(70, 70)], 32, 256, 1, 2), ([(20, 513), (0, 30)], 16, 192, 2, 5), ([(6, 3), (2, 0), (1, 50)], 16, 128, 1, 4),
-    ([(129, 300)], 128, 128, 2, 4), ([(1, 4100), (1, 4096), (1, 31)], 64, 128, 2, 16)]
+    ([(129, 300)], 128, 128, 2, 4), ([(100, 100)], 16, 64, 1, 1), ([(40, 513), (64, 64), (3, 700), (130, 90)], 32, 128, 2, 4),
+    ([(128, 128)], 128, 96, 1, 2), ([(50, 900)], 64, 192, 2, 3), ([(300, 333)], 64, 256, 1, 1), ([(65, 1000), (0, 5)], 16, 32, 2, 3),
+    ([(1, 4100), (1, 4096), (1, 31)], 64, 128, 2, 16)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
