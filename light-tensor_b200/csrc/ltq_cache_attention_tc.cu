@@ -77,6 +77,32 @@ struct TcGeo {
     static __device__ __forceinline__ uint32_t s_col(uint32_t rt, uint32_t sb) { return 256 + rt * 128 + sb * 64; }
 };
 
+// Two floats at a time.
+__device__ __forceinline__ uint64_t pair(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 template <int N>
 __device__ __forceinline__ void regs_up()
 {
@@ -130,6 +156,17 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
         "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+        "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16])
@@ -282,61 +319,73 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             tc_fence_after();
             const uint32_t s_addr = lane_addr + G::s_col(rt, sb);
             const TilePar &par = s_par[j & 7];
+            uint32_t x[2][32];
+            auto load_scores = [&]() {
+                tmem_ld32(s_addr, x[0]);
+                tmem_ld32(s_addr + 32, x[1]);
+            };
+            load_scores();   // (the tile's parameters are read while they are on their way)
+            GroupPar g[G::GROUPS];
+#pragma unroll
+            for (int k = 0; k < G::GROUPS; k++) g[k] = par.g[k];
             const int key0 = (int)(j * G::KEYS);
             const uint32_t bad = par.bad;
             const bool masked = bad || key0 + G::KEYS - 1 > first_pos;
             v_ref = par.v_ref;
             float alpha = par.rescale, sum = 0.f;
             uint32_t p[G::KEYS / 2];
-            uint32_t v[2][32];
-            // P of the whole tile under the reference `ref`, and the sum of its probabilities
+            // P of the tile under the reference `ref`, and the sum of its probabilities
             auto probabilities = [&](float ref) {
-                sum = 0.f;
-                tmem_ld32(s_addr, v[0]);
                 tmem_ld_wait();
+                uint64_t add[G::GROUPS];
 #pragma unroll
-                for (int c = 0; c < G::KEYS / 32; c++) {
-                    uint32_t(&x)[32] = v[c & 1];
-                    if (c + 1 < G::KEYS / 32) tmem_ld32(s_addr + 32 * (c + 1), v[(c + 1) & 1]);
+                for (int k = 0; k < G::GROUPS; k++) {
+                    const float ks = row_scale * g[k].ks, base = g[k].lr - fmaf(zero_scale, g[k].kzs, ref);
+                    const uint64_t ks2 = pair(ks, ks), base2 = pair(base, base);
+                    float2 y[8];
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const GroupPar g = par.g[2 * c + k];
-                        const float ks = row_scale * g.ks, base = g.lr - fmaf(zero_scale, g.kzs, ref);
-                        float y[16];
-#pragma unroll
-                        for (int i = 0; i < 16; i++) y[i] = fmaf(__uint_as_float(x[16 * k + i]), ks, base);
-                        if (masked) {
-                            const int see = bad >> (2 * c + k) & 1 ? -1 : pos - key0 - 32 * c - 16 * k;   // the last key of these that the row sees
-#pragma unroll
-                            for (int i = 0; i < 16; i++)
-                                if (i > see) y[i] = -INFINITY;
-                        }
-                        float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            const float y0 = ex2(y[i]), y1 = ex2(y[i + 1]);
-                            s0 += y0;
-                            s1 += y1;
-                            p[16 * c + 8 * k + i / 2] = h2pack(y0, y1);
-                        }
-                        sum = fmaf(s0 + s1, g.inv, sum);
+                    for (int i = 0; i < 8; i++) {
+                        const int c = 16 * k + 2 * i;
+                        y[i] = unpair(fma2(pair(__uint_as_float(x[c / 32][c % 32]), __uint_as_float(x[c / 32][c % 32 + 1])), ks2, base2));
                     }
-                    if (c + 1 < G::KEYS / 32) tmem_ld_wait();
+                    if (masked) {
+                        const int see = bad >> k & 1 ? -1 : pos - key0 - 16 * k;   // the last key of these that the row sees
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            if (2 * i > see) y[i].x = -INFINITY;
+                            if (2 * i + 1 > see) y[i].y = -INFINITY;
+                        }
+                    }
+                    add[k] = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        y[i].x = ex2(y[i].x);
+                        y[i].y = ex2(y[i].y);
+                        add[k] = i == 0 ? pair(y[i].x, y[i].y) : add2(add[k], pair(y[i].x, y[i].y));
+                        p[8 * k + i] = h2pack(y[i].x, y[i].y);
+                    }
+                }
+                sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < G::GROUPS; k++) {
+                    const float2 s2 = unpair(add[k]);
+                    sum = fmaf(s2.x + s2.y, g[k].inv, sum);
                 }
             };
             probabilities(m);   // (with m at -inf everything visible is inf, and so is the sum)
             if (__any_sync(0xFFFFFFFFu, sum > TC_MAX_SUM)) {
+                load_scores();
+                tmem_ld_wait();
                 float best = -INFINITY;
-#pragma unroll 1
-                for (int c = 0; c < G::KEYS / 16; c++) {
-                    uint32_t x[16];
-                    tmem_ld16(s_addr + 16 * c, x);
-                    tmem_ld_wait();
-                    const GroupPar g = par.g[c];
-                    const float ks = row_scale * g.ks, base = -zero_scale * g.kzs;
-                    const int see = bad >> c & 1 ? -1 : pos - key0 - 16 * c;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) best = i > see ? best : fmaxf(best, fmaf(__uint_as_float(x[i]), ks, base));
+                for (int k = 0; k < G::GROUPS; k++) {
+                    const float ks = row_scale * g[k].ks, base = -zero_scale * g[k].kzs;
+                    const int see = bad >> k & 1 ? -1 : pos - key0 - 16 * k;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int c = 16 * k + i;
+                        best = i > see ? best : fmaxf(best, fmaf(__uint_as_float(x[c / 32][c % 32]), ks, base));
+                    }
                 }
                 const float mx = fmaxf(m, best), down = m == mx ? 1.f : ex2(m - mx);
                 m = mx;
@@ -361,13 +410,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                     tmem_st16(o_addr + d, o);
                 }
             }
-#pragma unroll
-            for (int c = 0; c < G::KEYS / 32; c++) {
-                uint32_t w[16];
-#pragma unroll
-                for (int i = 0; i < 16; i++) w[i] = p[16 * c + i];
-                tmem_st16(s_addr + 16 * c, w);
-            }
+            tmem_st32(s_addr, p);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
