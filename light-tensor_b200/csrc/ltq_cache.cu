@@ -187,30 +187,59 @@ CacheBatch make_batch(const ltq_kv_cache *c, const int32_t *offsets, const int32
 
 // How the attention call is laid out: CTAs, row tiles per sequence, and the workspace behind them.
 struct AttnPlan {
-    uint32_t rows_per_tile, row_tiles, ctas, cluster;
+    uint32_t rows_per_tile, row_tiles, ctas, cluster, splits;
     bool tc;
     uint64_t o_floats, ml, items, bytes;
 };
 AttnPlan attn_plan(const ltq_kv_cache *c, int dtype, uint32_t q_heads, uint64_t seqs, uint64_t table_width, uint64_t max_new, int sms)
 {
-    AttnPlan p;
-    const uint64_t rows = max_new * (q_heads / c->kv_heads);
+    AttnPlan p{};
+    const uint64_t rows = max_new * (q_heads / c->kv_heads), keys = table_width * c->block_tokens;
+    const uint64_t heads = seqs * c->kv_heads, steps = keys / 16;
+    // The tensor-core form needs its 256 (128) rows filled to be worth it, the others read the keys once per 8 or 16 rows.
+    // Estimates in microseconds from a sweep over 1 to 64 sequences, 8 to 1536 rows, 300 and 4000 keys, head_dim 64, 128, 256:
+    //   the others    8 + 0.0008 per 16 keys of a row tile at head_dim 128       (64 x 8 heads, 96 rows, 4000 keys: 361 us)
+    //   tensor cores  6 + 8 per wave of CTAs + 1.15 per 64 keys (+ 5 for a join)  (the same: 259 us;
+    //                 1 x 8 heads, 512 rows: 300 keys 24 us against 15, 4000 keys 35 us against 70)
+    if (dtype != LTQ_F32 && rows > 16) {
+        AttnPlan t{};
+        t.tc = true;
+        t.rows_per_tile = attn_tc_rows(c->head_dim);
+        const uint64_t tiles = (rows + t.rows_per_tile - 1) / t.rows_per_tile, waves = (heads * tiles + sms - 1) / sms;
+        // where the groups of row tiles do not fill the device, several CTAs share a group's keys
+        const uint64_t most = (keys + 64 * ATTN_TC_MIN_TILES - 1) / (64 * ATTN_TC_MIN_TILES), fit = (uint64_t)sms / (heads * tiles);
+        t.splits = (uint32_t)(fit < 1 || most < 1 ? 1 : (most < fit ? most : fit));
+        const uint32_t per = attn_rows_per_tile(dtype, c->head_dim, rows);
+        const double other = 8 + 0.0008 * (double)(heads * ((rows + per - 1) / per) * steps) * c->head_dim / 128;
+        const double tc = 6 + (double)waves * (8 + 1.15 * (double)(keys / 64) / t.splits) + (t.splits > 1 ? 5 : 0);
+        if (tc < other && tiles <= 65535) {
+            t.row_tiles = (uint32_t)tiles;
+            t.items = heads * tiles;
+            if (t.splits > 1) {
+                t.ml = t.items * t.splits * t.rows_per_tile;
+                t.o_floats = t.ml * c->head_dim;
+            }
+            t.bytes = t.splits > 1 ? t.o_floats * sizeof(float) + t.ml * sizeof(float2) + t.items * sizeof(int2) : 16;
+            return t;
+        }
+    }
     p.rows_per_tile = attn_rows_per_tile(dtype, c->head_dim, rows);
     p.row_tiles = (uint32_t)((rows + p.rows_per_tile - 1) / p.rows_per_tile);
-    const uint64_t steps = table_width * c->block_tokens / 16;
-    // Few keys: a cluster per item (see cache_attention_cluster_kernel), as many CTAs as the device holds at once, up to eight
-    const uint64_t items = seqs * p.row_tiles * c->kv_heads, slots = (uint64_t)sms * attn_ctas_per_sm(dtype, c->head_dim, p.rows_per_tile);
+    p.items = heads * p.row_tiles;
+    // Few keys: a cluster per item (see cache_attention_cluster_kernel), as many CTAs as the device holds at once, up to eight.
+    const uint64_t slots = (uint64_t)sms * attn_ctas_per_sm(dtype, c->head_dim, p.rows_per_tile);
     p.cluster = 8;
-    while (p.cluster > 1 && items * p.cluster > slots) p.cluster /= 2;
-    if (steps > (uint64_t)p.cluster * ATTN_WARPS * ATTN_CLUSTER_STEPS) p.cluster = 0;
-    const uint64_t most = (seqs * p.row_tiles * c->kv_heads * (steps ? steps : 1) + ATTN_MIN_STEPS - 1) / ATTN_MIN_STEPS;
-    const uint64_t fit = (uint64_t)sms * attn_ctas_per_sm(dtype, c->head_dim, p.rows_per_tile);
-    p.ctas = (uint32_t)(most < fit ? most : fit);
+    while (p.cluster > 1 && p.items * p.cluster > slots) p.cluster /= 2;
+    if (steps <= (uint64_t)p.cluster * ATTN_WARPS * ATTN_CLUSTER_STEPS) {
+        p.bytes = 16;
+        return p;
+    }
+    p.cluster = 0;
+    const uint64_t most = (p.items * steps + ATTN_MIN_STEPS - 1) / ATTN_MIN_STEPS;
+    p.ctas = (uint32_t)(most < slots ? most : slots);
     p.ml = (uint64_t)2 * ATTN_WARPS * p.ctas * p.rows_per_tile;
     p.o_floats = p.ml * c->head_dim;
-    p.items = items;
-    p.tc = dtype != LTQ_F32 && rows >= ATTN_TC_ROWS && rows <= (uint64_t)65535 * 128;
-    p.bytes = p.cluster || p.tc ? 16 : p.o_floats * sizeof(float) + p.ml * sizeof(float2) + p.items * sizeof(int2);
+    p.bytes = p.o_floats * sizeof(float) + p.ml * sizeof(float2) + p.items * sizeof(int2);
     return p;
 }
 
@@ -299,6 +328,7 @@ int ltq_cache_attention(const ltq_kv_cache *cache, const void *q_dev, int dtype,
     a.out_vec8 = ((uintptr_t)out_dev & 15) == 0;
     a.out_vec = ((uintptr_t)out_dev % (4 * dtype_size(dtype))) == 0;
     a.cluster = p.cluster;
+    a.splits = p.splits;
     a.ctas = p.ctas;
     a.row_tiles = p.row_tiles;
     a.part_o = static_cast<float *>(workspace_dev);

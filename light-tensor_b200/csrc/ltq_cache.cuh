@@ -49,6 +49,7 @@ struct AttnArgs {
     float2 *part_ml;               // [2 * warps][rows per tile]: running maximum (base 2), sum
     int2 *item;                    // [seqs][row tiles][kv_heads]: first slot, last warp
     uint32_t ctas, row_tiles;
+    uint32_t splits;               // tensor-core form: CTAs that share one's keys
     uint32_t cluster;              // CTAs per item in the form without workspace; 0: the form with
 };
 constexpr uint32_t ATTN_WARPS = 4;             // per CTA
@@ -64,6 +65,11 @@ cudaError_t launch_attention_f16(const AttnArgs &a, cudaStream_t stream);
 cudaError_t launch_attention_bf16(const AttnArgs &a, cudaStream_t stream);
 // The tensor-core form for many new tokens (half and bfloat16 queries), ltq_cache_attention_tc.cu.
 cudaError_t launch_attention_tc(const AttnArgs &a, int dtype, cudaStream_t stream);
-constexpr uint64_t ATTN_TC_ROWS = 64;          // rows (new tokens x group) of a sequence from which it is faster
+uint32_t attn_tc_rows(uint32_t head_dim);      // rows per CTA
+constexpr uint32_t ATTN_TC_MIN_TILES = 4;      // a split takes at least as many tiles of 64 keys
+// Joins its parts.
+cudaError_t launch_attention_join_f16(const AttnArgs &a, uint32_t rows_per_tile, cudaStream_t stream);
+cudaError_t launch_attention_join_bf16(const AttnArgs &a, uint32_t rows_per_tile, cudaStream_t stream);
+cudaError_t launch_attention_join_f32(const AttnArgs &a, uint32_t rows_per_tile, cudaStream_t stream);
 
 }  // namespace ltq

@@ -1,5 +1,5 @@
 // Attention of a few new tokens over the 8-bit cache, one instantiation per element type of q (the including file defines
-// LTQ_ATTN_DT and LTQ_ATTN_LAUNCH).
+// LTQ_ATTN_DT, LTQ_ATTN_LAUNCH and LTQ_ATTN_JOIN).
 //
 // Reading the cache is the floor (2 * head_dim bytes per key and head); all query heads of a group and all new tokens of a
 // sequence share that read.  A warp streams 16 keys at a time straight from global memory into the operand layout of
@@ -637,7 +637,7 @@ cache_attention_kernel(const __grid_constant__ AttnArgs a)
 // where there are few and a row may have hundreds of parts.
 template <int D, int WPR>
 __global__ void __launch_bounds__(256)
-cache_attention_join_kernel(const __grid_constant__ AttnArgs a, uint32_t rows_per_tile)
+cache_attention_join_kernel(const __grid_constant__ AttnArgs a, uint32_t rows_per_tile, bool dense)
 {
     griddep_launch_dependents();
     griddep_wait();
@@ -649,9 +649,10 @@ cache_attention_join_kernel(const __grid_constant__ AttnArgs a, uint32_t rows_pe
     const uint32_t t = i / a.q_heads, head = i - t * a.q_heads, h = head / a.group;
     const uint32_t row = t * a.group + (head - h * a.group), tile = row / rows_per_tile, rr = row - tile * rows_per_tile;
     const int2 it = a.item[((uint64_t)blockIdx.y * a.row_tiles + tile) * a.cache.kv_heads + h];
-    const int first = it.x >> 1;
+    // Parts are numbered by the warps that made them, two slots each: the first one's part lies in slot it.x, those of the
+    // warps behind it in their first slots.  `dense` (the tensor-core form): parts are slots.
+    const int first = dense ? it.x : it.x >> 1;
     if (first == it.y) return;   // one warp had it all
-    // the first warp's part lies in slot it.x, those of the warps behind it in their first slots
     float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
     for (int j = 0; j < V; j++) o[j] = 0.f;
@@ -662,7 +663,7 @@ cache_attention_join_kernel(const __grid_constant__ AttnArgs a, uint32_t rows_pe
 #pragma unroll
         for (int e = 0; e < BATCH; e++) {
             const int k = k0 + e;
-            const uint64_t place = (uint64_t)(k == first ? it.x : 2 * k) * rows_per_tile + rr;
+            const uint64_t place = (uint64_t)(dense ? k : (k == first ? it.x : 2 * k)) * rows_per_tile + rr;
             ml[e] = k <= it.y ? a.part_ml[place] : make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int j = 0; j < V; j++) part[e][j] = k <= it.y ? a.part_o[place * D + 32 * j + lane] : 0.f;
@@ -809,6 +810,16 @@ cache_attention_cluster_kernel(const __grid_constant__ AttnArgs a)
     if (size > 1) cluster.sync();   // nobody leaves while its shared memory may still be read
 }
 
+template <int D>
+cudaError_t launch_join(const AttnArgs &a, uint32_t rows_per_tile, bool dense, cudaStream_t stream)
+{
+    const uint64_t rows = (uint64_t)a.bt.max_new * a.q_heads;   // of one sequence
+    count_launch();
+    if (rows * a.bt.seqs <= ATTN_FEW_ROWS)
+        return launch_chained(cache_attention_join_kernel<D, 8>, dim3((unsigned)rows, a.bt.seqs), dim3(256), 0, stream, a, rows_per_tile, dense);
+    return launch_chained(cache_attention_join_kernel<D, 1>, dim3((unsigned)((rows + 7) / 8), a.bt.seqs), dim3(256), 0, stream, a, rows_per_tile, dense);
+}
+
 template <int D, int NT>
 cudaError_t launch_nt(const AttnArgs &a, cudaStream_t stream)
 {
@@ -831,14 +842,7 @@ cudaError_t launch_nt(const AttnArgs &a, cudaStream_t stream)
     cudaError_t e = launch_chained(cache_attention_kernel<D, NT>, dim3(a.ctas), dim3(32 * WARPS), 0, stream, a);
     count_launch();
     if (e != cudaSuccess) return e;
-    const uint64_t rows = (uint64_t)a.bt.max_new * a.q_heads;   // of one sequence
-    if (rows * a.bt.seqs <= ATTN_FEW_ROWS) {
-        e = launch_chained(cache_attention_join_kernel<D, 8>, dim3((unsigned)rows, a.bt.seqs), dim3(256), 0, stream, a, 8u * NT);
-    } else {
-        e = launch_chained(cache_attention_join_kernel<D, 1>, dim3((unsigned)((rows + 7) / 8), a.bt.seqs), dim3(256), 0, stream, a, 8u * NT);
-    }
-    count_launch();
-    return e;
+    return launch_join<D>(a, 8 * NT, false, stream);
 }
 
 template <int D>
@@ -851,6 +855,19 @@ cudaError_t launch_d(const AttnArgs &a, cudaStream_t stream)
 }
 
 }  // namespace
+
+cudaError_t LTQ_ATTN_JOIN(const AttnArgs &a, uint32_t rows_per_tile, cudaStream_t stream)
+{
+    switch (a.cache.head_dim) {
+        case 32: return launch_join<32>(a, rows_per_tile, true, stream);
+        case 64: return launch_join<64>(a, rows_per_tile, true, stream);
+        case 96: return launch_join<96>(a, rows_per_tile, true, stream);
+        case 128: return launch_join<128>(a, rows_per_tile, true, stream);
+        case 192: return launch_join<192>(a, rows_per_tile, true, stream);
+        case 256: return launch_join<256>(a, rows_per_tile, true, stream);
+        default: return cudaErrorInvalidValue;
+    }
+}
 
 cudaError_t LTQ_ATTN_LAUNCH(const AttnArgs &a, cudaStream_t stream)
 {

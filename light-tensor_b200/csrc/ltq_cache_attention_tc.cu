@@ -189,7 +189,8 @@ __device__ __forceinline__ float elem(uint32_t w, int i)   // half i (0, 1) of a
 
 }  // namespace
 
-// Grid: (kv_heads, sequences, groups of row tiles); those that see most keys come first.
+// Grid: (kv_heads * splits, sequences, groups of row tiles); those that see most keys come first.  Where the groups do not fill
+// the device, `splits` CTAs share one's keys and leave their parts in the workspace for the join kernel.
 template <int DT, int D>
 __global__ void __launch_bounds__(TcGeo<D>::THREADS, 1)
 cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
@@ -239,7 +240,8 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
     griddep_wait();
     const uint32_t tmem = s_misc[0];
 
-    const uint32_t h = blockIdx.x, b = blockIdx.y, row0 = (gridDim.z - 1 - blockIdx.z) * (TC_ROWS * RT);
+    const uint32_t split = blockIdx.x / a.cache.kv_heads, h = blockIdx.x - split * a.cache.kv_heads, b = blockIdx.y;
+    const uint32_t group = gridDim.z - 1 - blockIdx.z, row0 = group * (TC_ROWS * RT);
     const CacheSeq s = cache_seq(a.bt, b);
     if (!s.ok && threadIdx.x == 0) atomicCAS(status, 0u, STATUS_BAD_SEQUENCE);
     const uint32_t rows = s.ok ? (uint32_t)s.n * a.group : 0u;
@@ -250,7 +252,14 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
         const int keys = s.len - s.n + (int)(last / a.group) + 1;
         return keys > 0 ? ((uint32_t)keys + G::KEYS - 1) / G::KEYS : 0u;
     };
-    const uint32_t tiles0 = tiles_of(0), tiles1 = RT == 2 ? tiles_of(RT - 1) : 0u, tiles = tiles0 > tiles1 ? tiles0 : tiles1;
+    const uint32_t all0 = tiles_of(0), all1 = RT == 2 ? tiles_of(RT - 1) : 0u, all = all0 > all1 ? all0 : all1;
+    // this CTA's tiles: [tile0, tile0 + tiles), of which the row tiles see the first tiles0 and tiles1
+    const uint32_t tile0 = (uint32_t)((uint64_t)all * split / a.splits), tiles = (uint32_t)((uint64_t)all * (split + 1) / a.splits) - tile0;
+    auto part_of = [&](uint32_t n) { return n <= tile0 ? 0u : (n - tile0 < tiles ? n - tile0 : tiles); };
+    const uint32_t tiles0 = part_of(all0), tiles1 = part_of(all1);
+    const uint32_t place = ((b * gridDim.z + group) * a.cache.kv_heads + h) * a.splits;   // workspace slot of split 0
+    if (a.splits > 1 && split == 0 && row0 < rows && threadIdx.x == 0)
+        a.item[((uint64_t)b * gridDim.z + group) * a.cache.kv_heads + h] = make_int2((int)place, (int)(place + a.splits - 1));
 
     if (wg < RT) {
         // ---------------- softmax: one row per thread ----------------
@@ -328,7 +337,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             GroupPar g[G::GROUPS];
 #pragma unroll
             for (int k = 0; k < G::GROUPS; k++) g[k] = par.g[k];
-            const int key0 = (int)(j * G::KEYS);
+            const int key0 = (int)((tile0 + j) * G::KEYS);
             const uint32_t bad = par.bad;
             const bool masked = bad || key0 + G::KEYS - 1 > first_pos;
             v_ref = par.v_ref;
@@ -421,7 +430,25 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             ok = __all_sync(0xFFFFFFFFu, mbar_wait(pv_bar + 8 * (pj % SB), (pj / SB) & 1, abort_flag, status, 0xB20u | (pj % SB)));
             tc_fence_after();
         }
-        if (ok) {
+        if (ok && a.splits > 1) {
+            const uint64_t at = (uint64_t)(place + split) * (TC_ROWS * RT) + rt * TC_ROWS + r;
+            if (real) a.part_ml[at] = make_float2(m, l);
+            float4 *dst = reinterpret_cast<float4 *>(a.part_o + at * D);
+#pragma unroll 1
+            for (int d = 0; d < D; d += 16) {
+                uint32_t o[16];
+                if (mine > 0) {
+                    tmem_ld16(o_addr + d, o);
+                    tmem_ld_wait();
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (real)
+                        dst[d / 4 + i] = mine > 0 ? make_float4(__uint_as_float(o[4 * i]) * v_ref, __uint_as_float(o[4 * i + 1]) * v_ref,
+                                                                __uint_as_float(o[4 * i + 2]) * v_ref, __uint_as_float(o[4 * i + 3]) * v_ref)
+                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        } else if (ok) {
             const float inv = l == 0.f ? 0.f : __fdiv_rn(v_ref, l);   // a row that sees nothing: zeros
             uint16_t *dst = static_cast<uint16_t *>(a.out) + (((uint64_t)s.off + t) * a.q_heads + h * a.group + (row - t * a.group)) * D;
 #pragma unroll 1
@@ -454,7 +481,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
         const int tid = threadIdx.x & 127;
         const int32_t *table = a.bt.table + (uint64_t)b * a.bt.table_width;
         const uint32_t in_block = (1u << a.bt.log2_bt) - 1, parts = G::PARTS * tiles;
-        const uint32_t last_key = tiles * G::KEYS - 1 < (uint32_t)s.len - 1 ? tiles * G::KEYS - 1 : (uint32_t)s.len - 1;
+        const uint32_t begin = tile0 * G::KEYS, end = (tile0 + tiles) * G::KEYS, last_key = end < (uint32_t)s.len ? end - 1 : (uint32_t)s.len - 1;
         // the block that holds a key; keys behind the sequence's last read its block (masked later)
         auto page_of = [&](uint32_t key) { return __ldg(table + ((key < last_key ? key : last_key) >> a.bt.log2_bt)); };
         auto slot_of = [&](int32_t page) { return (uint64_t)((uint32_t)page < a.cache.blocks ? (uint32_t)page : 0u) * a.cache.kv_heads + h; };
@@ -467,25 +494,25 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             int32_t page[PER];
             auto pages = [&](uint32_t hf) {
 #pragma unroll
-                for (int i = 0; i < PER; i++) page[i] = page_of(hf * G::PART + key_of(i));
+                for (int i = 0; i < PER; i++) page[i] = page_of(begin + hf * G::PART + key_of(i));
             };
             auto load = [&](uint4 (&c)[PER], uint32_t hf) {
 #pragma unroll
                 for (int i = 0; i < PER; i++) {
-                    const uint32_t key = hf * G::PART + key_of(i);
+                    const uint32_t key = begin + hf * G::PART + key_of(i);
                     c[i] = __ldg(reinterpret_cast<const uint4 *>(a.cache.k_dev + ((slot_of(page[i]) << a.bt.log2_bt) + (key & in_block)) * D + piece_of(i) * 16));
                 }
             };
             // first warp: lane i % GROUPS looks after a tile's group i
             int32_t g_page = 0;
             float v_ref = TC_SMALLEST;
-            if (warp % 4 == 0 && tiles > 0) g_page = page_of((lane % G::GROUPS) * 16);
+            if (warp % 4 == 0 && tiles > 0) g_page = page_of(begin + (lane % G::GROUPS) * 16);
             auto params = [&](uint32_t j) {   // of tile j, in the place of tile j - 8: S of tile j - 3 is done, so P of tile j - 5 was
                 const uint64_t slot = slot_of(g_page);
                 const bool bad = (uint32_t)g_page >= a.cache.blocks;
                 const ltq_qparams kq = a.cache.k_qp_dev[slot];
                 const float vs = a.cache.v_qp_dev[slot].scale;
-                if (j + 1 < tiles) g_page = page_of((j + 1) * G::KEYS + (lane % G::GROUPS) * 16);
+                if (j + 1 < tiles) g_page = page_of(begin + (j + 1) * G::KEYS + (lane % G::GROUPS) * 16);
                 if (bad && lane < G::GROUPS) atomicCAS(status, 0u, STATUS_BAD_BLOCK);
                 float top = vs;   // (NaN is passed over)
 #pragma unroll
@@ -557,7 +584,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             auto load = [&](Codes &c, uint32_t hf) {
                 if (!busy) return;
                 const uint64_t slot = slot_of(page);
-                const uint32_t key = hf * G::PART + kg * 8;
+                const uint32_t key = begin + hf * G::PART + kg * 8;
                 const uint8_t *p = a.cache.v_dev + ((slot << a.bt.log2_bt) + (key & in_block)) * D + d0;
 #pragma unroll
                 for (int k = 0; k < 8; k++) c.c[k] = __ldg(reinterpret_cast<const uint2 *>(p + k * D));
@@ -567,7 +594,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             auto convert = [&](uint32_t hf, Codes &cur, Codes &nxt) -> bool {
                 const uint32_t j = hf / G::PARTS, st = j & 1;
                 if (hf + 1 < parts) load(nxt, hf + 1);
-                if (hf + 2 < parts) page = page_of((hf + 2) * G::PART + kg * 8);
+                if (hf + 2 < parts) page = page_of(begin + (hf + 2) * G::PART + kg * 8);
                 if (hf % G::PARTS == 0 && j >= 2 && !mbar_wait(v_empty + 8 * st, ((j - 2) >> 1) & 1, abort_flag, status, 0xB40u | st)) return false;
                 if (busy) {
                     const uint32_t z = 0x64006400u + cur.z * 0x10001u;
@@ -600,9 +627,9 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             };
             Codes even, odd;
             if (tiles > 0) {
-                page = page_of(kg * 8);
+                page = page_of(begin + kg * 8);
                 load(even, 0);
-                page = page_of(G::PART + kg * 8);
+                page = page_of(begin + G::PART + kg * 8);
             }
             for (uint32_t hf = 0; hf < parts; hf += 2)
                 if (!convert(hf, even, odd) || hf + 1 >= parts || !convert(hf + 1, odd, even)) break;
@@ -697,10 +724,9 @@ cudaError_t launch_tc(const AttnArgs &a, cudaStream_t stream)
         if (e != cudaSuccess) return e;
         attr_done[dev] = true;
     }
-    constexpr uint32_t PER = TC_ROWS * TcGeo<D>::RT;
-    const uint32_t tiles = (a.bt.max_new * a.group + PER - 1) / PER;
     count_launch();
-    return launch_chained(cache_attention_tc_kernel<DT, D>, dim3(a.cache.kv_heads, a.bt.seqs, tiles), dim3(TcGeo<D>::THREADS), TcGeo<D>::SMEM, stream, a);
+    e = launch_chained(cache_attention_tc_kernel<DT, D>, dim3(a.cache.kv_heads * a.splits, a.bt.seqs, a.row_tiles), dim3(TcGeo<D>::THREADS), TcGeo<D>::SMEM, stream, a);
+    return e != cudaSuccess || a.splits == 1 ? e : (DT == LTQ_F16 ? launch_attention_join_f16 : launch_attention_join_bf16)(a, TC_ROWS * TcGeo<D>::RT, stream);
 }
 
 template <int DT>
@@ -718,6 +744,8 @@ cudaError_t launch_tc_d(const AttnArgs &a, cudaStream_t stream)
 }
 
 }  // namespace
+
+uint32_t attn_tc_rows(uint32_t head_dim) { return head_dim <= 128 ? 2 * TC_ROWS : TC_ROWS; }
 
 cudaError_t launch_attention_tc(const AttnArgs &a, int dtype, cudaStream_t stream)
 {

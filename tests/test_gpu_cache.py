@@ -218,26 +218,25 @@ def attention_want(torch, cache, q, b, scale):
     for i, length in enumerate(b["lengths"]):
         off, n = b["offsets"][i], b["offsets"][i + 1] - b["offsets"][i]
         pages = torch.tensor(b["table"][i][:-(-length // bt)], device="cuda", dtype=torch.long)
-        for h in range(heads):
+        pos = length - n + torch.arange(n, device="cuda")
+        live = pos >= 0
+        for h in range(heads if bool(live.any()) else 0):
             k, v = (val[x][pages, h].reshape(-1, D)[:length] for x in "kv")
-            for t in range(n):
-                pos = length - n + t
-                if pos < 0:
-                    continue
-                qq = q[off + t, h * group:(h + 1) * group].double()
-                kk, vv = k[:pos + 1], v[:pos + 1]
-                s = qq @ kk.t() * scale
-                p = torch.softmax(s, 1)
-                want[off + t, h * group:(h + 1) * group] = p @ vv
-                # scores: q to 2^-22 of its largest entry (float) or exact, products summed in float by the tensor core
-                # (at most 2^-23 per addition), one more rounding each for the two scales and the subtraction of the maximum
-                size = (qq.abs() @ kk.abs().t()).amax(1, keepdim=True) + (qq.abs().amax(1, keepdim=True) * kk.abs().sum(1).amax())
-                ds = abs(scale) * size * (2.0 ** -22 + D * 2.0 ** -23 + 4 * 2.0 ** -24)
-                # probabilities: 2^-11 (half) or 2^-22 (two halves) relative, the exponential's 2^-22, and 2^-25 of the
-                # reference maximum's (at least 2^-8 of the largest one's inverse) for subnormal halves; sums in float
-                keys = pos + 1
-                dp = 2 * ds + (2.0 ** -21 if fine else 2.0 ** -11) + 2.0 ** -21 + keys * 2.0 ** -23 + keys * 2.0 ** -24
-                tol[off + t, h * group:(h + 1) * group] = dp * vv.abs().amax(0) + 1e-300
+            qq = q[off:off + n, h * group:(h + 1) * group].double()[live]
+            seen = (torch.arange(length, device="cuda") <= pos[live][:, None])[:, None]
+            s = (qq @ k.t() * scale).masked_fill(~seen, -math.inf)
+            rows = slice(off + n - int(live.sum()), off + n)
+            want[rows, h * group:(h + 1) * group] = torch.softmax(s, 2) @ v
+            # scores: q to 2^-22 of its largest entry (float) or exact, products summed in float by the tensor core
+            # (at most 2^-23 per addition), one more rounding each for the two scales and the subtraction of the maximum
+            size = (qq.abs() @ k.abs().t()).masked_fill(~seen, 0).amax(2, keepdim=True) + qq.abs().amax(2, keepdim=True) * k.abs().sum(1).amax()
+            ds = abs(scale) * size * (2.0 ** -22 + D * 2.0 ** -23 + 4 * 2.0 ** -24)
+            # probabilities: 2^-11 (half) or 2^-22 (two halves) relative, the exponential's 2^-22, and 2^-25 of the
+            # reference maximum's (at least 2^-8 of the largest one's inverse) for subnormal halves; sums in float
+            keys = (pos[live] + 1)[:, None, None]
+            dp = 2 * ds + (2.0 ** -21 if fine else 2.0 ** -11) + 2.0 ** -21 + keys * 2.0 ** -23 + keys * 2.0 ** -24
+            largest = torch.cummax(v.abs(), 0).values[pos[live]][:, None]
+            tol[rows, h * group:(h + 1) * group] = dp * largest + 1e-300
     return want, tol + eps / 2 * (want.abs() + tol)
 
 
@@ -246,6 +245,8 @@ CASES = [  # spans, block_tokens, head_dim, kv_heads, group
     ([(1, 700)], 64, 128, 1, 12), ([(1, 2000), (1, 5)], 128, 96, 1, 7), ([(3, 40), (1, 129), (5, 5)], 16, 32, 2, 3),
     ([(33, 100), (2, 260)], 64, 64, 2, 2), ([(70, 70)], 32, 256, 1, 2), ([(20, 513), (0, 30)], 16, 192, 2, 5), ([(6, 3), (2, 0), (1, 50)], 16, 128, 1, 4),
     ([(129, 300)], 128, 128, 2, 4), ([(100, 100)], 16, 64, 1, 1), ([(40, 513), (64, 64), (3, 700), (130, 90)], 32, 128, 2, 4),
+    ([(65, 90 + i) for i in range(40)], 16, 128, 2, 2), ([(40, 70 + 3 * i) for i in range(80)], 32, 256, 1, 2),
+    ([(600, 700)], 16, 64, 2, 4), ([(700, 700), (0, 5)], 16, 32, 1, 24), ([(300, 305)], 128, 96, 2, 4),
     ([(128, 128)], 128, 96, 1, 2), ([(50, 900)], 64, 192, 2, 3), ([(300, 333)], 64, 256, 1, 1), ([(65, 1000), (0, 5)], 16, 32, 2, 3),
     ([(1, 4100), (1, 4096), (1, 31)], 64, 128, 2, 16)]
 
