@@ -8,34 +8,41 @@ namespace ltq {
 
 namespace {
 
-constexpr int APPEND_THREADS = 128;
+constexpr int APPEND_THREADS = 128, APPEND_KEEP = 8;
 constexpr float SMALLEST_SCALE = 1.17549435e-38f;   // 2^-126
 
-// Four neighbouring elements as floats.
+// A 16-byte vector of 8 (float: 4) neighbouring elements, element by element where it is not aligned.
 template <int DT>
-__device__ __forceinline__ float4 load4(const void *base, uint64_t at, bool vec)
-{
-    if (DT == LTQ_F32) {
-        const float *p = static_cast<const float *>(base) + at;
-        if (vec) return __ldg(reinterpret_cast<const float4 *>(p));
-        return make_float4(p[0], p[1], p[2], p[3]);
+struct Vec {
+    static constexpr int N = DT == LTQ_F32 ? 4 : 8;
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const void *base, uint64_t at, bool vec)
+    {
+        if (DT == LTQ_F32) {
+            const uint32_t *p = static_cast<const uint32_t *>(base) + at;
+            if (vec) *reinterpret_cast<uint4 *>(w) = __ldg(reinterpret_cast<const uint4 *>(p));
+            else
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = p[i];
+        } else {
+            const uint16_t *p = static_cast<const uint16_t *>(base) + at;
+            if (vec) *reinterpret_cast<uint4 *>(w) = __ldg(reinterpret_cast<const uint4 *>(p));
+            else
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+        }
     }
-    const uint16_t *p = static_cast<const uint16_t *>(base) + at;
-    uint32_t a, b;
-    if (vec) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
-        a = v.x;
-        b = v.y;
-    } else {
-        a = (uint32_t)p[0] | (uint32_t)p[1] << 16;
-        b = (uint32_t)p[2] | (uint32_t)p[3] << 16;
+    __device__ __forceinline__ float4 four(int h) const   // elements 4 h .. 4 h + 3
+    {
+        if (DT == LTQ_F32) return make_float4(__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]), __uint_as_float(w[3]));
+        const uint32_t a = w[2 * h % 4], b = w[(2 * h + 1) % 4];
+        if (DT == LTQ_F16) {
+            const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&a)), y = __half22float2(*reinterpret_cast<const __half2 *>(&b));
+            return make_float4(x.x, x.y, y.x, y.y);
+        }
+        return make_float4(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u), __uint_as_float(b << 16), __uint_as_float(b & 0xFFFF0000u));
     }
-    if (DT == LTQ_F16) {
-        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&a)), y = __half22float2(*reinterpret_cast<const __half2 *>(&b));
-        return make_float4(x.x, x.y, y.x, y.y);
-    }
-    return make_float4(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u), __uint_as_float(b << 16), __uint_as_float(b & 0xFFFF0000u));
-}
+};
 __device__ __forceinline__ float max_nan(float a, float b)
 {
     float r;
@@ -46,8 +53,9 @@ __device__ __forceinline__ float max_nan(float a, float b)
 }  // namespace
 
 // One CTA per (block that a sequence touches, head, K or V): the largest magnitude of the block's new tokens fixes its scale,
-// older codes of the block follow if the scale grew, the new codes are written.  Bound by HBM at large sizes (element + 1
-// bytes per value; the second look at the new tokens hits L1 / L2), by launch latency for one token per sequence.
+// older codes of the block follow if the scale grew, the new codes are written.  The first APPEND_KEEP vectors of every thread (64
+// tokens of 128 halves) stay in registers in between, all loads on their way at once; what goes beyond is read again, out of L2.
+// Bound by HBM at large sizes (element + 1 bytes per value), by launch latency for one token per sequence.
 // Grid: (2 * blocks per sequence, kv_heads, sequences).
 template <int DT>
 __global__ void __launch_bounds__(APPEND_THREADS)
@@ -70,7 +78,8 @@ cache_append_kernel(const ltq_kv_cache cache, const CacheBatch bt, const void *_
         if (threadIdx.x == 0) atomicCAS(bt.status, 0u, STATUS_BAD_BLOCK);
         return;
     }
-    const uint32_t D = cache.head_dim, h = blockIdx.y, per = D / 4;
+    constexpr int VN = Vec<DT>::N;
+    const uint32_t D = cache.head_dim, h = blockIdx.y, per = D / VN;
     const uint64_t slot = (uint64_t)(uint32_t)page * cache.kv_heads + h;
     uint32_t *codes = reinterpret_cast<uint32_t *>((is_v ? cache.v_dev : cache.k_dev) + (slot << bt.log2_bt) * D);
     ltq_qparams *qp = (is_v ? cache.v_qp_dev : cache.k_qp_dev) + slot;
@@ -78,12 +87,30 @@ cache_append_kernel(const ltq_kv_cache cache, const CacheBatch bt, const void *_
     // row of the block's token i: the sequence's row of position p is off + p - (len - n)
     const uint64_t row0 = (uint64_t)((int64_t)s.off + first - (s.len - s.n));
     const uint32_t chunks = (uint32_t)(end - used) * per;
+    auto load = [&](Vec<DT> &x, uint32_t i) {
+        const uint32_t t = i / per;
+        x.load(src, (row0 + used + t) * ld + (uint64_t)h * D + (i - t * per) * VN, vec);
+    };
 
     float most = 0.f;
-    for (uint32_t i = threadIdx.x; i < chunks; i += APPEND_THREADS) {
-        const uint32_t t = i / per, d = (i - t * per) * 4;
-        const float4 x = load4<DT>(src, (row0 + used + t) * ld + (uint64_t)h * D + d, vec);
-        most = max_nan(max_nan(most, max_nan(fabsf(x.x), fabsf(x.y))), max_nan(fabsf(x.z), fabsf(x.w)));
+    auto look = [&](const Vec<DT> &x) {
+#pragma unroll
+        for (int k = 0; k < VN / 4; k++) {
+            const float4 v = x.four(k);
+            most = max_nan(max_nan(most, max_nan(fabsf(v.x), fabsf(v.y))), max_nan(fabsf(v.z), fabsf(v.w)));
+        }
+    };
+    Vec<DT> keep[APPEND_KEEP];
+#pragma unroll
+    for (int j = 0; j < APPEND_KEEP; j++)
+        if (threadIdx.x + j * APPEND_THREADS < chunks) load(keep[j], threadIdx.x + j * APPEND_THREADS);
+#pragma unroll
+    for (int j = 0; j < APPEND_KEEP; j++)
+        if (threadIdx.x + j * APPEND_THREADS < chunks) look(keep[j]);
+    for (uint32_t i = threadIdx.x + APPEND_KEEP * APPEND_THREADS; i < chunks; i += APPEND_THREADS) {
+        Vec<DT> x;
+        load(x, i);
+        look(x);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
@@ -99,20 +126,30 @@ cache_append_kernel(const ltq_kv_cache cache, const CacheBatch bt, const void *_
         const float stored = finite ? scale : __int_as_float(0x7FC00000);
         if (((uintptr_t)qp & 7) == 0) *reinterpret_cast<uint2 *>(qp) = make_uint2(__float_as_uint(stored), 128u);
     }
-    const float inv = quant_screen_inv(scale);
+    const float inv = quant_row_inv(scale);
     if (finite && used && scale > old) {
-        for (uint32_t i = threadIdx.x; i < (uint32_t)used * per; i += APPEND_THREADS) {
+        for (uint32_t i = threadIdx.x; i < (uint32_t)used * (D / 4); i += APPEND_THREADS) {
             const uint32_t w = codes[i];
             const float4 x = make_float4(__fmul_rn(old, (float)((int)(w & 0xFF) - 128)), __fmul_rn(old, (float)((int)((w >> 8) & 0xFF) - 128)),
                                          __fmul_rn(old, (float)((int)((w >> 16) & 0xFF) - 128)), __fmul_rn(old, (float)((int)(w >> 24) - 128)));
-            codes[i] = quant4_u8(x, scale, 128.f, inv);
+            codes[i] = quant4_row(x, scale, 128.f, inv);
         }
     }
-    for (uint32_t i = threadIdx.x; i < chunks; i += APPEND_THREADS) {
-        const uint32_t t = i / per, d = (i - t * per) * 4;
-        uint32_t w = 0x80808080u;
-        if (finite) w = quant4_u8(load4<DT>(src, (row0 + used + t) * ld + (uint64_t)h * D + d, vec), scale, 128.f, inv);
-        codes[(uint32_t)used * per + i] = w;
+    auto put = [&](const Vec<DT> &x, uint32_t i) {
+        uint32_t w[VN / 4];
+#pragma unroll
+        for (int k = 0; k < VN / 4; k++) w[k] = finite ? quant4_row(x.four(k), scale, 128.f, inv) : 0x80808080u;
+        uint32_t *at = codes + ((uint32_t)used * per + i) * (VN / 4);
+        if (VN == 8) *reinterpret_cast<uint2 *>(at) = make_uint2(w[0], w[VN / 4 - 1]);
+        else at[0] = w[0];
+    };
+#pragma unroll
+    for (int j = 0; j < APPEND_KEEP; j++)
+        if (threadIdx.x + j * APPEND_THREADS < chunks) put(keep[j], threadIdx.x + j * APPEND_THREADS);
+    for (uint32_t i = threadIdx.x + APPEND_KEEP * APPEND_THREADS; i < chunks; i += APPEND_THREADS) {
+        Vec<DT> x;
+        load(x, i);
+        put(x, i);
     }
 }
 
@@ -122,8 +159,7 @@ cudaError_t launch_cache_append(const ltq_kv_cache &c, const CacheBatch &bt, con
     // n tokens from any offset touch at most (n + block_tokens - 2) / block_tokens + 1 blocks
     const uint32_t bt_tokens = 1u << bt.log2_bt, blocks = (bt.max_new + bt_tokens - 2) / bt_tokens + 1;
     const dim3 grid(2 * blocks, c.kv_heads, bt.seqs);
-    const uint64_t e4 = 4 * dtype_size(dtype);
-    const bool vec = ld % 4 == 0 && (((uintptr_t)k | (uintptr_t)v) % e4) == 0;
+    const bool vec = (ld * dtype_size(dtype)) % 16 == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
     count_launch();
     if (dtype == LTQ_F32) return launch_chained(cache_append_kernel<LTQ_F32>, grid, dim3(APPEND_THREADS), 0, stream, c, bt, k, v, ld, vec);
     if (dtype == LTQ_F16) return launch_chained(cache_append_kernel<LTQ_F16>, grid, dim3(APPEND_THREADS), 0, stream, c, bt, k, v, ld, vec);

@@ -96,4 +96,33 @@ __device__ __forceinline__ uint32_t quant4_u8(float4 x, float scale, float zpf, 
     return quant4_u8_careful(x, scale, zpf, inv);
 }
 
+// ---- without screening, for parameters per row or block ------------------------------------------------------------------
+// The reference's sequence in eight operations and no branch, for callers whose scale changes from row to row and whose
+// elements are many per byte (16-bit input): the screened form's branch per four elements costs more there than it saves
+// (16384 x 8192 bfloat16: 108 us screened, 134 M elements).
+//
+// The quotient: with y = fl(1 / scale), q = fl(x y), r = x - q scale (exact as a fused multiply-add), fl(q + r y) is the
+// correctly rounded x / scale (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990)
+// while nothing underflows: scale within [1e-20, 1e30], and quotients too small for that round to the zero point anyway.
+// Rounding half away from zero: v + 0.5 and the sum with 2^23, both rounded down, leave floor(v + 0.5).
+__device__ __forceinline__ float quant_row_inv(float scale) { return scale > 1e-20f && scale < 1e30f ? __fdiv_rn(1.f, scale) : 0.f; }
+
+// The byte in the low mantissa bits.  zpf + x / scale must not be below -0.5: with zpf = round(-lo / scale), half away from zero, the
+// row's smallest value lies above it.
+__device__ __forceinline__ uint32_t quant_row1(float x, float scale, float zpf, float inv)
+{
+    const float q = __fmul_rn(x, inv), v = fminf(__fadd_rn(zpf, fmaf(fmaf(-q, scale, x), inv, q)), 255.f);
+    return __float_as_uint(__fadd_rz(__fadd_rz(v, 0.5f), 8388608.f));
+}
+// Four values of a row that the parameters were made from; same bytes as quant_u8_exact.  inv: quant_row_inv(scale); 0 takes the exact path.
+__device__ __forceinline__ uint32_t quant4_row(float4 x, float scale, float zpf, float inv)
+{
+    if (inv == 0.f)
+        return quant_u8_exact(x.x, scale, zpf) | quant_u8_exact(x.y, scale, zpf) << 8 | quant_u8_exact(x.z, scale, zpf) << 16 |
+               quant_u8_exact(x.w, scale, zpf) << 24;
+    const uint32_t a = quant_row1(x.x, scale, zpf, inv), b = quant_row1(x.y, scale, zpf, inv);
+    const uint32_t c = quant_row1(x.z, scale, zpf, inv), d = quant_row1(x.w, scale, zpf, inv);
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
 }  // namespace ltq
