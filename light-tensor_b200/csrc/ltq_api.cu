@@ -11,6 +11,7 @@
 
 #include "ltq_common.cuh"
 #include "ltq_gemm_tc.cuh"
+#include "ltq_gemm_small.cuh"
 #include "ltq_gemv.cuh"
 #include "ltq_conv_direct.cuh"
 #include "ltq_layer.cuh"
@@ -285,10 +286,15 @@ int ltq::run_fc_gemm(const GemmDevice &gd, uint64_t M, uint64_t N, uint64_t K, c
                                      layer != nullptr, layer && layer->next.W ? &layer->next : nullptr));
             break;
         case PATH_TC: {
+            const bool tokens = out_is_tokens(epi.out_mode);
+            const SmallPlan plan = tokens ? small_plan(M, N, K, dev->sms) : SmallPlan{0, 0, 0, 0};
+            // Parameters per token: the kernel for few tiles where its tiles are one round of the device, the pair kernel beyond it
+            // (N = 11008, K = 4096: 77 tokens, one round, 12.0 us against 13.9; 256 tokens, two rounds, 23.3 against 14.9).
             const bool pair = !(flags & LTQ_FLAG_FORCE_TC_SINGLE) &&
-                              ((flags & LTQ_FLAG_FORCE_TC_PAIR) || tc_pair_preferred(M, N, dev->sms));
+                              ((flags & LTQ_FLAG_FORCE_TC_PAIR) || tc_pair_preferred(M, N, dev->sms) || plan.rounds > 1);
+            const bool small = !pair && tokens;
             TcOperandMap map_a;
-            int er = tc_make_map(&map_a, A, M, K, 128);
+            int er = small ? 0 : tc_make_map(&map_a, A, M, K, 128);
             LTQ_REQUIRE(er == 0, LTQ_ERR_CUDA, "cuTensorMapEncodeTiled failed for the activation operand (CUresult %d)", er);
             // Weight maps by box height: the tile width for the single-CTA kernel (64, 128, 256), half the width of
             // each class of tiles for the pair kernel.  A layer caches the ones it has needed so far.
@@ -319,6 +325,11 @@ int ltq::run_fc_gemm(const GemmDevice &gd, uint64_t M, uint64_t N, uint64_t K, c
                     LTQ_REQUIRE(er == 0, LTQ_ERR_CUDA, "cuTensorMapEncodeTiled failed for the weight operand (CUresult %d)", er);
                 }
                 LTQ_CUDA_TRY(launch_gemm_tc_pair(map_a, maps, tl, M, N, K, epi, out, dev->status, dev->sms, stream));
+            } else if (small) {
+                TcOperandMap *mb = layer ? &layer->map_w_small : &tmp_b[0];
+                er = small_maps(plan, A, M, K, &map_a, B, N, mb);
+                LTQ_REQUIRE(er == 0, LTQ_ERR_CUDA, "cuTensorMapEncodeTiled failed for an operand (CUresult %d)", er);
+                LTQ_CUDA_TRY(launch_gemm_small(map_a, *mb, plan, M, N, K, epi, out, dev->status, stream, layer != nullptr));
             } else {
                 const int bn = tc_pick_bn(M, N, dev->sms);
                 TcOperandMap *mb;
@@ -440,6 +451,7 @@ int ltq_layer_set_weights(ltq_layer *layer, const uint8_t *w_dev, const int32_t 
     layer->qp_channels = nullptr;   // parameters per channel belong to the weights they were given for
     for (auto &m : layer->map_w) m = TcOperandMap();
     layer->map_w_gemv = GemvWeightMaps();
+    layer->map_w_small = TcOperandMap();
     LTQ_CUDA_TRY(launch_row_sums(w_dev, layer->N, layer->K, layer->wsum, (cudaStream_t)stream));
     LTQ_CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
     return LTQ_OK;

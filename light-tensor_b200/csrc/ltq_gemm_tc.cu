@@ -32,37 +32,34 @@ constexpr int BK = 128;          // bytes (= elements) of K per smem stage: one 
 constexpr int UMMA_K = 32;       // kind::i8
 constexpr int NUM_THREADS = 192;
 
-// Bytes of column terms per output column in shared memory: one correction word, or the 16 bytes of token_col.
-__host__ __device__ constexpr int col_bytes(int out) { return out_is_tokens(out) ? 16 : 4; }
-
-template <int BN, int OUT>
+template <int BN>
 struct Cfg {
     static constexpr int STAGES = (BN == 256) ? 4 : (BN == 128 ? 6 : 8);
     static constexpr int A_BYTES = BM * BK;
     static constexpr int B_BYTES = BN * BK;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int TMEM_COLS = (2 * BN < 32) ? 32 : 2 * BN;  // power of two >= 32
-    // ring + 1024 B alignment slack + column terms (two tiles) + barriers
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 2 * BN * col_bytes(OUT) + 256;
+    // ring + 1024 B alignment slack + column terms (2 x BN x 4) + barriers
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 2 * BN * 4 + 256;
 };
 
 }  // namespace
 
-// OUT: 0 = uint8, 1 = float, 2 = int32 (ltq_out_mode), OUT_TOKENS + ltq_dtype = parameters per token and channel.
+// OUT: 0 = uint8, 1 = float, 2 = int32 (ltq_out_mode).
 template <int BN, int OUT>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, uint32_t M,
                uint32_t N, uint32_t K, Epilogue epi, void *__restrict__ out, uint32_t *status)
 {
     griddep_launch_dependents();
-    using C = Cfg<BN, OUT>;
+    using C = Cfg<BN>;
     extern __shared__ uint8_t smem_raw[];
     // 128B-swizzled tiles need a 1024-byte aligned base.
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;
     uint8_t *after = smem_raw + (ring - raw) + C::STAGES * C::STAGE_BYTES;
     uint32_t *s_col = reinterpret_cast<uint32_t *>(after);                 // [2][BN] column terms
-    uint64_t *bars = reinterpret_cast<uint64_t *>(after + 2 * BN * col_bytes(OUT));  // full[S] empty[S] tfull[2] tempty[2]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(after + 2 * BN * 4);     // full[S] empty[S] tfull[2] tempty[2]
     uint32_t *s_misc = reinterpret_cast<uint32_t *>(bars + 2 * C::STAGES + 4);  // [0] tmem base, [1] abort flag
     volatile uint32_t *abort_flag = s_misc + 1;
 
@@ -156,42 +153,6 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         // ---------------- epilogue (warps 2..5 = 128 threads) ----------------
         const uint32_t q = (uint32_t)warp & 3u;       // TMEM lane quarter this warp may read
         const uint32_t et = threadIdx.x - 64;         // 0..127
-        if constexpr (out_is_tokens(OUT)) {
-            const bool relu = epi.flags & LTQ_FLAG_RELU;
-            const uint64_t ldc = epilogue_pitch(epi, N);
-            const bool vec_ok = epilogue_vec_ok(epi, out, N, OUT == OUT_TOKENS + LTQ_F32 ? 4 : 2);
-            uint32_t as = 0, aph = 0;
-            bool ok = true;
-            for (uint32_t t = blockIdx.x; t < num_tiles; t += gridDim.x) {
-                const uint32_t m0 = (t / tiles_n) * BM, n0 = (t % tiles_n) * BN;
-                uint4 *col = reinterpret_cast<uint4 *>(s_col) + as * BN;
-                for (uint32_t j = et; j < (uint32_t)BN; j += 128) {
-                    const uint32_t gj = n0 + j;
-                    col[j] = gj < N ? token_col(epi, gj) : make_uint4(0, 0, 0, 0);
-                }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                const uint32_t row = m0 + q * 32 + lane;
-                const TokenRow tr = row < M ? token_row(epi, row) : TokenRow{0, 0, 0.f};
-                if (ok) ok = mbar_wait(tfull0 + 8 * as, aph, abort_flag, status, 0x400u | as);
-                if (ok) {
-                    tc_fence_after();
-                    const uint32_t taddr = tmem_base + ((q * 32u) << 16) + as * BN;
-#pragma unroll 1
-                    for (int ch = 0; ch < BN / 32; ch++) {
-                        uint32_t v[32];
-                        tmem_ld32(taddr + ch * 32, v);
-                        tmem_ld_wait();
-                        const uint32_t c0 = n0 + ch * 32;
-                        if (row < M && c0 < N)
-                            token_chunk<OUT, 32>(v, tr, col + ch * 32, relu, out, row * ldc + c0, vec_ok, (N - c0) < 32u ? (int)(N - c0) : 32);
-                    }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(tempty0 + 8 * as);
-                }
-                if (++as == 2) { as = 0; aph ^= 1; }
-            }
-        } else {
         const EpilogueConsts c = epilogue_consts(epi);
         const bool relu = epi.flags & LTQ_FLAG_RELU, sat = epi.flags & LTQ_FLAG_SATURATE;
         using OutT = typename std::conditional<OUT == 0, uint8_t, typename std::conditional<OUT == 1, float, int32_t>::type>::type;
@@ -234,7 +195,6 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             }
             if (++as == 2) { as = 0; aph ^= 1; }
         }
-        }
     }
 
     // Teardown: nobody leaves before every role is done with TMEM and shared memory.
@@ -276,6 +236,9 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 // exchange's three dependent L2 round trips cost 6 us).
 namespace {
 
+// Bytes of column terms per output column in shared memory: one correction word, or the 16 bytes of token_col.
+__host__ __device__ constexpr int col_bytes(int out) { return out_is_tokens(out) ? 16 : 4; }
+
 constexpr int P_MAX_STAGES = 6;
 constexpr int P_THREADS = 64 + 8 * 32;  // producer warp, MMA warp, 8 epilogue warps
 constexpr int P_BN = 256;               // widest tile
@@ -285,8 +248,9 @@ constexpr int P_STAGE_BYTES = P_A_BYTES + P_B_BYTES;
 constexpr int P_PEER_STAGE_BYTES = 8 * PeerStage::BYTES_PER_WARP;
 inline size_t pair_smem_bytes(int stages, bool peer_stage, int out)
 {
-    // ring + alignment slack + column terms + barriers
-    return (size_t)stages * P_STAGE_BYTES + 1024 + 2 * P_BN * col_bytes(out) + 256 + (peer_stage ? P_PEER_STAGE_BYTES : 0);
+    // ring + alignment slack + column terms + barriers, then the epilogue warps' staging areas
+    return (size_t)stages * P_STAGE_BYTES + 1024 + 2 * P_BN * col_bytes(out) + 256 + (peer_stage ? P_PEER_STAGE_BYTES : 0) +
+           (out_is_tokens(out) ? 8 * TokenStage::BYTES_PER_WARP : 0);
 }
 
 struct PairTile {
@@ -443,6 +407,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             const bool relu = epi.flags & LTQ_FLAG_RELU;
             const uint64_t ldc = epilogue_pitch(epi, N);
             const bool vec_ok = epilogue_vec_ok(epi, out, N, OUT == OUT_TOKENS + LTQ_F32 ? 4 : 2);
+            float *stage = reinterpret_cast<float *>(s_stage + (warp - 2) * TokenStage::BYTES_PER_WARP);
             uint32_t as = 0, aph = 0;
             bool ok = true;
             for (uint32_t t = pair; t < num_tiles; t += num_pairs) {
@@ -467,8 +432,13 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     auto chunk = [&](auto &v) {
                         constexpr int CW = (int)(sizeof(v) / sizeof(uint32_t));
                         const uint32_t c0 = n0 + cc;
-                        if (row < M && c0 < N)
-                            token_chunk<OUT, CW>(v, tr, col + cc, relu, out, row * ldc + c0, vec_ok, (N - c0) < (uint32_t)CW ? (int)(N - c0) : CW);
+                        const int valid = c0 >= N ? 0 : ((N - c0) < (uint32_t)CW ? (int)(N - c0) : CW);
+                        if (vec_ok) {
+                            if (row < M && valid) token_chunk<OUT, CW>(v, tr, col + cc, relu, out, row * ldc + c0, true, valid);
+                        } else {
+                            TokenStage::chunk<OUT, CW>(stage, v, tr, col + cc, relu, out, (uint64_t)(m0 + q * 32) * ldc + c0, ldc,
+                                                       m0 + q * 32 < M ? (int)(M - m0 - q * 32) : 0, valid);
+                        }
                     };
 #pragma unroll 1
                     for (; cc + 32 <= ce; cc += 32) {
@@ -614,7 +584,7 @@ template <int BN, int OUT>
 cudaError_t launch_cfg(const CUtensorMap &ma, const CUtensorMap &mb, uint64_t M, uint64_t N, uint64_t K,
                        const Epilogue &epi, void *out, uint32_t *status, int sms, cudaStream_t stream)
 {
-    using C = Cfg<BN, OUT>;
+    using C = Cfg<BN>;
     static bool attr_done[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -640,9 +610,6 @@ cudaError_t launch_out(const CUtensorMap &ma, const CUtensorMap &mb, uint64_t M,
     switch (epi.out_mode) {
         case LTQ_OUT_U8: return launch_cfg<BN, 0>(ma, mb, M, N, K, epi, out, status, sms, stream);
         case LTQ_OUT_F32: return launch_cfg<BN, 1>(ma, mb, M, N, K, epi, out, status, sms, stream);
-        case OUT_TOKENS + LTQ_F32: return launch_cfg<BN, OUT_TOKENS + LTQ_F32>(ma, mb, M, N, K, epi, out, status, sms, stream);
-        case OUT_TOKENS + LTQ_F16: return launch_cfg<BN, OUT_TOKENS + LTQ_F16>(ma, mb, M, N, K, epi, out, status, sms, stream);
-        case OUT_TOKENS + LTQ_BF16: return launch_cfg<BN, OUT_TOKENS + LTQ_BF16>(ma, mb, M, N, K, epi, out, status, sms, stream);
         default: return launch_cfg<BN, 2>(ma, mb, M, N, K, epi, out, status, sms, stream);
     }
 }

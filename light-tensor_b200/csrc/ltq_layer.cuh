@@ -27,6 +27,7 @@ struct ltq_layer {
     uint64_t padded_k() const { return (K + 15) / 16 * 16; }
     ltq::TcOperandMap map_w[LAYER_MAPS];  // weight tensor maps of the tensor-core kernels, one per box height, built on demand
     int map_w_next = 0;
+    ltq::TcOperandMap map_w_small;      // weight tensor map of the kernel for few tiles, of its last plan
     ltq::GemvWeightMaps map_w_gemv;     // weight tensor maps of the skinny kernel
     ltq::GemvNext next;                 // weights of the layer that runs after this one (ltq_layer_set_next), with
     ltq::GemvWeightMaps map_next_gemv;  // their tensor maps as the skinny kernel of THIS layer needs them

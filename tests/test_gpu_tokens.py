@@ -178,7 +178,9 @@ def run_product(ltq, c, dtype, flags, out=None):
 
 
 SHAPES = [(1, 1, 1), (1, 8, 128), (3, 130, 256), (16, 264, 1024), (17, 64, 48), (5, 7, 3), (33, 31, 100), (128, 128, 128), (129, 257, 272),
-          (64, 4099, 256), (300, 640, 512), (1, 11008, 512), (16, 2048, 4096)]
+          (64, 4099, 256), (300, 640, 512), (1, 11008, 512), (16, 2048, 4096),
+          # few tiles: K divided over clusters, one, two and four lines of K per copy, rows that are no multiple of eight
+          (77, 1024, 4096), (32, 200, 8192), (20, 1030, 2048), (100, 264, 8192), (40, 100, 2064), (33, 520, 5008), (130, 96, 4096), (24, 4096, 1152)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -192,9 +194,9 @@ def test_product_is_exact_up_to_its_float_steps(cuda, dtype, M, N, K):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("flag,kernel,M,N,K", [("FLAG_FORCE_SIMT", "gemm_simt", 70, 90, 64), ("FLAG_FORCE_TC_SINGLE", "gemm_tc_kernel", 200, 500, 144),
+@pytest.mark.parametrize("flag,kernel,M,N,K", [("FLAG_FORCE_SIMT", "gemm_simt", 70, 90, 64), ("FLAG_FORCE_TC_SINGLE", "gemm_small_kernel", 200, 500, 144),
                                                ("FLAG_FORCE_TC_PAIR", "gemm_tc_pair_kernel", 333, 777, 208), ("FLAG_FORCE_SKINNY", "gemv_kernel", 11, 1000, 384),
-                                               ("FLAG_FORCE_TC_PAIR", "gemm_tc_pair_kernel", 2048, 2048, 256)])
+                                               ("FLAG_FORCE_TC_PAIR", "gemm_tc_pair_kernel", 2048, 2048, 256), ("FLAG_FORCE_TC_PAIR", "gemm_tc_pair_kernel", 700, 2051, 384)])
 def test_every_kernel_gives_the_same_product(cuda, dtype, flag, kernel, M, N, K):
     import ltq
     c = product_case(cuda, N, M, N, K, True)
