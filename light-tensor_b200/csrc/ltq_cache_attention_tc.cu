@@ -52,26 +52,30 @@ template <int D>
 struct TcGeo {
     static constexpr int RT = D <= 128 ? 2 : 1;                    // row tiles per CTA
     static constexpr int KEYS = 64, GROUPS = KEYS / 16;
-    static constexpr int PARTS = RT == 2 ? 1 : 2, PART = KEYS / PARTS;   // a tile is converted in so many parts
+    static constexpr int PARTS = RT == 2 ? 1 : 2, PART = KEYS / PARTS;   // a tile is fetched and converted in so many parts
+    static constexpr int RAW = RT == 2 ? 4 : 2;                    // parts whose codes are on their way or waiting
+    static constexpr int V_GROUP = 8 * D + 16;                     // eight keys of V, 16 bytes apart: reads of a column spread over the banks
+    static constexpr int RAW_BYTES = PART * D + PART / 8 * V_GROUP - 16;
     static constexpr int SB = 2;                                   // S buffers per row tile
     static constexpr int PANELS = (D + 63) / 64;                   // 64 halves = one 128-byte swizzle row
     static constexpr int Q_BYTES = PANELS * TC_ROWS * 128;
     static constexpr int K_BYTES = PANELS * KEYS * 128;
     static constexpr int V_BYTES = D * 128;                        // rows = head dimensions, 64 keys = 128 bytes
-    static constexpr int THREADS = 128 * (RT + 3);                 // warpgroups: softmax per row tile, K, V, MMA issue
-    // Registers per thread: as launched (640 or 512 threads), and after setmaxnreg, which may only raise with .inc, lower with .dec,
+    static constexpr int SW = RT * SB;                             // softmax warpgroups: one per row tile and S buffer
+    static constexpr int THREADS = 128 * (SW + 3);                 // warpgroups: softmax, K, V, MMA issue
+    // Registers per thread: as launched (896 or 640 threads), and after setmaxnreg, which may only raise with .inc, lower with .dec,
     // and hands out no more than the block was launched with.
-    static constexpr int REGS = RT == 2 ? 96 : 128;
-    static constexpr int REGS_SOFTMAX = RT == 2 ? 136 : 200, REGS_CONVERT = RT == 2 ? 80 : 128, REGS_MMA = RT == 2 ? 48 : 56;
-    static_assert(RT * REGS_SOFTMAX + 2 * REGS_CONVERT + REGS_MMA == (RT + 3) * REGS, "register shares");
+    static constexpr int REGS = RT == 2 ? 72 : 96;
+    static constexpr int REGS_SOFTMAX = RT == 2 ? 88 : 136, REGS_CONVERT = RT == 2 ? 56 : 80, REGS_MMA = RT == 2 ? 40 : 48;
+    static_assert(SW * REGS_SOFTMAX + 2 * REGS_CONVERT + REGS_MMA == (SW + 3) * REGS, "register shares");
     static_assert(REGS_SOFTMAX >= REGS && REGS_CONVERT <= REGS && REGS_MMA <= REGS, "register shares");
-    static constexpr int BARS = 8 + RT * (2 * SB + SB) + 1;        // k_full k_empty v_full v_empty; s_full p_full pv_done per row tile; q_full
+    static constexpr int BARS = 9 + RT * 3 * SB + SW * 4 + 2 * RAW;   // k_full k_empty v_full v_empty q_full; s_full p_full pv_done; m_done; raw_full raw_empty
     struct TilePar {
         GroupPar g[GROUPS];
         float v_ref, rescale;   // the reference, and what O so far has to be multiplied with for it
         uint32_t bad, pad;      // bit i: group i's block does not exist
     };
-    static constexpr size_t SMEM = 1024 + RT * Q_BYTES + 2 * K_BYTES + 2 * V_BYTES + 8 * sizeof(TilePar) + BARS * 8 + 16;
+    static constexpr size_t SMEM = 1024 + RT * Q_BYTES + 2 * K_BYTES + 2 * V_BYTES + RAW * RAW_BYTES + 8 * sizeof(TilePar) + SW * TC_ROWS * 4 + (BARS + BARS % 2) * 8 + RAW * 16 + 16;
     static_assert(SMEM <= 227 * 1024, "shared memory");
     static __device__ __forceinline__ uint32_t o_col(uint32_t rt) { return rt * 128; }
     static __device__ __forceinline__ uint32_t s_col(uint32_t rt, uint32_t sb) { return 256 + rt * 128 + sb * 64; }
@@ -158,17 +162,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32])
-{
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
-        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
-        "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
-        : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16])
 {
     asm volatile(
@@ -202,20 +195,24 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), sq = (raw + 1023u) & ~1023u;
     const uint32_t sk = sq + RT * G::Q_BYTES, sv = sk + 2 * G::K_BYTES;
-    uint8_t *after = smem_raw + (sv - raw) + 2 * G::V_BYTES;
+    uint8_t *codes = smem_raw + (sv - raw) + 2 * G::V_BYTES, *after = codes + G::RAW * G::RAW_BYTES;   // a part: K, then V in groups of eight keys
     TilePar *s_par = reinterpret_cast<TilePar *>(after);     // of eight tiles
-    uint64_t *bars = reinterpret_cast<uint64_t *>(after + 8 * sizeof(TilePar));
-    uint32_t *s_misc = reinterpret_cast<uint32_t *>(bars + G::BARS);   // [0] tmem base, [1] abort flag
+    float *s_m = reinterpret_cast<float *>(after + 8 * sizeof(TilePar));   // [row tile][S buffer][row]: the reference maximum
+    uint64_t *bars = reinterpret_cast<uint64_t *>(s_m + G::SW * TC_ROWS);
+    uint32_t(*s_zero)[4] = reinterpret_cast<uint32_t(*)[4]>(bars + G::BARS + G::BARS % 2);   // zero points of a part's V, per 16 keys
+    uint32_t *s_misc = reinterpret_cast<uint32_t *>(s_zero + G::RAW);   // [0] tmem base, [1] abort flag, [2] stays 0
     volatile uint32_t *abort_flag = s_misc + 1;
     const uint32_t k_full = smem_u32(bars), k_empty = k_full + 16, v_full = k_full + 32, v_empty = k_full + 48, q_full = k_full + 64;
-    const uint32_t s_full = k_full + 72, p_full = s_full + 8 * SB * RT, pv_done = p_full + 8 * SB * RT;   // [row tile][S buffer]
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t s_full = k_full + 72, p_full = s_full + 8 * SB * RT, pv_done = p_full + 8 * SB * RT,   // [row tile][S buffer]
+                   m_done = pv_done + 8 * SB * RT,                                                           // [row tile][S buffer][warp]
+                   raw_full = m_done + 8 * 4 * G::SW, raw_empty = raw_full + 8 * G::RAW;
+    const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // (known to be uniform)
     const uint32_t wg = (uint32_t)warp >> 2;
     uint32_t *status = a.bt.status;
 
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < 2; i++) {
-            mbar_init(k_full + 8 * i, 128);
+            mbar_init(k_full + 8 * i, 129);
             mbar_init(k_empty + 8 * i, RT);
             mbar_init(v_full + 8 * i, 128);
             mbar_init(v_empty + 8 * i, RT);
@@ -225,8 +222,13 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             mbar_init(p_full + 8 * i, 4);
             mbar_init(pv_done + 8 * i, 1);
         }
-        mbar_init(q_full, 128 * RT);
-        s_misc[1] = 0;
+        for (uint32_t i = 0; i < G::SW * 4; i++) mbar_init(m_done + 8 * i, 1);
+        for (uint32_t i = 0; i < (uint32_t)G::RAW; i++) {
+            mbar_init(raw_full + 8 * i, 1);
+            mbar_init(raw_empty + 8 * i, 8);
+        }
+        mbar_init(q_full, 128 * G::SW);
+        s_misc[1] = s_misc[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -261,152 +263,196 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
     if (a.splits > 1 && split == 0 && row0 < rows && threadIdx.x == 0)
         a.item[((uint64_t)b * gridDim.z + group) * a.cache.kv_heads + h] = make_int2((int)place, (int)(place + a.splits - 1));
 
-    if (wg < RT) {
-        // ---------------- softmax: one row per thread ----------------
-        regs_up<G::REGS_SOFTMAX>();
-        const uint32_t rt = wg, mine = rt ? tiles1 : tiles0;
-        const uint32_t r = ((uint32_t)warp & 3) * 32 + lane, row = row0 + rt * TC_ROWS + r, t = row / a.group;
-        const bool real = row < rows;
-        const uint16_t *q = static_cast<const uint16_t *>(a.q) + ((uint64_t)s.off + t) * a.ld_q + (uint64_t)(h * a.group + row - t * a.group) * D;
-        auto eight = [&](int d, uint32_t (&w)[4]) {   // eight neighbouring elements
-            if (!real) {
-                w[0] = w[1] = w[2] = w[3] = 0;
-            } else if (a.q_vec8) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(q + d));
-                w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = (uint32_t)q[d + 2 * i] | (uint32_t)q[d + 2 * i + 1] << 16;
-            }
-        };
-        uint32_t qw[D / 8][4];   // the whole row: one memory latency
-#pragma unroll
-        for (int d = 0; d < D / 8; d++) eight(8 * d, qw[d]);
-        float most = 0.f;
-        bool finite = true;
-#pragma unroll
-        for (int d = 0; d < D / 8; d++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float v = fabsf(elem<DT>(qw[d][i / 2], i & 1));
-                finite = finite && v < INFINITY;
-                most = fmaxf(most, v);
-            }
-        int e = 0;   // most * 2^e in [2^10, 2^11)
-        if (most > 0.f && finite) {
-            e = 10 - ilogbf(most);
-            e = e > 100 ? 100 : e;
-        }
-        const float f = ldexpf(1.f, e);
-        const float row_scale = finite ? a.scale_log2 * ldexpf(1.f, -e) : __int_as_float(0x7FC00000);
-        float q_sum = 0.f;
-#pragma unroll
-        for (int d = 0; d < D / 8; d++) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                w[i] = finite ? h2pack(elem<DT>(qw[d][i], 0) * f, elem<DT>(qw[d][i], 1) * f) : 0u;
-                const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-                q_sum += x.x + x.y;
-            }
-            sts16(sq + rt * G::Q_BYTES + (d / 8) * (TC_ROWS * 128) + r * 128 + (((d & 7) ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(q_full);
+    const int32_t *table = a.bt.table + (uint64_t)b * a.bt.table_width;
+    const uint32_t in_block = (1u << a.bt.log2_bt) - 1, parts = G::PARTS * tiles;
+    const uint32_t begin = tile0 * G::KEYS, end = (tile0 + tiles) * G::KEYS, last_key = end < (uint32_t)s.len ? end - 1 : (uint32_t)s.len - 1;
+    // the block that holds a key; keys behind the sequence's last read its block (masked later)
+    auto page_of = [&](uint32_t key) { return __ldg(table + ((key < last_key ? key : last_key) >> a.bt.log2_bt)); };
+    auto slot_of = [&](int32_t page) { return (uint64_t)((uint32_t)page < a.cache.blocks ? (uint32_t)page : 0u) * a.cache.kv_heads + h; };
 
-        const float zero_scale = row_scale * q_sum;
+    if (wg < G::SW) {
+        // ---------------- softmax: one row per thread, this warpgroup's half of the tiles ----------------
+        regs_up<G::REGS_SOFTMAX>();
+        const uint32_t rt = wg / SB, sb = wg % SB, quarter = (uint32_t)warp & 3, mine = rt ? tiles1 : tiles0;
+        const uint32_t r = quarter * 32 + lane, row = row0 + rt * TC_ROWS + r, t = row / a.group;
+        const bool real = row < rows;
+        auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + rt * 4 + quarter) : "memory"); };             // with the rows' other warp
+        auto meet_all = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(1 + RT * 4 + rt) : "memory"); };   // the row tile's warps
+        // 16 rows of q per warp, whole rows at a time: a power of two on each, so that halves hold it.
+        float2 *const row_par = reinterpret_cast<float2 *>(s_m) + rt * TC_ROWS;
+        {
+            constexpr int LANES = D <= 32 ? 4 : (D <= 64 ? 8 : (D <= 128 ? 16 : 32)), PASSES = LANES / 2;   // lanes per row, eight elements each
+            const int at = lane % LANES;
+            const bool has = at < D / 8;
+            uint32_t qw[PASSES][4];   // one memory latency
+            auto row_of = [&](int i) { return (sb * 4 + quarter) * 16 + (uint32_t)(i * (32 / LANES) + lane / LANES); };
+#pragma unroll
+            for (int i = 0; i < PASSES; i++) {
+                const uint32_t qr = row0 + rt * TC_ROWS + row_of(i), qt = qr / a.group;
+                const uint16_t *q = static_cast<const uint16_t *>(a.q) + ((uint64_t)s.off + qt) * a.ld_q + (uint64_t)(h * a.group + qr - qt * a.group) * D + 8 * at;
+                qw[i][0] = qw[i][1] = qw[i][2] = qw[i][3] = 0;
+                if (qr < rows && has) {
+                    if (a.q_vec8) {
+                        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(q));
+                        qw[i][0] = v.x; qw[i][1] = v.y; qw[i][2] = v.z; qw[i][3] = v.w;
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) qw[i][k] = (uint32_t)q[2 * k] | (uint32_t)q[2 * k + 1] << 16;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < PASSES; i++) {
+                float most = 0.f;   // infinity for a row with anything that is not finite
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float v = fabsf(elem<DT>(qw[i][k / 2], k & 1));
+                    most = v < INFINITY ? fmaxf(most, v) : INFINITY;
+                }
+#pragma unroll
+                for (int o = 1; o < LANES; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+                const bool finite = most < INFINITY;
+                int e = 0;   // most * 2^e in [2^10, 2^11)
+                if (most > 0.f && finite) {
+                    e = 10 - ilogbf(most);
+                    e = e > 100 ? 100 : e;
+                }
+                const float f = ldexpf(1.f, e);
+                float q_sum = 0.f;
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    w[k] = finite ? h2pack(elem<DT>(qw[i][k], 0) * f, elem<DT>(qw[i][k], 1) * f) : 0u;
+                    const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
+                    q_sum += x.x + x.y;
+                }
+#pragma unroll
+                for (int o = 1; o < LANES; o <<= 1) q_sum += __shfl_xor_sync(0xFFFFFFFFu, q_sum, o);
+                const uint32_t qr = row_of(i);
+                if (has) sts16(sq + rt * G::Q_BYTES + (at / 8) * (TC_ROWS * 128) + qr * 128 + (((at & 7) ^ (qr & 7)) << 4), w[0], w[1], w[2], w[3]);
+                if (at == 0) {
+                    const float row_scale = finite ? a.scale_log2 * ldexpf(1.f, -e) : __int_as_float(0x7FC00000);
+                    row_par[qr] = make_float2(row_scale, row_scale * q_sum);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(q_full);
+        }
+        meet_all();
+        const float row_scale = row_par[r].x, zero_scale = row_par[r].y;
+        meet_all();   // (what follows takes the place)
         const int pos = real ? s.len - s.n + (int)t : 0x7FFFFFFF;
         const int first_pos = __reduce_min_sync(0xFFFFFFFFu, pos);
-        const uint32_t lane_addr = tmem + ((((uint32_t)warp & 3) * 32) << 16), o_addr = lane_addr + G::o_col(rt);
-        const uint32_t s_bar = s_full + 8 * SB * rt, p_bar = p_full + 8 * SB * rt, pv_bar = pv_done + 8 * SB * rt;
-        float m = -INFINITY, l = 0.f, v_ref = TC_SMALLEST;
+        const uint32_t lane_addr = tmem + ((quarter * 32) << 16), o_addr = lane_addr + G::o_col(rt), s_addr = lane_addr + G::s_col(rt, sb);
+        const uint32_t s_bar = s_full + 8 * wg, p_bar = p_full + 8 * wg, pv_bar = pv_done + 8 * SB * rt;
+        const uint32_t m_bar = m_done + 8 * (wg * 4 + quarter), m_other = m_done + 8 * ((wg ^ 1) * 4 + quarter);
+        float m = -INFINITY, l = 0.f;
         bool ok = true;
-        for (uint32_t j = 0; j < mine; j++) {
-            const uint32_t sb = j % SB, ph = (j / SB) & 1;
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(s_bar + 8 * sb, ph, abort_flag, status, 0xB00u | sb));
+        for (uint32_t j = sb; j < mine; j += SB) {
+            const uint32_t ph = (j / SB) & 1;
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(s_bar, ph, abort_flag, status, 0xB00u | sb));
             if (!ok) break;
             tc_fence_after();
-            const uint32_t s_addr = lane_addr + G::s_col(rt, sb);
             const TilePar &par = s_par[j & 7];
-            uint32_t x[2][32];
-            auto load_scores = [&]() {
-                tmem_ld32(s_addr, x[0]);
-                tmem_ld32(s_addr + 32, x[1]);
-            };
-            load_scores();   // (the tile's parameters are read while they are on their way)
-            GroupPar g[G::GROUPS];
-#pragma unroll
-            for (int k = 0; k < G::GROUPS; k++) g[k] = par.g[k];
             const int key0 = (int)((tile0 + j) * G::KEYS);
             const uint32_t bad = par.bad;
             const bool masked = bad || key0 + G::KEYS - 1 > first_pos;
-            v_ref = par.v_ref;
-            float alpha = par.rescale, sum = 0.f;
-            uint32_t p[G::KEYS / 2];
-            // P of the tile under the reference `ref`, and the sum of its probabilities
-            auto probabilities = [&](float ref) {
-                tmem_ld_wait();
-                uint64_t add[G::GROUPS];
-#pragma unroll
-                for (int k = 0; k < G::GROUPS; k++) {
-                    const float ks = row_scale * g[k].ks, base = g[k].lr - fmaf(zero_scale, g[k].kzs, ref);
-                    const uint64_t ks2 = pair(ks, ks), base2 = pair(base, base);
-                    float2 y[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int c = 16 * k + 2 * i;
-                        y[i] = unpair(fma2(pair(__uint_as_float(x[c / 32][c % 32]), __uint_as_float(x[c / 32][c % 32 + 1])), ks2, base2));
-                    }
-                    if (masked) {
-                        const int see = bad >> k & 1 ? -1 : pos - key0 - 16 * k;   // the last key of these that the row sees
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            if (2 * i > see) y[i].x = -INFINITY;
-                            if (2 * i + 1 > see) y[i].y = -INFINITY;
-                        }
-                    }
-                    add[k] = 0;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        y[i].x = ex2(y[i].x);
-                        y[i].y = ex2(y[i].y);
-                        add[k] = i == 0 ? pair(y[i].x, y[i].y) : add2(add[k], pair(y[i].x, y[i].y));
-                        p[8 * k + i] = h2pack(y[i].x, y[i].y);
-                    }
-                }
-                sum = 0.f;
-#pragma unroll
-                for (int k = 0; k < G::GROUPS; k++) {
-                    const float2 s2 = unpair(add[k]);
-                    sum = fmaf(s2.x + s2.y, g[k].inv, sum);
-                }
-            };
-            probabilities(m);   // (with m at -inf everything visible is inf, and so is the sum)
-            if (__any_sync(0xFFFFFFFFu, sum > TC_MAX_SUM)) {
-                load_scores();
-                tmem_ld_wait();
-                float best = -INFINITY;
-#pragma unroll
-                for (int k = 0; k < G::GROUPS; k++) {
-                    const float ks = row_scale * g[k].ks, base = -zero_scale * g[k].kzs;
-                    const int see = bad >> k & 1 ? -1 : pos - key0 - 16 * k;
+            // P of the first n times 32 keys, times a power of two
+            auto scale_p = [&](int n, float by) {
+                tmem_st_wait();
+#pragma unroll 1
+                for (int c = 0; c < n; c++) {
+                    uint32_t w[16];
+                    tmem_ld16(s_addr + 16 * c, w);
+                    tmem_ld_wait();
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const int c = 16 * k + i;
-                        best = i > see ? best : fmaxf(best, fmaf(__uint_as_float(x[c / 32][c % 32]), ks, base));
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                        w[i] = h2pack(f.x * by, f.y * by);
                     }
+                    tmem_st16(s_addr + 16 * c, w);
                 }
-                const float mx = fmaxf(m, best), down = m == mx ? 1.f : ex2(m - mx);
-                m = mx;
-                l *= down;
-                alpha *= down;
-                probabilities(m == -INFINITY ? 0.f : m);
+            };
+#pragma unroll 1
+            for (int c = 0; c < G::KEYS / 32; c++) {   // 32 keys at a time; P takes the place of scores that are in registers already
+                uint32_t p[16];
+                GroupPar g[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++) g[k] = par.g[2 * c + k];
+                int see[2];   // the last key of a group that the row sees
+#pragma unroll
+                for (int k = 0; k < 2; k++) see[k] = bad >> (2 * c + k) & 1 ? -1 : pos - key0 - 32 * c - 16 * k;
+                float ref = m, sum;
+                for (bool again = false;; again = true) {
+                    uint32_t x[32];   // (read again where they are needed again: that leaves more registers to the common way)
+                    tmem_ld32(s_addr + 32 * c, x);
+                    sum = 0.f;
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const float ks = row_scale * g[k].ks, base = g[k].lr - fmaf(zero_scale, g[k].kzs, ref);
+                        const uint64_t ks2 = pair(ks, ks), base2 = pair(base, base);
+                        float2 y[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            y[i] = unpair(fma2(pair(__uint_as_float(x[16 * k + 2 * i]), __uint_as_float(x[16 * k + 2 * i + 1])), ks2, base2));
+                        if (masked) {
+#pragma unroll
+                            for (int i = 0; i < 8; i++) {
+                                if (2 * i > see[k]) y[i].x = -INFINITY;
+                                if (2 * i + 1 > see[k]) y[i].y = -INFINITY;
+                            }
+                        }
+                        uint64_t add[2];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            y[i].x = ex2(y[i].x);
+                            y[i].y = ex2(y[i].y);
+                            add[i & 1] = i < 2 ? pair(y[i].x, y[i].y) : add2(add[i & 1], pair(y[i].x, y[i].y));
+                            p[8 * k + i] = h2pack(y[i].x, y[i].y);
+                        }
+                        const float2 s2 = unpair(add2(add[0], add[1]));
+                        sum = fmaf(s2.x + s2.y, g[k].inv, sum);
+                    }
+                    // (with m at -inf everything visible is inf, and so is the sum)
+                    if (again || !__any_sync(0xFFFFFFFFu, sum > TC_MAX_SUM)) break;
+                    float best = -INFINITY;
+                    tmem_ld32(s_addr + 32 * c, x);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        const float y = fmaf(__uint_as_float(x[i]), row_scale * g[i / 16].ks, -zero_scale * g[i / 16].kzs);
+                        best = i % 16 > see[i / 16] ? best : fmaxf(best, y);
+                    }
+                    const float mx = fmaxf(m, ceilf(best)), down = m == mx ? 1.f : ex2(m - mx);
+                    m = mx;
+                    l *= down;
+                    if (c > 0) scale_p(c, down);
+                    ref = m == -INFINITY ? 0.f : m;
+                }
+                l += sum;
+                tmem_st16(s_addr + 16 * c, p);
             }
-            l += sum;
+            // The tile in front has its reference by now: the larger one holds for both.
+            float alpha = par.rescale;
+            if (j > 0) {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(m_other, ((j - 1) / SB) & 1, abort_flag, status, 0xB40u | sb));
+                if (!ok) break;
+                const float before = s_m[(wg ^ 1) * TC_ROWS + r], mx = fmaxf(m, before);
+                if (__any_sync(0xFFFFFFFFu, m < before)) {
+                    const float down = m == mx ? 1.f : ex2(m - mx);
+                    l *= down;
+                    scale_p(G::KEYS / 32, down);
+                }
+                if (before != mx) alpha *= ex2(before - mx);
+                m = mx;
+            }
+            s_m[wg * TC_ROWS + r] = m;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(m_bar);
             if (j > 0 && __any_sync(0xFFFFFFFFu, alpha != 1.f)) {
-                // O so far times alpha: once the MMA that last added to it is done
-                const uint32_t pj = j - 1;
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(pv_bar + 8 * (pj % SB), (pj / SB) & 1, abort_flag, status, 0xB10u | (pj % SB)));
+                // O so far times alpha: once the MMA that last added to it is done (S of the tile in front is, so the one before that was)
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(pv_bar + 8 * (sb ^ 1), ((j - 1) / SB) & 1, abort_flag, status, 0xB10u | sb));
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll 1
@@ -419,23 +465,36 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                     tmem_st16(o_addr + d, o);
                 }
             }
-            tmem_st32(s_addr, p);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_bar + 8 * sb);
+            if (lane == 0) mbar_arrive(p_bar);
         }
+        // The last tile's reference holds for all.
+        float v_ref = 1.f;
         if (ok && mine > 0) {
-            const uint32_t pj = mine - 1;
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(pv_bar + 8 * (pj % SB), (pj / SB) & 1, abort_flag, status, 0xB20u | (pj % SB)));
+            const uint32_t last = mine - 1, lb = last % SB, ph = (last / SB) & 1;
+            if (lb != sb) {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(m_other, ph, abort_flag, status, 0xB20u | sb));
+                const float mx = s_m[(wg ^ 1) * TC_ROWS + r];
+                if (m != mx) l *= ex2(m - mx);
+                m = mx;
+            }
+            ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(pv_bar + 8 * lb, ph, abort_flag, status, 0xB28u | sb));
             tc_fence_after();
+            v_ref = s_par[last & 7].v_ref;
         }
+        meet();
+        s_m[wg * TC_ROWS + r] = l;
+        meet();
+        l += s_m[(wg ^ 1) * TC_ROWS + r];
+        // this warpgroup's half of the head dimensions
         if (ok && a.splits > 1) {
             const uint64_t at = (uint64_t)(place + split) * (TC_ROWS * RT) + rt * TC_ROWS + r;
-            if (real) a.part_ml[at] = make_float2(m, l);
+            if (real && sb == 0) a.part_ml[at] = make_float2(m, l);
             float4 *dst = reinterpret_cast<float4 *>(a.part_o + at * D);
 #pragma unroll 1
-            for (int d = 0; d < D; d += 16) {
+            for (int d = sb * (D / 2); d < (int)(sb + 1) * (D / 2); d += 16) {
                 uint32_t o[16];
                 if (mine > 0) {
                     tmem_ld16(o_addr + d, o);
@@ -452,67 +511,173 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             const float inv = l == 0.f ? 0.f : __fdiv_rn(v_ref, l);   // a row that sees nothing: zeros
             uint16_t *dst = static_cast<uint16_t *>(a.out) + (((uint64_t)s.off + t) * a.q_heads + h * a.group + (row - t * a.group)) * D;
 #pragma unroll 1
-            for (int d = 0; d < D; d += 32) {
-                uint32_t o[32];
+            for (int d = sb * (D / 2); d < (int)(sb + 1) * (D / 2); d += 16) {
+                uint32_t o[16];
                 if (mine > 0) {
-                    tmem_ld32(o_addr + d, o);
+                    tmem_ld16(o_addr + d, o);
                     tmem_ld_wait();
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; i++) o[i] = 0;
+                    for (int i = 0; i < 16; i++) o[i] = 0;
                 }
-                uint32_t w[16];
+                uint32_t w[8];
 #pragma unroll
-                for (int i = 0; i < 16; i++) w[i] = token_bits2<DT>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+                for (int i = 0; i < 8; i++) w[i] = token_bits2<DT>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
                 if (real) {
                     if (a.out_vec8) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) reinterpret_cast<uint4 *>(dst + d)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                        for (int i = 0; i < 2; i++) reinterpret_cast<uint4 *>(dst + d)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) dst[d + i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+                        for (int i = 0; i < 16; i++) dst[d + i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
                     }
                 }
             }
         }
-    } else if (wg < RT + 2) {
+    } else if (wg < G::SW + 2) {
         // ---------------- conversion ----------------
         if constexpr (G::REGS_CONVERT < G::REGS) regs_down<G::REGS_CONVERT>();
         const int tid = threadIdx.x & 127;
-        const int32_t *table = a.bt.table + (uint64_t)b * a.bt.table_width;
-        const uint32_t in_block = (1u << a.bt.log2_bt) - 1, parts = G::PARTS * tiles;
-        const uint32_t begin = tile0 * G::KEYS, end = (tile0 + tiles) * G::KEYS, last_key = end < (uint32_t)s.len ? end - 1 : (uint32_t)s.len - 1;
-        // the block that holds a key; keys behind the sequence's last read its block (masked later)
-        auto page_of = [&](uint32_t key) { return __ldg(table + ((key < last_key ? key : last_key) >> a.bt.log2_bt)); };
-        auto slot_of = [&](int32_t page) { return (uint64_t)((uint32_t)page < a.cache.blocks ? (uint32_t)page : 0u) * a.cache.kv_heads + h; };
-        if (wg == RT) {
-            // K: 16-byte pieces; lanes 0..7 of a group take eight keys, so that their stores meet eight different banks
+        auto take = [&](uint32_t hf) {   // part hf of the codes is there
+            return __all_sync(0xFFFFFFFFu, mbar_wait(raw_full + 8 * (hf % G::RAW), hf / G::RAW & 1, abort_flag, status, 0xB50u | hf % G::RAW));
+        };
+        auto give = [&](uint32_t hf) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(raw_empty + 8 * (hf % G::RAW));
+        };
+        if (wg == G::SW) {
+            // K: 16-byte pieces, those of a row to neighbouring lanes; odd groups of four write their second half first (other banks)
             constexpr int KC = D / 16, PER = G::PART * KC / 128;
             static_assert(PER * 128 == G::PART * KC, "pieces");
-            auto key_of = [&](int i) { return (uint32_t)(((i * 128 + tid) & 7) | ((i * 128 + tid) / (8 * KC)) << 3); };
-            auto piece_of = [&](int i) { return (uint32_t)((i * 128 + tid) / 8 % KC); };
-            int32_t page[PER];
-            auto pages = [&](uint32_t hf) {
+#pragma unroll 1
+            for (uint32_t hf = 0; hf < parts; hf++) {
+                const uint32_t j = hf / G::PARTS, st = j & 1;
+                if (!take(hf)) break;
+                if (hf % G::PARTS == 0 && j >= 2 &&
+                    !__all_sync(0xFFFFFFFFu, mbar_wait(k_empty + 8 * st, ((j - 2) >> 1) & 1, abort_flag, status, 0xB30u | st))) break;
+                const uint4 *src = reinterpret_cast<const uint4 *>(codes + hf % G::RAW * G::RAW_BYTES) + tid;
+                uint4 w[PER];
 #pragma unroll
-                for (int i = 0; i < PER; i++) page[i] = page_of(begin + hf * G::PART + key_of(i));
-            };
-            auto load = [&](uint4 (&c)[PER], uint32_t hf) {
+                for (int i = 0; i < PER; i++) w[i] = src[i * 128];
 #pragma unroll
                 for (int i = 0; i < PER; i++) {
-                    const uint32_t key = begin + hf * G::PART + key_of(i);
-                    c[i] = __ldg(reinterpret_cast<const uint4 *>(a.cache.k_dev + ((slot_of(page[i]) << a.bt.log2_bt) + (key & in_block)) * D + piece_of(i) * 16));
+                    const uint32_t u = (uint32_t)(i * 128 + tid) / KC, ch = (uint32_t)(i * 128 + tid) % KC, key = hf % G::PARTS * G::PART + u;
+                    const bool second = ch & 4;
+                    const uint32_t w0 = second ? w[i].z : w[i].x, w1 = second ? w[i].w : w[i].y, w2 = second ? w[i].x : w[i].z, w3 = second ? w[i].y : w[i].w;
+                    const uint32_t at = sk + st * G::K_BYTES + (ch / 4) * (G::KEYS * 128) + key * 128, c0 = ((ch & 3) * 2 + second) ^ (key & 7);
+                    sts16(at + (c0 << 4), __byte_perm(w0, 0, 0x4140), __byte_perm(w0, 0, 0x4342), __byte_perm(w1, 0, 0x4140), __byte_perm(w1, 0, 0x4342));
+                    sts16(at + ((c0 ^ 1) << 4), __byte_perm(w2, 0, 0x4140), __byte_perm(w2, 0, 0x4342), __byte_perm(w3, 0, 0x4140), __byte_perm(w3, 0, 0x4342));
                 }
-            };
-            // first warp: lane i % GROUPS looks after a tile's group i
-            int32_t g_page = 0;
+                give(hf);
+                if (hf % G::PARTS == G::PARTS - 1) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    mbar_arrive(k_full + 8 * st);
+                }
+            }
+        } else {
+            // V: units of 8 keys x 8 head dimensions; neighbouring lanes take neighbouring groups of keys
+            constexpr int KG = G::PART / 8, UNITS = KG * (D / 8);
+            static_assert(UNITS <= 128, "units");
+            const bool busy = UNITS == 128 || tid < UNITS;
+            const uint32_t kg = (uint32_t)tid % KG, d0 = (uint32_t)tid / KG * 8;
+            const uint32_t magic = 0x64646464u;
+#pragma unroll 1
+            for (uint32_t hf = 0; hf < parts; hf++) {
+                const uint32_t j = hf / G::PARTS, st = j & 1;
+                if (!take(hf)) break;
+                if (hf % G::PARTS == 0 && j >= 2 &&
+                    !__all_sync(0xFFFFFFFFu, mbar_wait(v_empty + 8 * st, ((j - 2) >> 1) & 1, abort_flag, status, 0xB48u | st))) break;
+                if (busy) {
+                    const uint8_t *src = codes + hf % G::RAW * G::RAW_BYTES + G::PART * D + kg * G::V_GROUP + d0;
+                    uint2 c[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) c[k] = *reinterpret_cast<const uint2 *>(src + k * D);
+                    const uint32_t z = 0x64006400u + s_zero[hf % G::RAW][kg / 2] * 0x10001u;
+                    const uint32_t chunk = (hf % G::PARTS * G::PART + kg * 8) / 8, at = sv + st * G::V_BYTES;
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {   // head dimensions d0 + 4 * half + 0..3
+                        uint32_t lo[4], hi[4];                 // key pairs 2k, 2k+1: {d, d+1} and {d+2, d+3} interleaved
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const uint32_t u = half ? c[2 * k].y : c[2 * k].x, v = half ? c[2 * k + 1].y : c[2 * k + 1].x;
+                            lo[k] = __byte_perm(u, v, 0x5140);
+                            hi[k] = __byte_perm(u, v, 0x7362);
+                        }
+#pragma unroll
+                        for (int d = 0; d < 4; d++) {
+                            uint32_t x[4];
+#pragma unroll
+                            for (int k = 0; k < 4; k++) x[k] = h2sub(__byte_perm(d < 2 ? lo[k] : hi[k], magic, d & 1 ? 0x4342 : 0x4140), z);
+                            const uint32_t dd = d0 + 4 * half + d;
+                            sts16(at + dd * 128 + ((chunk ^ (dd & 7)) << 4), x[0], x[1], x[2], x[3]);
+                        }
+                    }
+                }
+                give(hf);
+                if (hf % G::PARTS == G::PARTS - 1) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    mbar_arrive(v_full + 8 * st);
+                }
+            }
+        }
+    } else {
+        // ---------------- MMA issue: a warp per row tile runs the loop, one elected lane issues ----------------
+        regs_down<G::REGS_MMA>();
+        constexpr uint32_t id_qk = idesc_f16(TC_ROWS, G::KEYS), id_pv = idesc_f16(TC_ROWS, D);
+        const uint32_t rt = (uint32_t)warp & 3;
+        if (rt == 2) {
+            // The codes: a lane copies a block's share of K in the part (at most four), lane 8 + g eight keys of V.
+            const uint32_t piece = G::PART <= in_block ? (uint32_t)G::PART : in_block + 1;   // keys of K per copy
+            const bool k_lane = lane < G::PART / piece, v_lane = lane >= 8 && lane < 8 + G::PART / 8;
+            const uint32_t first = k_lane ? lane * piece : (v_lane ? (lane - 8) * 8 : 0u);
+            auto page_at = [&](uint32_t hf) { return page_of(begin + hf * G::PART + first); };
+            auto zero_at = [&](int32_t page) { return (uint32_t)a.cache.v_qp_dev[slot_of(page)].zero_point; };
+            int32_t page = 0, next = 0;
+            uint32_t zero = 0, hf = 0;
+            if (parts > 0) {
+                page = page_at(0);
+                zero = zero_at(page);
+            }
+            if (parts > 1) next = page_at(1);
+            for (; hf < parts; hf++) {
+                const uint32_t st = hf % G::RAW, bar = raw_full + 8 * st;
+                if (!__all_sync(0xFFFFFFFFu, hf < (uint32_t)G::RAW || mbar_wait(raw_empty + 8 * st, (hf / G::RAW - 1) & 1, abort_flag, status, 0xB58u | st))) break;
+                if (v_lane && lane % 2 == 0) s_zero[st][(lane - 8) / 2] = zero;
+                __syncwarp();
+                if (lane == 0) mbar_expect_tx(bar, G::PART * D * 2);
+                __syncwarp();
+                const uint64_t at = ((slot_of(page) << a.bt.log2_bt) + ((begin + hf * G::PART + first) & in_block)) * D;
+                const uint32_t dst = smem_u32(codes) + st * G::RAW_BYTES;
+                if (k_lane) bulk_load_1d(dst + first * D, a.cache.k_dev + at, piece * D, bar);
+                if (v_lane) bulk_load_1d(dst + G::PART * D + (lane - 8) * G::V_GROUP, a.cache.v_dev + at, 8 * D, bar);
+                page = next;
+                if (hf + 1 < parts) zero = zero_at(page);
+                if (hf + 2 < parts) next = page_at(hf + 2);
+            }
+            // given up: the copies still under way have to land before the block ends (a second, bounded wait)
+            if (hf < parts)
+                for (uint32_t i = hf > (uint32_t)G::RAW ? hf - G::RAW : 0u; i < hf; i++)
+                    mbar_wait(raw_full + 8 * (i % G::RAW), i / G::RAW & 1, s_misc + 2, status, 0xB5Cu);
+        } else if (rt == 3) {
+            // what the softmax needs of every tile: lane i % GROUPS looks after its group i
             float v_ref = TC_SMALLEST;
-            if (warp % 4 == 0 && tiles > 0) g_page = page_of(begin + (lane % G::GROUPS) * 16);
-            auto params = [&](uint32_t j) {   // of tile j, in the place of tile j - 8: S of tile j - 3 is done, so P of tile j - 5 was
-                const uint64_t slot = slot_of(g_page);
-                const bool bad = (uint32_t)g_page >= a.cache.blocks;
-                const ltq_qparams kq = a.cache.k_qp_dev[slot];
-                const float vs = a.cache.v_qp_dev[slot].scale;
-                if (j + 1 < tiles) g_page = page_of(begin + (j + 1) * G::KEYS + (lane % G::GROUPS) * 16);
+            auto page_at = [&](uint32_t j) { return page_of(begin + j * G::KEYS + (lane % G::GROUPS) * 16); };
+            int32_t page = tiles > 0 ? page_at(0) : 0;
+            ltq_qparams kq{};
+            float vs = 0.f;
+            bool bad = false;
+            auto fetch = [&]() {   // of the tile whose page is here
+                const uint64_t slot = slot_of(page);
+                bad = (uint32_t)page >= a.cache.blocks;
+                kq = a.cache.k_qp_dev[slot];
+                vs = a.cache.v_qp_dev[slot].scale;
+            };
+            if (tiles > 0) fetch();
+            if (tiles > 1) page = page_at(1);
+            for (uint32_t j = 0; j < tiles; j++) {
+                // in the place of tile j - 8: S of tile j - 2 is done, so P of tile j - 4 was
+                const uint32_t st = j & 1;
+                if (!__all_sync(0xFFFFFFFFu, j < 2 || mbar_wait(k_empty + 8 * st, ((j - 2) >> 1) & 1, abort_flag, status, 0xB38u | st))) break;
                 if (bad && lane < G::GROUPS) atomicCAS(status, 0u, STATUS_BAD_BLOCK);
                 float top = vs;   // (NaN is passed over)
 #pragma unroll
@@ -534,112 +699,12 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                     p.rescale = rescale;
                     p.bad = any;
                 }
-            };
-            auto convert = [&](uint32_t hf, uint4 (&cur)[PER], uint4 (&nxt)[PER]) -> bool {
-                const uint32_t j = hf / G::PARTS, st = j & 1;
-                if (hf + 1 < parts) load(nxt, hf + 1);
-                if (hf + 2 < parts) pages(hf + 2);
-                if (hf % G::PARTS == 0) {
-                    if (warp % 4 == 0) params(j);
-                    if (j >= 2 && !mbar_wait(k_empty + 8 * st, ((j - 2) >> 1) & 1, abort_flag, status, 0xB30u | st)) return false;
-                }
-#pragma unroll
-                for (int i = 0; i < PER; i++) {
-                    const uint32_t key = hf % G::PARTS * G::PART + key_of(i), ch = piece_of(i), w[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
-                    uint32_t x[8];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        x[2 * k] = __byte_perm(w[k], 0, 0x4140);
-                        x[2 * k + 1] = __byte_perm(w[k], 0, 0x4342);
-                    }
-                    const uint32_t at = sk + st * G::K_BYTES + (ch / 4) * (G::KEYS * 128) + key * 128, c0 = (ch & 3) * 2;
-                    sts16(at + ((c0 ^ (key & 7)) << 4), x[0], x[1], x[2], x[3]);
-                    sts16(at + (((c0 + 1) ^ (key & 7)) << 4), x[4], x[5], x[6], x[7]);
-                }
-                if (hf % G::PARTS == G::PARTS - 1) {
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    mbar_arrive(k_full + 8 * st);
-                }
-                return true;
-            };
-            uint4 even[PER], odd[PER];
-            if (tiles > 0) {
-                pages(0);
-                load(even, 0);
-                pages(1);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(k_full + 8 * st);
+                if (j + 1 < tiles) fetch();
+                if (j + 2 < tiles) page = page_at(j + 2);
             }
-            for (uint32_t hf = 0; hf < parts; hf += 2)
-                if (!convert(hf, even, odd) || hf + 1 >= parts || !convert(hf + 1, odd, even)) break;
-        } else {
-            // V: units of 8 keys x 8 head dimensions; neighbouring lanes take neighbouring groups of keys, for the banks again
-            constexpr int KG = G::PART / 8, UNITS = KG * (D / 8), PER = (UNITS + 127) / 128;
-            static_assert(PER == 1, "units");
-            const bool busy = UNITS == 128 || tid < UNITS;
-            const uint32_t kg = (uint32_t)tid % KG, d0 = (uint32_t)tid / KG * 8;
-            int32_t page = 0;
-            struct Codes {
-                uint2 c[8];
-                uint32_t z;
-            };
-            auto load = [&](Codes &c, uint32_t hf) {
-                if (!busy) return;
-                const uint64_t slot = slot_of(page);
-                const uint32_t key = begin + hf * G::PART + kg * 8;
-                const uint8_t *p = a.cache.v_dev + ((slot << a.bt.log2_bt) + (key & in_block)) * D + d0;
-#pragma unroll
-                for (int k = 0; k < 8; k++) c.c[k] = __ldg(reinterpret_cast<const uint2 *>(p + k * D));
-                c.z = __ldg(&a.cache.v_qp_dev[slot].zero_point);
-            };
-            const uint32_t magic = 0x64646464u;
-            auto convert = [&](uint32_t hf, Codes &cur, Codes &nxt) -> bool {
-                const uint32_t j = hf / G::PARTS, st = j & 1;
-                if (hf + 1 < parts) load(nxt, hf + 1);
-                if (hf + 2 < parts) page = page_of(begin + (hf + 2) * G::PART + kg * 8);
-                if (hf % G::PARTS == 0 && j >= 2 && !mbar_wait(v_empty + 8 * st, ((j - 2) >> 1) & 1, abort_flag, status, 0xB40u | st)) return false;
-                if (busy) {
-                    const uint32_t z = 0x64006400u + cur.z * 0x10001u;
-                    const uint32_t key = hf % G::PARTS * G::PART + kg * 8, chunk = key / 8;
-                        const uint32_t at = sv + st * G::V_BYTES;
-#pragma unroll
-                    for (int half = 0; half < 2; half++) {   // head dimensions d0 + 4 * half + 0..3
-                        uint32_t lo[4], hi[4];                 // key pairs 2k, 2k+1: {d, d+1} and {d+2, d+3} interleaved
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const uint32_t u = half ? cur.c[2 * k].y : cur.c[2 * k].x, v = half ? cur.c[2 * k + 1].y : cur.c[2 * k + 1].x;
-                            lo[k] = __byte_perm(u, v, 0x5140);
-                            hi[k] = __byte_perm(u, v, 0x7362);
-                        }
-#pragma unroll
-                        for (int d = 0; d < 4; d++) {
-                            uint32_t x[4];
-#pragma unroll
-                            for (int k = 0; k < 4; k++) x[k] = h2sub(__byte_perm(d < 2 ? lo[k] : hi[k], magic, d & 1 ? 0x4342 : 0x4140), z);
-                            const uint32_t dd = d0 + 4 * half + d;
-                            sts16(at + dd * 128 + ((chunk ^ (dd & 7)) << 4), x[0], x[1], x[2], x[3]);
-                        }
-                    }
-                }
-                if (hf % G::PARTS == G::PARTS - 1) {
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    mbar_arrive(v_full + 8 * st);
-                }
-                return true;
-            };
-            Codes even, odd;
-            if (tiles > 0) {
-                page = page_of(begin + kg * 8);
-                load(even, 0);
-                page = page_of(begin + G::PART + kg * 8);
-            }
-            for (uint32_t hf = 0; hf < parts; hf += 2)
-                if (!convert(hf, even, odd) || hf + 1 >= parts || !convert(hf + 1, odd, even)) break;
-        }
-    } else {
-        // ---------------- MMA issue: a warp per row tile runs the loop, one elected lane issues ----------------
-        regs_down<G::REGS_MMA>();
-        constexpr uint32_t id_qk = idesc_f16(TC_ROWS, G::KEYS), id_pv = idesc_f16(TC_ROWS, D);
-        const uint32_t rt = (uint32_t)warp & 3;
-        if (rt < RT) {
+        } else if (rt < RT) {
             const uint32_t mine = rt ? tiles1 : tiles0;
             const uint32_t s_bar = s_full + 8 * SB * rt, p_bar = p_full + 8 * SB * rt, pv_bar = pv_done + 8 * SB * rt;
             auto wait = [&](uint32_t bar, uint32_t phase, uint32_t code) {
