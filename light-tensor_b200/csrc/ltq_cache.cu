@@ -250,6 +250,7 @@ AttnPlan attn_plan(const ltq_kv_cache *c, int dtype, uint32_t q_heads, uint64_t 
         const double tc = 6 + (double)waves * (8 + 1.15 * (double)(keys / 64) / t.splits) + (t.splits > 1 ? 5 : 0);
         if (tc < other && tiles <= 65535) {
             t.row_tiles = (uint32_t)tiles;
+            t.ctas = (uint32_t)sms;
             t.items = heads * tiles;
             if (t.splits > 1) {
                 t.ml = t.items * t.splits * t.rows_per_tile;

@@ -200,7 +200,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
     float *s_m = reinterpret_cast<float *>(after + 8 * sizeof(TilePar));   // [row tile][S buffer][row]: the reference maximum
     uint64_t *bars = reinterpret_cast<uint64_t *>(s_m + G::SW * TC_ROWS);
     uint32_t(*s_zero)[4] = reinterpret_cast<uint32_t(*)[4]>(bars + G::BARS + G::BARS % 2);   // zero points of a part's V, per 16 keys
-    uint32_t *s_misc = reinterpret_cast<uint32_t *>(s_zero + G::RAW);   // [0] tmem base, [1] abort flag, [2] stays 0
+    uint32_t *s_misc = reinterpret_cast<uint32_t *>(s_zero + G::RAW);   // [0] tmem base, [1] abort flag, [2] another one, [3] the group
     volatile uint32_t *abort_flag = s_misc + 1;
     const uint32_t k_full = smem_u32(bars), k_empty = k_full + 16, v_full = k_full + 32, v_empty = k_full + 48, q_full = k_full + 64;
     const uint32_t s_full = k_full + 72, p_full = s_full + 8 * SB * RT, pv_done = p_full + 8 * SB * RT,   // [row tile][S buffer]
@@ -242,17 +242,41 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
     griddep_wait();
     const uint32_t tmem = s_misc[0];
 
-    const uint32_t split = blockIdx.x / a.cache.kv_heads, h = blockIdx.x - split * a.cache.kv_heads, b = blockIdx.y;
-    const uint32_t group = gridDim.z - 1 - blockIdx.z, row0 = group * (TC_ROWS * RT);
+    auto tiles_to = [&](const CacheSeq &s, uint32_t row) -> uint32_t {   // key tiles that a sequence's rows up to this one see
+        const int keys = s.len - s.n + (int)(row / a.group) + 1;
+        return keys > 0 ? ((uint32_t)keys + G::KEYS - 1) / G::KEYS : 0u;
+    };
+    // This CTA's group of row tiles.  Where there is more than the device takes at once the groups go by the tiles they see, most first
+    // (2 x 1500 new tokens behind up to 4500: 270 us in the grid's order, the last groups first, LPT us by tiles).
+    const uint32_t split = blockIdx.x / a.cache.kv_heads, h = blockIdx.x - split * a.cache.kv_heads, pairs = gridDim.y * gridDim.z;
+    uint32_t b = blockIdx.y, group = gridDim.z - 1 - blockIdx.z;
+    if (pairs * gridDim.x > a.ctas && pairs <= G::THREADS) {
+        uint32_t *s_weight = reinterpret_cast<uint32_t *>(smem_raw);   // (nothing else is there yet)
+        const uint32_t mine_b = threadIdx.x % gridDim.y, mine_group = threadIdx.x / gridDim.y;
+        uint32_t weight = 0;   // tiles, plus one for the group itself
+        if (threadIdx.x < pairs) {
+            const CacheSeq s = cache_seq(a.bt, mine_b);
+            const uint32_t rows = s.ok ? (uint32_t)s.n * a.group : 0u, first = mine_group * (TC_ROWS * RT);
+            if (first < rows) weight = 1 + tiles_to(s, (first + TC_ROWS * RT < rows ? first + TC_ROWS * RT : rows) - 1);
+        }
+        s_weight[threadIdx.x] = weight;
+        __syncthreads();
+        if (threadIdx.x < pairs) {
+            uint32_t rank = 0;
+            for (uint32_t i = 0; i < pairs; i++) rank += s_weight[i] > weight || (s_weight[i] == weight && i < threadIdx.x);
+            if (rank == blockIdx.y + blockIdx.z * gridDim.y) s_misc[3] = threadIdx.x;
+        }
+        __syncthreads();
+        b = s_misc[3] % gridDim.y;
+        group = s_misc[3] / gridDim.y;
+    }
+    const uint32_t row0 = group * (TC_ROWS * RT);
     const CacheSeq s = cache_seq(a.bt, b);
     if (!s.ok && threadIdx.x == 0) atomicCAS(status, 0u, STATUS_BAD_SEQUENCE);
     const uint32_t rows = s.ok ? (uint32_t)s.n * a.group : 0u;
     auto tiles_of = [&](uint32_t rt) -> uint32_t {   // key tiles that row tile rt sees
         const uint32_t first = row0 + rt * TC_ROWS;
-        if (first >= rows) return 0u;
-        const uint32_t last = first + TC_ROWS < rows ? first + TC_ROWS - 1 : rows - 1;
-        const int keys = s.len - s.n + (int)(last / a.group) + 1;
-        return keys > 0 ? ((uint32_t)keys + G::KEYS - 1) / G::KEYS : 0u;
+        return first >= rows ? 0u : tiles_to(s, (first + TC_ROWS < rows ? first + TC_ROWS : rows) - 1);
     };
     const uint32_t all0 = tiles_of(0), all1 = RT == 2 ? tiles_of(RT - 1) : 0u, all = all0 > all1 ? all0 : all1;
     // this CTA's tiles: [tile0, tile0 + tiles), of which the row tiles see the first tiles0 and tiles1
@@ -303,21 +327,17 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             }
 #pragma unroll
             for (int i = 0; i < PASSES; i++) {
-                float most = 0.f;   // infinity for a row with anything that is not finite
+                // the largest magnitude, by its bits: both types' order like integers
+                uint32_t top = 0;
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const float v = fabsf(elem<DT>(qw[i][k / 2], k & 1));
-                    most = v < INFINITY ? fmaxf(most, v) : INFINITY;
-                }
+                for (int k = 0; k < 4; k++) top = __vmaxu2(top, qw[i][k] & 0x7FFF7FFFu);
 #pragma unroll
-                for (int o = 1; o < LANES; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
-                const bool finite = most < INFINITY;
-                int e = 0;   // most * 2^e in [2^10, 2^11)
-                if (most > 0.f && finite) {
-                    e = 10 - ilogbf(most);
-                    e = e > 100 ? 100 : e;
-                }
-                const float f = ldexpf(1.f, e);
+                for (int o = 1; o < LANES; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+                top = top >> 16 > (top & 0xFFFFu) ? top >> 16 : top & 0xFFFFu;
+                const bool finite = top < (DT == LTQ_F16 ? 0x7C00u : 0x7F80u);
+                const int size = (int)(__float_as_uint(elem<DT>(top, 0)) >> 23) - 127;   // its exponent
+                const int e = size < -90 ? 100 : 10 - size;   // most * 2^e in [2^10, 2^11), where that is a float
+                const float f = __uint_as_float((uint32_t)(127 + e) << 23);
                 float q_sum = 0.f;
                 uint32_t w[4];
 #pragma unroll
@@ -331,7 +351,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                 const uint32_t qr = row_of(i);
                 if (has) sts16(sq + rt * G::Q_BYTES + (at / 8) * (TC_ROWS * 128) + qr * 128 + (((at & 7) ^ (qr & 7)) << 4), w[0], w[1], w[2], w[3]);
                 if (at == 0) {
-                    const float row_scale = finite ? a.scale_log2 * ldexpf(1.f, -e) : __int_as_float(0x7FC00000);
+                    const float row_scale = finite ? a.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23) : __int_as_float(0x7FC00000);
                     row_par[qr] = make_float2(row_scale, row_scale * q_sum);
                 }
             }
