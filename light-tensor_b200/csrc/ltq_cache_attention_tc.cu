@@ -66,7 +66,7 @@ struct TcGeo {
     // Registers per thread: as launched (896 or 640 threads), and after setmaxnreg, which may only raise with .inc, lower with .dec,
     // and hands out no more than the block was launched with.
     static constexpr int REGS = RT == 2 ? 72 : 96;
-    static constexpr int REGS_SOFTMAX = RT == 2 ? 88 : 136, REGS_CONVERT = RT == 2 ? 56 : 80, REGS_MMA = RT == 2 ? 40 : 48;
+    static constexpr int REGS_SOFTMAX = RT == 2 ? 88 : 136, REGS_CONVERT = RT == 2 ? 48 : 80, REGS_MMA = RT == 2 ? 56 : 48;
     static_assert(SW * REGS_SOFTMAX + 2 * REGS_CONVERT + REGS_MMA == (SW + 3) * REGS, "register shares");
     static_assert(REGS_SOFTMAX >= REGS && REGS_CONVERT <= REGS && REGS_MMA <= REGS, "register shares");
     static constexpr int BARS = 9 + RT * 3 * SB + SW * 4 + 2 * RAW;   // k_full k_empty v_full v_empty q_full; s_full p_full pv_done; m_done; raw_full raw_empty
@@ -161,6 +161,23 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
         "r"(idesc), "r"(accumulate)
         : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+        "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16])
 {
@@ -375,86 +392,61 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             tc_fence_after();
             const TilePar &par = s_par[j & 7];
             const int key0 = (int)((tile0 + j) * G::KEYS);
-            const uint32_t bad = par.bad;
-            const bool masked = bad || key0 + G::KEYS - 1 > first_pos;
-            // P of the first n times 32 keys, times a power of two
-            auto scale_p = [&](int n, float by) {
-                tmem_st_wait();
-#pragma unroll 1
-                for (int c = 0; c < n; c++) {
-                    uint32_t w[16];
-                    tmem_ld16(s_addr + 16 * c, w);
-                    tmem_ld_wait();
+            auto last_seen = [&](int k) { return par.bad >> k & 1 ? -1 : pos - key0 - 16 * k; };   // the last key of group k that the row sees
+            uint32_t p[G::KEYS / 2];
+            // The common way: everything is seen, and the reference stays.  Else the careful way, from the scores as they still are.
+            bool careful = par.bad || key0 + G::KEYS - 1 > first_pos;
+            if (!careful) {
+                float sum = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-                        w[i] = h2pack(f.x * by, f.y * by);
-                    }
-                    tmem_st16(s_addr + 16 * c, w);
-                }
-            };
-#pragma unroll 1
-            for (int c = 0; c < G::KEYS / 32; c++) {   // 32 keys at a time; P takes the place of scores that are in registers already
-                uint32_t p[16];
-                GroupPar g[2];
-#pragma unroll
-                for (int k = 0; k < 2; k++) g[k] = par.g[2 * c + k];
-                int see[2];   // the last key of a group that the row sees
-#pragma unroll
-                for (int k = 0; k < 2; k++) see[k] = bad >> (2 * c + k) & 1 ? -1 : pos - key0 - 32 * c - 16 * k;
-                float ref = m, sum;
-                for (bool again = false;; again = true) {
-                    uint32_t x[32];   // (read again where they are needed again: that leaves more registers to the common way)
+                for (int c = 0; c < G::KEYS / 32; c++) {   // 32 keys at a time
+                    uint32_t x[32];
                     tmem_ld32(s_addr + 32 * c, x);
-                    sum = 0.f;
+                    GroupPar g[2];
+#pragma unroll
+                    for (int k = 0; k < 2; k++) g[k] = par.g[2 * c + k];
                     tmem_ld_wait();
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
-                        const float ks = row_scale * g[k].ks, base = g[k].lr - fmaf(zero_scale, g[k].kzs, ref);
+                        const float ks = row_scale * g[k].ks, base = g[k].lr - fmaf(zero_scale, g[k].kzs, m);
                         const uint64_t ks2 = pair(ks, ks), base2 = pair(base, base);
                         float2 y[8];
 #pragma unroll
                         for (int i = 0; i < 8; i++)
                             y[i] = unpair(fma2(pair(__uint_as_float(x[16 * k + 2 * i]), __uint_as_float(x[16 * k + 2 * i + 1])), ks2, base2));
-                        if (masked) {
-#pragma unroll
-                            for (int i = 0; i < 8; i++) {
-                                if (2 * i > see[k]) y[i].x = -INFINITY;
-                                if (2 * i + 1 > see[k]) y[i].y = -INFINITY;
-                            }
-                        }
                         uint64_t add[2];
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             y[i].x = ex2(y[i].x);
                             y[i].y = ex2(y[i].y);
                             add[i & 1] = i < 2 ? pair(y[i].x, y[i].y) : add2(add[i & 1], pair(y[i].x, y[i].y));
-                            p[8 * k + i] = h2pack(y[i].x, y[i].y);
+                            p[16 * c + 8 * k + i] = h2pack(y[i].x, y[i].y);
                         }
                         const float2 s2 = unpair(add2(add[0], add[1]));
                         sum = fmaf(s2.x + s2.y, g[k].inv, sum);
                     }
-                    // (with m at -inf everything visible is inf, and so is the sum)
-                    if (again || !__any_sync(0xFFFFFFFFu, sum > TC_MAX_SUM)) break;
-                    float best = -INFINITY;
-                    tmem_ld32(s_addr + 32 * c, x);
+                }
+                careful = __any_sync(0xFFFFFFFFu, sum > TC_MAX_SUM);   // (with m at -inf everything is inf, and so is the sum)
+                if (!careful) l += sum;
+            }
+            if (careful) {   // the maximum first
+                float best = -INFINITY;
+#pragma unroll 1
+                for (int k = 0; k < G::GROUPS; k++) {
+                    uint32_t x[16];
+                    tmem_ld16(s_addr + 16 * k, x);
+                    const float ks = row_scale * par.g[k].ks, base = -zero_scale * par.g[k].kzs;
+                    const int see = last_seen(k);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        const float y = fmaf(__uint_as_float(x[i]), row_scale * g[i / 16].ks, -zero_scale * g[i / 16].kzs);
-                        best = i % 16 > see[i / 16] ? best : fmaxf(best, y);
-                    }
-                    const float mx = fmaxf(m, ceilf(best)), down = m == mx ? 1.f : ex2(m - mx);
-                    m = mx;
-                    l *= down;
-                    if (c > 0) scale_p(c, down);
-                    ref = m == -INFINITY ? 0.f : m;
+                    for (int i = 0; i < 16; i++) best = i > see ? best : fmaxf(best, fmaf(__uint_as_float(x[i]), ks, base));
                 }
-                l += sum;
-                tmem_st16(s_addr + 16 * c, p);
+                const float mx = fmaxf(m, ceilf(best));
+                if (m != mx) l *= ex2(m - mx);
+                m = mx;
             }
             // The tile in front has its reference by now: the larger one holds for both.
-            float alpha = par.rescale;
+            float alpha = 1.f;
             if (j > 0) {
                 ok = __all_sync(0xFFFFFFFFu, mbar_wait(m_other, ((j - 1) / SB) & 1, abort_flag, status, 0xB40u | sb));
                 if (!ok) break;
@@ -462,15 +454,19 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                 if (__any_sync(0xFFFFFFFFu, m < before)) {
                     const float down = m == mx ? 1.f : ex2(m - mx);
                     l *= down;
-                    scale_p(G::KEYS / 32, down);
+                    if (!careful) {
+                        const __half2 by = __float2half2_rn(down);   // a power of two
+#pragma unroll
+                        for (int i = 0; i < G::KEYS / 2; i++) *reinterpret_cast<__half2 *>(&p[i]) = __hmul2(*reinterpret_cast<__half2 *>(&p[i]), by);
+                    }
                 }
-                if (before != mx) alpha *= ex2(before - mx);
+                alpha = before != mx ? par.rescale * ex2(before - mx) : par.rescale;
                 m = mx;
             }
             s_m[wg * TC_ROWS + r] = m;
             __syncwarp();
             if (lane == 0) mbar_arrive(m_bar);
-            if (j > 0 && __any_sync(0xFFFFFFFFu, alpha != 1.f)) {
+            if (__any_sync(0xFFFFFFFFu, alpha != 1.f)) {
                 // O so far times alpha: once the MMA that last added to it is done (S of the tile in front is, so the one before that was)
                 ok = __all_sync(0xFFFFFFFFu, mbar_wait(pv_bar + 8 * (sb ^ 1), ((j - 1) / SB) & 1, abort_flag, status, 0xB10u | sb));
                 if (!ok) break;
@@ -483,6 +479,30 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
 #pragma unroll
                     for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
                     tmem_st16(o_addr + d, o);
+                }
+            }
+            if (!careful) {
+                tmem_st32(s_addr, p);
+            } else {
+                const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+                for (int k = 0; k < G::GROUPS; k++) {   // P takes the place of scores that are in registers already
+                    uint32_t x[16], w[8];
+                    tmem_ld16(s_addr + 16 * k, x);
+                    const GroupPar g = par.g[k];
+                    const float ks = row_scale * g.ks, base = g.lr - fmaf(zero_scale, g.kzs, ref);
+                    const int see = last_seen(k);
+                    float sum = 0.f;
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float y0 = 2 * i > see ? 0.f : ex2(fmaf(__uint_as_float(x[2 * i]), ks, base));
+                        const float y1 = 2 * i + 1 > see ? 0.f : ex2(fmaf(__uint_as_float(x[2 * i + 1]), ks, base));
+                        sum += y0 + y1;
+                        w[i] = h2pack(y0, y1);
+                    }
+                    l = fmaf(sum, g.inv, l);
+                    tmem_st8(s_addr + 8 * k, w);
                 }
             }
             tmem_st_wait();
