@@ -233,10 +233,11 @@ AttnPlan attn_plan(const ltq_kv_cache *c, int dtype, uint32_t q_heads, uint64_t 
     const uint64_t rows = max_new * (q_heads / c->kv_heads), keys = table_width * c->block_tokens;
     const uint64_t heads = seqs * c->kv_heads, steps = keys / 16;
     // The tensor-core form needs its 256 (128) rows filled to be worth it, the others read the keys once per 8 or 16 rows.
-    // Estimates in microseconds from a sweep over 1 to 64 sequences, 8 to 1536 rows, 300 and 4000 keys, head_dim 64, 128, 256:
-    //   the others    8 + 0.0008 per 16 keys of a row tile at head_dim 128       (64 x 8 heads, 96 rows, 4000 keys: 361 us)
-    //   tensor cores  6 + 8 per wave of CTAs + 1.15 per 64 keys (+ 5 for a join)  (the same: 259 us;
-    //                 1 x 8 heads, 512 rows: 300 keys 24 us against 15, 4000 keys 35 us against 70)
+    // Estimates in microseconds from a sweep over 1 to 64 sequences, 32 to 1024 rows, 300 to 4000 keys, head_dim 64, 128, 256:
+    //   the others    10 + per row tile and head 0.02 + (0.00025 + head_dim * 0.000004) per 16 keys
+    //   tensor cores  3 (6 with a join) + per wave of CTAs 11 + 1.05 (head_dim above 128: 1.7) per 64 keys
+    // (8 x 8 heads of 128, 96 rows: 300 keys 29 us against 19, 4000 keys 102 us against 44; 1 x 8 heads, 256 rows: 300 keys 15 us
+    // against 23, 4000 keys 46 us against 30).  Where it chose wrongly the other form was at most 28 % faster.
     if (dtype != LTQ_F32 && rows > 16) {
         AttnPlan t{};
         t.tc = true;
@@ -246,8 +247,8 @@ AttnPlan attn_plan(const ltq_kv_cache *c, int dtype, uint32_t q_heads, uint64_t 
         const uint64_t most = (keys + 64 * ATTN_TC_MIN_TILES - 1) / (64 * ATTN_TC_MIN_TILES), fit = (uint64_t)sms / (heads * tiles);
         t.splits = (uint32_t)(fit < 1 || most < 1 ? 1 : (most < fit ? most : fit));
         const uint32_t per = attn_rows_per_tile(dtype, c->head_dim, rows);
-        const double other = 8 + 0.0008 * (double)(heads * ((rows + per - 1) / per) * steps) * c->head_dim / 128;
-        const double tc = 6 + (double)waves * (8 + 1.15 * (double)(keys / 64) / t.splits) + (t.splits > 1 ? 5 : 0);
+        const double other = 10 + (double)(heads * ((rows + per - 1) / per)) * (0.02 + (0.00025 + 0.000004 * c->head_dim) * (double)steps);
+        const double tc = (t.splits > 1 ? 6 : 3) + (double)waves * (11 + (c->head_dim <= 128 ? 1.05 : 1.7) * (double)(keys / 64) / t.splits);
         if (tc < other && tiles <= 65535) {
             t.row_tiles = (uint32_t)tiles;
             t.ctas = (uint32_t)sms;

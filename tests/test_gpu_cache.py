@@ -231,10 +231,11 @@ def attention_want(torch, cache, q, b, scale):
             # (at most 2^-23 per addition), one more rounding each for the two scales and the subtraction of the maximum
             size = (qq.abs() @ k.abs().t()).masked_fill(~seen, 0).amax(2, keepdim=True) + qq.abs().amax(2, keepdim=True) * k.abs().sum(1).amax()
             ds = abs(scale) * size * (2.0 ** -22 + D * 2.0 ** -23 + 4 * 2.0 ** -24)
-            # probabilities: 2^-11 (half) or 2^-22 (two halves) relative, the exponential's 2^-22, and 2^-25 of the
-            # reference maximum's (at least 2^-8 of the largest one's inverse) for subnormal halves; sums in float
+            # probabilities: 2^-11 (half) or 2^-22 (two halves) relative, the exponential's 2^-22; sums in float.  Subnormal halves
+            # are off by 2^-25: in units of v's reference scale, at most twice the largest of the row's, times codes up to twice
+            # the largest value's, over a sum of at least 1/2 (the reference maximum is rounded up to an integer): 2^-22 per key
             keys = (pos[live] + 1)[:, None, None]
-            dp = 2 * ds + (2.0 ** -21 if fine else 2.0 ** -11) + 2.0 ** -21 + keys * 2.0 ** -23 + keys * 2.0 ** -24
+            dp = 2 * ds + (2.0 ** -21 if fine else 2.0 ** -11) + 2.0 ** -21 + keys * 2.0 ** -23 + keys * 2.0 ** -22
             largest = torch.cummax(v.abs(), 0).values[pos[live]][:, None]
             tol[rows, h * group:(h + 1) * group] = dp * largest + 1e-300
     return want, tol + eps / 2 * (want.abs() + tol)
@@ -248,7 +249,10 @@ CASES = [  # spans, block_tokens, head_dim, kv_heads, group
     ([(65, 90 + i) for i in range(40)], 16, 128, 2, 2), ([(40, 70 + 3 * i) for i in range(80)], 32, 256, 1, 2),
     ([(600, 700)], 16, 64, 2, 4), ([(700, 700), (0, 5)], 16, 32, 1, 24), ([(300, 305)], 128, 96, 2, 4),
     ([(128, 128)], 128, 96, 1, 2), ([(50, 900)], 64, 192, 2, 3), ([(300, 333)], 64, 256, 1, 1), ([(65, 1000), (0, 5)], 16, 32, 2, 3),
-    ([(1, 4100), (1, 4096), (1, 31)], 64, 128, 2, 16)]
+    ([(1, 4100), (1, 4096), (1, 31)], 64, 128, 2, 16),
+    # more groups of rows than the device takes at once: dealt out by what they see, and too many for that
+    ([(1 + 37 * i % 200, 60 + 211 * i % 700) for i in range(40)], 32, 64, 2, 4),
+    ([(300, 320)] + [(1 + i % 5, 20 + i) for i in range(299)], 16, 32, 1, 4)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -296,6 +300,36 @@ def test_attention_sharp_large_and_small_scores(cuda, dtype):
         assert torch.isfinite(got).all()
         inside = cache.values()[1].abs().max()
         assert (got.abs() <= inside * (1 + 2 ** -7)).all()
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_prompt_attention_sharp_scores_and_growing_scales(cuda, dtype, head_dim):
+    """The same for rows enough to fill the large tiles: the maximum and the largest v scale rise, or fall, from block to block."""
+    import ltq
+    torch = cuda
+    b = batch(torch, 15, [(260, 2300), (150, 900), (300, 300)], 16)
+    cache = random_cache(torch, ltq, 15, b["blocks"], 2, 16, head_dim)
+    for up_k, up_v in ((1.04, 1.06), (0.97, 0.96), (1.03, 0.97)):
+        for row in b["table"]:
+            for j, page in enumerate(row):
+                if page >= 0:
+                    cache.k_qparams.view(torch.float32)[page, :, 0] = 0.002 * up_k ** j
+                    cache.v_qparams.view(torch.float32)[page, :, 0] = 0.01 * up_v ** j
+        q = torch.randn(b["tokens"], 6, head_dim, generator=torch.Generator().manual_seed(head_dim))
+        q[:, 1] *= 30
+        q[:, 2] *= 3e-5
+        q[::7, 3] = 0
+        q = q.to(getattr(torch, dtype)).cuda()
+        args = (ints(torch, b["table"]), ints(torch, b["lengths"]), ints(torch, b["offsets"]), b["max_new"])
+        for scale in (head_dim ** -0.5, -0.3, 0.0):
+            got = cache.attention(q, *args, scale=scale)
+            want, tol = attention_want(torch, cache, q, b, float(np.float32(scale)))
+            largest = cache.values()[1].abs().max()
+            loose = tol > largest   # scores so large that their own rounding moves probabilities freely
+            assert not ((got.double() - want).abs() > tol)[~loose].any()
+            assert torch.isfinite(got).all() and (got.abs() <= largest * (1 + 2 ** -7)).all()
+            assert torch.equal(cache.attention(q, *args, scale=scale), got)
 
 
 def test_attention_ignores_what_it_may_not_see(cuda):
