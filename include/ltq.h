@@ -255,7 +255,8 @@ int ltq_layer_set_channel_qparams(ltq_layer *layer, const ltq_qparams *qp_channe
  *   out[i, j] = float(sum_k (x[i,k] - z_i) (w[j,k] - z_j)) * s_i * s_j (+ bias[j]), LTQ_FLAG_RELU on request,
  * the sum exact, each float step rounded, the result rounded to out_dtype.  x_dev uint8 [M, in_features] (dense),
  * qp_tokens_dev and asum_dev [M] as ltq_quantize_tokens_u8 leaves them, out_dev rows ld_out elements apart.  A scale of NaN
- * makes its row (or column) NaN.  Nothing is allocated; may be captured.  LTQ_FLAG_FORCE_* as in ltq_layer_forward. */
+ * makes its row (or column) NaN.  Nothing is allocated; may be captured.  LTQ_FLAG_FORCE_* as in ltq_layer_forward; the
+ * single-CTA tcgen05 kernel of this form is one for few tiles, in which a cluster shares the K of a tile. */
 int ltq_layer_forward_tokens(ltq_layer *layer, const uint8_t *x_dev, const ltq_qparams *qp_tokens_dev, const int32_t *asum_dev, uint64_t M,
                              int out_dtype, unsigned flags, void *out_dev, uint64_t ld_out, void *stream);
 
@@ -427,7 +428,8 @@ int ltq_cache_append(const ltq_kv_cache *cache, const void *k_dev, const void *v
  * 0 .. p of its sequence,  out = sum_j softmax_j(scale * q . k_j) v_j  over the dequantised keys and values.
  * q_dev [tokens][q_heads][head_dim] of `dtype`, tokens ld_q elements apart; query head h reads key/value head
  * h / (q_heads / kv_heads).  out_dev [tokens][q_heads][head_dim], same type, dense.  One token per sequence and many take the
- * same call.  workspace_dev: 16-byte aligned, ltq_cache_attention_workspace bytes, contents meaningless before and after;
+ * same call.  workspace_dev: 16-byte aligned, ltq_cache_attention_workspace bytes (none for some sizes: then it may be NULL),
+ * contents meaningless before and after;
  * calls that may overlap on the GPU need workspaces of their own.  q is taken to 22 significant bits (relative to its row's
  * largest entry) and the probabilities to 11 bits - 22 for float output; sums are held in float. */
 uint64_t ltq_cache_attention_workspace(const ltq_kv_cache *cache, uint64_t tokens, uint32_t q_heads, uint64_t seqs, uint64_t table_width,

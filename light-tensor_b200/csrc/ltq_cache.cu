@@ -257,7 +257,7 @@ AttnPlan attn_plan(const ltq_kv_cache *c, int dtype, uint32_t q_heads, uint64_t 
                 t.ml = t.items * t.splits * t.rows_per_tile;
                 t.o_floats = t.ml * c->head_dim;
             }
-            t.bytes = t.splits > 1 ? t.o_floats * sizeof(float) + t.ml * sizeof(float2) + t.items * sizeof(int2) : 16;
+            t.bytes = t.splits > 1 ? t.o_floats * sizeof(float) + t.ml * sizeof(float2) + t.items * sizeof(int2) : 0;
             return t;
         }
     }
@@ -269,8 +269,7 @@ AttnPlan attn_plan(const ltq_kv_cache *c, int dtype, uint32_t q_heads, uint64_t 
     p.cluster = 8;
     while (p.cluster > 1 && p.items * p.cluster > slots) p.cluster /= 2;
     if (steps <= (uint64_t)p.cluster * ATTN_WARPS * ATTN_CLUSTER_STEPS) {
-        p.bytes = 16;
-        return p;
+        return p;   // (no workspace)
     }
     p.cluster = 0;
     const uint64_t most = (p.items * steps + ATTN_MIN_STEPS - 1) / ATTN_MIN_STEPS;
@@ -335,7 +334,7 @@ int ltq_cache_attention(const ltq_kv_cache *cache, const void *q_dev, int dtype,
     LTQ_REQUIRE(q_heads >= 1 && q_heads % cache->kv_heads == 0 && q_heads / cache->kv_heads <= 1024, LTQ_ERR_INVALID_ARG,
                 "%u query heads do not divide over %u key/value heads", q_heads, cache->kv_heads);
     if (tokens == 0 || seqs == 0 || max_new == 0) return LTQ_OK;
-    LTQ_REQUIRE(q_dev && out_dev && workspace_dev, LTQ_ERR_INVALID_ARG, "Invalid argument");
+    LTQ_REQUIRE(q_dev && out_dev, LTQ_ERR_INVALID_ARG, "Invalid argument");
     rc = check_batch(cache, offsets_dev, lengths_dev, table_dev, tokens, seqs, table_width, max_new);
     if (rc != LTQ_OK) return rc;
     const uint64_t row = (uint64_t)q_heads * cache->head_dim;
@@ -359,7 +358,7 @@ int ltq_cache_attention(const ltq_kv_cache *cache, const void *q_dev, int dtype,
     a.group = q_heads / cache->kv_heads;
     a.scale_log2 = scale * 1.4426950408889634f;
     const AttnPlan p = attn_plan(cache, dtype, q_heads, seqs, table_width, max_new, dev->sms);
-    LTQ_REQUIRE(workspace_bytes >= p.bytes, LTQ_ERR_INVALID_ARG, "the workspace holds %llu bytes, %llu are needed",
+    LTQ_REQUIRE(p.bytes == 0 || (workspace_dev && workspace_bytes >= p.bytes), LTQ_ERR_INVALID_ARG, "the workspace holds %llu bytes, %llu are needed",
                 (unsigned long long)workspace_bytes, (unsigned long long)p.bytes);
     a.q_vec = ld_q % 4 == 0 && ((uintptr_t)q_dev % (4 * dtype_size(dtype))) == 0;
     a.q_vec8 = (ld_q * dtype_size(dtype)) % 16 == 0 && ((uintptr_t)q_dev & 15) == 0;

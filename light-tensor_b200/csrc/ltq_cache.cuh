@@ -48,7 +48,7 @@ struct AttnArgs {
     float *part_o;                 // [2 * warps][rows per tile][head_dim]
     float2 *part_ml;               // [2 * warps][rows per tile]: running maximum (base 2), sum
     int2 *item;                    // [seqs][row tiles][kv_heads]: first slot, last warp
-    uint32_t ctas, row_tiles;
+    uint32_t ctas, row_tiles;      // (tensor-core form: the SMs, groups of row tiles)
     uint32_t splits;               // tensor-core form: CTAs that share one's keys
     uint32_t cluster;              // CTAs per item in the form without workspace; 0: the form with
 };
@@ -70,6 +70,5 @@ constexpr uint32_t ATTN_TC_MIN_TILES = 4;      // a split takes at least as many
 // Joins its parts.
 cudaError_t launch_attention_join_f16(const AttnArgs &a, uint32_t rows_per_tile, cudaStream_t stream);
 cudaError_t launch_attention_join_bf16(const AttnArgs &a, uint32_t rows_per_tile, cudaStream_t stream);
-cudaError_t launch_attention_join_f32(const AttnArgs &a, uint32_t rows_per_tile, cudaStream_t stream);
 
 }  // namespace ltq

@@ -1,5 +1,5 @@
 // Attention of a few new tokens over the 8-bit cache, one instantiation per element type of q (the including file defines
-// LTQ_ATTN_DT, LTQ_ATTN_LAUNCH and LTQ_ATTN_JOIN).
+// LTQ_ATTN_DT, LTQ_ATTN_LAUNCH and, where the type has a tensor-core form, LTQ_ATTN_JOIN).
 //
 // Reading the cache is the floor (2 * head_dim bytes per key and head); all query heads of a group and all new tokens of a
 // sequence share that read.  A warp streams 16 keys at a time straight from global memory into the operand layout of
@@ -856,6 +856,7 @@ cudaError_t launch_d(const AttnArgs &a, cudaStream_t stream)
 
 }  // namespace
 
+#ifdef LTQ_ATTN_JOIN   // the types that have a tensor-core form
 cudaError_t LTQ_ATTN_JOIN(const AttnArgs &a, uint32_t rows_per_tile, cudaStream_t stream)
 {
     switch (a.cache.head_dim) {
@@ -868,6 +869,7 @@ cudaError_t LTQ_ATTN_JOIN(const AttnArgs &a, uint32_t rows_per_tile, cudaStream_
         default: return cudaErrorInvalidValue;
     }
 }
+#endif
 
 cudaError_t LTQ_ATTN_LAUNCH(const AttnArgs &a, cudaStream_t stream)
 {

@@ -2,5 +2,4 @@
 #include "../../include/ltq.h"
 #define LTQ_ATTN_DT LTQ_F32
 #define LTQ_ATTN_LAUNCH launch_attention_f32
-#define LTQ_ATTN_JOIN launch_attention_join_f32
 #include "ltq_cache_attention.cuh"

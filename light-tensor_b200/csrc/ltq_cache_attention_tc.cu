@@ -6,19 +6,29 @@
 //   P               = exp2(S * scales - m)     one thread per row, straight out of tensor memory
 //   O [128 x D]    += P [128 x keys] . V       P as the operand in tensor memory (over S), V transposed in shared memory
 //
-//   softmax      four warps per row tile: thread = row = TMEM lane.  No reduction crosses threads.  The reference maximum m moves
-//                only when a tile's probabilities add up to more than 2^12, so that O is hardly ever rescaled and no maximum is
-//                taken on the way; P waits in registers until that is known.
+//   copies       one warp: a tile's codes by bulk copies into a ring, up to four parts ahead.
 //   conversion   four warps for K, four for V: codes -> halves, for both row tiles.  K's codes become subnormal halves, code * 2^-24, by
 //                a byte permute alone, their zero points come off the scores (times the sum of q).  V's get 0x64 above them,
 //                the half 1024 + code, minus (1024 + zero point), exact.  K is written as rows of keys, V as rows of head dimensions
 //                (eight keys' bytes gathered per 16-byte store), both under the 128-byte swizzle the MMA reads; lanes are
-//                dealt so that stores spread over the banks.  The next half tile's codes are on their way into registers meanwhile.
-//   MMA issue    one warp per row tile, so that each goes its own way: while one row tile is in its softmax, the tensor core has
-//                the other's products.
-// S has two buffers, so that the next tile's is there when a softmax is done; P overwrites it.  (Measured on 2 x 1500 new tokens
-// behind up to 4500, 32 query and 8 key/value heads of 128: one warp issuing for both row tiles was busy 2300 of 3250 cycles a
-// tile, 372 us; tiles of 128 keys with one S buffer leave the softmax waiting for the two products in between, 474 us.)
+//                dealt so that loads and stores spread over the banks.
+//   MMA issue    one warp per row tile, so that each goes its own way: S of a tile goes out before O of the one in front.
+//   softmax      two warpgroups per row tile take the tiles in turn, one per S buffer: thread = row = TMEM lane, so that no reduction
+//                crosses threads.  The reference maximum m moves only when a tile's probabilities add up to more than 2^12,
+//                O is hardly ever rescaled and no maximum is taken on the way.  m is an integer: what two tiles in a row, which
+//                two warps have at the same time, have to agree on is a power of two.  A tile with masked keys or a new
+//                maximum goes a careful way of its own, from the scores that are still in tensor memory.
+//   parameters   one warp: the scales and zero points of every 16 keys.
+//
+// Measured on 1500 and 1109 new tokens behind up to 4500, 32 query and 8 key/value heads of 128 (232 us, 109 us at the tensor cores'
+// measured rate).  A tile takes about 2000 cycles; its MMAs take 1300 of them (48 each for S, where Q's 4 KB per 16 of D come
+// through the shared memory port, 64 for O; nothing else slows them down, but every access to tensor memory waits about 90
+// cycles for a gap between them, whatever its width), its exponentials 1024, its instructions about 1400 issue slots.
+//  * one softmax warpgroup per row tile: 299 us (its chain of latencies is the bound)
+//  * codes loaded by the converting warps themselves: 330 us (load latency per tile)
+//  * masks as selects on the common way: 247 us
+//  * tiles of 128 keys, one S buffer: 375 us; the two row tiles issued by one warp: slower by a fifth
+//  * the tiles divided evenly over persistent CTAs, with a join: 289 us (each piece of a group costs about 15 000 cycles)
 // The warps' registers are divided by need (setmaxnreg).
 //
 // Scales: K's block scale multiplies the scores, V's goes into the exponent as log2 of its ratio to a reference (at least twice
@@ -264,7 +274,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
         return keys > 0 ? ((uint32_t)keys + G::KEYS - 1) / G::KEYS : 0u;
     };
     // This CTA's group of row tiles.  Where there is more than the device takes at once the groups go by the tiles they see, most first
-    // (2 x 1500 new tokens behind up to 4500: 270 us in the grid's order, the last groups first, LPT us by tiles).
+    // (the case above: 271 us in the grid's order, 247 us by tiles, both before the last step).
     const uint32_t split = blockIdx.x / a.cache.kv_heads, h = blockIdx.x - split * a.cache.kv_heads, pairs = gridDim.y * gridDim.z;
     uint32_t b = blockIdx.y, group = gridDim.z - 1 - blockIdx.z;
     if (pairs * gridDim.x > a.ctas && pairs <= G::THREADS) {

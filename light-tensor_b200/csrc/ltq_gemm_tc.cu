@@ -460,84 +460,84 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 if (++as == 2) { as = 0; aph ^= 1; }
             }
         } else {
-        const EpilogueConsts c = epilogue_consts(epi);
-        const bool relu = epi.flags & LTQ_FLAG_RELU, sat = epi.flags & LTQ_FLAG_SATURATE;
-        using OutT = typename std::conditional<OUT == 0, uint8_t, typename std::conditional<OUT == 1, float, int32_t>::type>::type;
-        const uint64_t ldc = epilogue_pitch(epi, N);
-        const bool vec_ok = epilogue_vec_ok(epi, out, N, sizeof(OutT));
-        const bool staged = epi.staged && vec_ok && epi.col_block == 0;
-        constexpr int ESZ = (int)sizeof(OutT), BLOCK_COLS = 128 / ESZ;   // a staged block: 128 bytes per row
-        uint8_t *stage = s_stage + (warp - 2) * PeerStage::BYTES_PER_WARP;
-        uint32_t as = 0, aph = 0;
-        bool ok = true;
-        for (uint32_t t = pair; t < num_tiles; t += num_pairs) {
-            const PairTile pt = pair_tile(tl, t);
-            const uint32_t m0 = pt.m0 + rank * BM, n0 = pt.n0;
-            const int width = (int)pt.width;
-            const int split = ((width / 2 + 15) / 16) * 16;   // columns [0, split) go to the h = 0 warps, the rest to h = 1
-            uint32_t *col = s_col + as * P_BN;
-            for (uint32_t j = et; j < (uint32_t)width; j += 256) {
-                const uint32_t gj = n0 + j;
-                col[j] = gj < N ? epilogue_col_term(epi, c, gj) : 0u;
-            }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            const uint32_t row = m0 + q * 32 + lane;
-            const uint32_t rt = row < M ? epilogue_row_term(epi, c, row) : 0u;
+            const EpilogueConsts c = epilogue_consts(epi);
+            const bool relu = epi.flags & LTQ_FLAG_RELU, sat = epi.flags & LTQ_FLAG_SATURATE;
+            using OutT = typename std::conditional<OUT == 0, uint8_t, typename std::conditional<OUT == 1, float, int32_t>::type>::type;
+            const uint64_t ldc = epilogue_pitch(epi, N);
+            const bool vec_ok = epilogue_vec_ok(epi, out, N, sizeof(OutT));
+            const bool staged = epi.staged && vec_ok && epi.col_block == 0;
+            constexpr int ESZ = (int)sizeof(OutT), BLOCK_COLS = 128 / ESZ;   // a staged block: 128 bytes per row
+            uint8_t *stage = s_stage + (warp - 2) * PeerStage::BYTES_PER_WARP;
+            uint32_t as = 0, aph = 0;
+            bool ok = true;
+            for (uint32_t t = pair; t < num_tiles; t += num_pairs) {
+                const PairTile pt = pair_tile(tl, t);
+                const uint32_t m0 = pt.m0 + rank * BM, n0 = pt.n0;
+                const int width = (int)pt.width;
+                const int split = ((width / 2 + 15) / 16) * 16;   // columns [0, split) go to the h = 0 warps, the rest to h = 1
+                uint32_t *col = s_col + as * P_BN;
+                for (uint32_t j = et; j < (uint32_t)width; j += 256) {
+                    const uint32_t gj = n0 + j;
+                    col[j] = gj < N ? epilogue_col_term(epi, c, gj) : 0u;
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                const uint32_t row = m0 + q * 32 + lane;
+                const uint32_t rt = row < M ? epilogue_row_term(epi, c, row) : 0u;
 
-            if (ok) ok = mbar_wait(tfull0 + 8 * as, aph, abort_flag, status, 0x400u | as);
-            if (ok) {
-                tc_fence_after();
-                const uint32_t taddr = tmem_base + ((q * 32u) << 16) + as * P_BN;
-                const int cb = h ? split : 0, ce = h ? width : split;
-                const bool rows_full = m0 + q * 32 + 32 <= M;
-                uint32_t rsum = 0;  // sum of this row's uint8 outputs in this warp's part of the tile
-                // One chunk of CW (32, or 16 for a remainder) accumulator columns.  Blocks of 128 output bytes per row go
-                // through the row-coalescing stage when results leave the GPU and the warp's 32 rows and the block's columns
-                // are all inside the matrix; everything else is stored directly.  (32-column chunks with two adjacent
-                // 16-byte stores per row measured 20 % faster than 16-column chunks with one, software-pipelined TMEM
-                // loads included: the stores, one 32-byte sector per row, are what the chunk waits for.)
-                auto chunk = [&](auto &v, int cc) {
-                    constexpr int CW = (int)(sizeof(v) / sizeof(uint32_t));
-                    const uint32_t c0 = n0 + cc;
-                    const int bc0 = cb + ((cc - cb) / BLOCK_COLS) * BLOCK_COLS;          // first column of cc's block
-                    const int bcols = (ce - bc0) < BLOCK_COLS ? (ce - bc0) : BLOCK_COLS;  // its width
-                    const bool via_stage = staged && rows_full && n0 + bc0 + bcols <= N;
-                    if (via_stage) {
-                        uint32_t res[CW];
-                        epilogue_convert<OUT, CW>(v, rt, col + cc, c, relu, sat, res);
-                        PeerStage::put<CW>(stage, lane, (cc - bc0) * ESZ / 16, res, CW * ESZ / 16);
-                        if (OUT == 0) rsum += packed_byte_sum<CW>(res, CW);
-                        const int next = cc + CW;
-                        if (next == ce || (next - cb) % BLOCK_COLS == 0)   // the block is complete
-                            PeerStage::flush(stage, lane, bcols * ESZ / 16, epi, out,
-                                             ((uint64_t)(m0 + q * 32) * ldc + n0 + bc0) * ESZ, ldc * ESZ);
-                    } else if (row < M && c0 < N) {
-                        rsum += epilogue_chunk<OUT, CW>(v, rt, col + cc, c, relu, sat, epi, out, epilogue_offset(epi, row, c0, ldc),
-                                                        vec_ok, (N - c0) < (uint32_t)CW ? (int)(N - c0) : CW);
-                    }
-                };
-                int cc = cb;
+                if (ok) ok = mbar_wait(tfull0 + 8 * as, aph, abort_flag, status, 0x400u | as);
+                if (ok) {
+                    tc_fence_after();
+                    const uint32_t taddr = tmem_base + ((q * 32u) << 16) + as * P_BN;
+                    const int cb = h ? split : 0, ce = h ? width : split;
+                    const bool rows_full = m0 + q * 32 + 32 <= M;
+                    uint32_t rsum = 0;  // sum of this row's uint8 outputs in this warp's part of the tile
+                    // One chunk of CW (32, or 16 for a remainder) accumulator columns.  Blocks of 128 output bytes per row go
+                    // through the row-coalescing stage when results leave the GPU and the warp's 32 rows and the block's columns
+                    // are all inside the matrix; everything else is stored directly.  (32-column chunks with two adjacent
+                    // 16-byte stores per row measured 20 % faster than 16-column chunks with one, software-pipelined TMEM
+                    // loads included: the stores, one 32-byte sector per row, are what the chunk waits for.)
+                    auto chunk = [&](auto &v, int cc) {
+                        constexpr int CW = (int)(sizeof(v) / sizeof(uint32_t));
+                        const uint32_t c0 = n0 + cc;
+                        const int bc0 = cb + ((cc - cb) / BLOCK_COLS) * BLOCK_COLS;          // first column of cc's block
+                        const int bcols = (ce - bc0) < BLOCK_COLS ? (ce - bc0) : BLOCK_COLS;  // its width
+                        const bool via_stage = staged && rows_full && n0 + bc0 + bcols <= N;
+                        if (via_stage) {
+                            uint32_t res[CW];
+                            epilogue_convert<OUT, CW>(v, rt, col + cc, c, relu, sat, res);
+                            PeerStage::put<CW>(stage, lane, (cc - bc0) * ESZ / 16, res, CW * ESZ / 16);
+                            if (OUT == 0) rsum += packed_byte_sum<CW>(res, CW);
+                            const int next = cc + CW;
+                            if (next == ce || (next - cb) % BLOCK_COLS == 0)   // the block is complete
+                                PeerStage::flush(stage, lane, bcols * ESZ / 16, epi, out,
+                                                 ((uint64_t)(m0 + q * 32) * ldc + n0 + bc0) * ESZ, ldc * ESZ);
+                        } else if (row < M && c0 < N) {
+                            rsum += epilogue_chunk<OUT, CW>(v, rt, col + cc, c, relu, sat, epi, out, epilogue_offset(epi, row, c0, ldc),
+                                                            vec_ok, (N - c0) < (uint32_t)CW ? (int)(N - c0) : CW);
+                        }
+                    };
+                    int cc = cb;
 #pragma unroll 1
-                for (; cc + 32 <= ce; cc += 32) {
-                    uint32_t v[32];
-                    tmem_ld32(taddr + cc, v);
-                    tmem_ld_wait();
-                    chunk(v, cc);
+                    for (; cc + 32 <= ce; cc += 32) {
+                        uint32_t v[32];
+                        tmem_ld32(taddr + cc, v);
+                        tmem_ld_wait();
+                        chunk(v, cc);
+                    }
+                    if (cc < ce) {  // widths are multiples of 16
+                        uint32_t v[16];
+                        tmem_ld16(taddr + cc, v);
+                        tmem_ld_wait();
+                        chunk(v, cc);
+                    }
+                    if (OUT == 0 && epi.out_rowsum && row < M) atomicAdd(&epi.out_rowsum[row], (int32_t)rsum);
+                    // this warp has read its part of the accumulator: tell the leader's MMA warp (in this or the other CTA)
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_remote(in_leader_cta(tempty0 + 8 * as));
                 }
-                if (cc < ce) {  // widths are multiples of 16
-                    uint32_t v[16];
-                    tmem_ld16(taddr + cc, v);
-                    tmem_ld_wait();
-                    chunk(v, cc);
-                }
-                if (OUT == 0 && epi.out_rowsum && row < M) atomicAdd(&epi.out_rowsum[row], (int32_t)rsum);
-                // this warp has read its part of the accumulator: tell the leader's MMA warp (in this or the other CTA)
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_remote(in_leader_cta(tempty0 + 8 * as));
+                if (++as == 2) { as = 0; aph ^= 1; }
             }
-            if (++as == 2) { as = 0; aph ^= 1; }
-        }
         }
     }
 

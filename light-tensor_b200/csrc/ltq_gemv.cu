@@ -352,43 +352,57 @@ gemv_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
                 if (++as == 2) { as = 0; aph ^= 1; }
             }
         } else {
-        const EpilogueConsts c = epilogue_consts(epi);
-        const bool relu = epi.flags & LTQ_FLAG_RELU, sat = epi.flags & LTQ_FLAG_SATURATE;
-        using OutT = typename std::conditional<OUT == 0, uint8_t, typename std::conditional<OUT == 1, float, int32_t>::type>::type;
-        OutT *o = static_cast<OutT *>(out);
-        const uint64_t ldc = epilogue_pitch(epi, N);
-        uint32_t rt[XROWS];  // per-token part of the correction; identical for every weight row
+            const EpilogueConsts c = epilogue_consts(epi);
+            const bool relu = epi.flags & LTQ_FLAG_RELU, sat = epi.flags & LTQ_FLAG_SATURATE;
+            using OutT = typename std::conditional<OUT == 0, uint8_t, typename std::conditional<OUT == 1, float, int32_t>::type>::type;
+            OutT *o = static_cast<OutT *>(out);
+            const uint64_t ldc = epilogue_pitch(epi, N);
+            uint32_t rt[XROWS];  // per-token part of the correction; identical for every weight row
 #pragma unroll
-        for (int m = 0; m < XROWS; m++) rt[m] = (uint32_t)m < M ? epilogue_row_term(epi, c, (uint32_t)m) : 0u;
-        uint32_t as = 0, aph = 0;
-        bool ok = true;
-        for (uint32_t t = t_begin; t < t_end; t++) {
-            const uint32_t o0 = (uint32_t)(((uint64_t)t * octs) / tiles), o1 = (uint32_t)(((uint64_t)(t + 1) * octs) / tiles);
-            const uint32_t n = o0 * 8 + q * 32 + lane;
-            const bool valid = (q * 32 + lane) < (o1 - o0) * 8 && n < N;
-            // fetched before waiting, so the global-memory latency passes under the stream
-            const uint32_t ct = valid ? epilogue_col_term(epi, c, n) : 0u;
-            if (ok) ok = mbar_wait(tfull0 + 8 * as, aph, abort_flag, status, 0x400u | as);
-            if (ok) {
-                tc_fence_after();
-                uint32_t v[XROWS];
-                const uint32_t tacc = tmem_base + ((q * 32u) << 16) + as * (NACC * XROWS);
-                uint32_t w1[XROWS], w2[XROWS], w3[XROWS];
-                static_assert(NACC == 4, "the epilogue adds four accumulators");
-                tmem_ld16(tacc, v);
-                tmem_ld16(tacc + XROWS, w1);
-                tmem_ld16(tacc + 2 * XROWS, w2);
-                tmem_ld16(tacc + 3 * XROWS, w3);
-                tmem_ld_wait();
+            for (int m = 0; m < XROWS; m++) rt[m] = (uint32_t)m < M ? epilogue_row_term(epi, c, (uint32_t)m) : 0u;
+            uint32_t as = 0, aph = 0;
+            bool ok = true;
+            for (uint32_t t = t_begin; t < t_end; t++) {
+                const uint32_t o0 = (uint32_t)(((uint64_t)t * octs) / tiles), o1 = (uint32_t)(((uint64_t)(t + 1) * octs) / tiles);
+                const uint32_t n = o0 * 8 + q * 32 + lane;
+                const bool valid = (q * 32 + lane) < (o1 - o0) * 8 && n < N;
+                // fetched before waiting, so the global-memory latency passes under the stream
+                const uint32_t ct = valid ? epilogue_col_term(epi, c, n) : 0u;
+                if (ok) ok = mbar_wait(tfull0 + 8 * as, aph, abort_flag, status, 0x400u | as);
+                if (ok) {
+                    tc_fence_after();
+                    uint32_t v[XROWS];
+                    const uint32_t tacc = tmem_base + ((q * 32u) << 16) + as * (NACC * XROWS);
+                    uint32_t w1[XROWS], w2[XROWS], w3[XROWS];
+                    static_assert(NACC == 4, "the epilogue adds four accumulators");
+                    tmem_ld16(tacc, v);
+                    tmem_ld16(tacc + XROWS, w1);
+                    tmem_ld16(tacc + 2 * XROWS, w2);
+                    tmem_ld16(tacc + 3 * XROWS, w3);
+                    tmem_ld_wait();
 #pragma unroll
-                for (int m = 0; m < XROWS; m++) v[m] += w1[m] + w2[m] + w3[m];
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(tempty0 + 8 * as);  // accumulator buffer may be overwritten
-                const bool plain = epi.n_more == 0 && epi.col_block == 0 && !(OUT == 0 && epi.out_rowsum);
-                if (plain) {
-                    // one dense destination: the common case, kept free of the general path's loops
-                    if (valid) {
+                    for (int m = 0; m < XROWS; m++) v[m] += w1[m] + w2[m] + w3[m];
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(tempty0 + 8 * as);  // accumulator buffer may be overwritten
+                    const bool plain = epi.n_more == 0 && epi.col_block == 0 && !(OUT == 0 && epi.out_rowsum);
+                    if (plain) {
+                        // one dense destination: the common case, kept free of the general path's loops
+                        if (valid) {
+#pragma unroll
+                            for (int m = 0; m < XROWS; m++) {
+                                if ((uint32_t)m < M) {
+                                    const int32_t a = epilogue_acc(v[m], rt[m], ct, relu);
+                                    OutT r;
+                                    if (OUT == 0) r = (OutT)epilogue_u8(a, c, sat);
+                                    else if (OUT == 1) r = (OutT)epilogue_f32(a, c);
+                                    else r = (OutT)a;
+                                    o[(size_t)m * ldc + n] = r;
+                                }
+                            }
+                        }
+                    } else {
+                        // several destinations, column-blocked output, row sums (warp-wide reductions: all lanes run the loop)
 #pragma unroll
                         for (int m = 0; m < XROWS; m++) {
                             if ((uint32_t)m < M) {
@@ -397,33 +411,19 @@ gemv_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
                                 if (OUT == 0) r = (OutT)epilogue_u8(a, c, sat);
                                 else if (OUT == 1) r = (OutT)epilogue_f32(a, c);
                                 else r = (OutT)a;
-                                o[(size_t)m * ldc + n] = r;
-                            }
-                        }
-                    }
-                } else {
-                    // several destinations, column-blocked output, row sums (warp-wide reductions: all lanes run the loop)
-#pragma unroll
-                    for (int m = 0; m < XROWS; m++) {
-                        if ((uint32_t)m < M) {
-                            const int32_t a = epilogue_acc(v[m], rt[m], ct, relu);
-                            OutT r;
-                            if (OUT == 0) r = (OutT)epilogue_u8(a, c, sat);
-                            else if (OUT == 1) r = (OutT)epilogue_f32(a, c);
-                            else r = (OutT)a;
-                            if (valid)
-                                for (int d = -1; d < epi.n_more; d++)
-                                    (d < 0 ? o : static_cast<OutT *>(epi.more_out[d]))[epilogue_offset(epi, (uint64_t)m, n, ldc)] = r;
-                            if (OUT == 0 && epi.out_rowsum) {  // token m: this warp's 32 outputs add up first
-                                const uint32_t t32 = __reduce_add_sync(0xFFFFFFFFu, valid ? (uint32_t)r : 0u);
-                                if (lane == 0 && t32) atomicAdd(&epi.out_rowsum[m], (int32_t)t32);
+                                if (valid)
+                                    for (int d = -1; d < epi.n_more; d++)
+                                        (d < 0 ? o : static_cast<OutT *>(epi.more_out[d]))[epilogue_offset(epi, (uint64_t)m, n, ldc)] = r;
+                                if (OUT == 0 && epi.out_rowsum) {  // token m: this warp's 32 outputs add up first
+                                    const uint32_t t32 = __reduce_add_sync(0xFFFFFFFFu, valid ? (uint32_t)r : 0u);
+                                    if (lane == 0 && t32) atomicAdd(&epi.out_rowsum[m], (int32_t)t32);
+                                }
                             }
                         }
                     }
                 }
+                if (++as == 2) { as = 0; aph ^= 1; }
             }
-            if (++as == 2) { as = 0; aph ^= 1; }
-        }
         }
     }
 

@@ -30,7 +30,7 @@ class KVCache:
         self._desc = KVCacheDesc(k.data_ptr(), k_qparams.data_ptr(), v.data_ptr(), v_qparams.data_ptr(), self.blocks, self.kv_heads,
                                  self.block_tokens, self.head_dim)
         self._ref = C.byref(self._desc)
-        self._as_rows = tuple((t.view(self.blocks * self.kv_heads, self.block_tokens * self.head_dim), p.view(-1, 8)) for t, p in ((k, k_qparams), (v, v_qparams)))
+        self._sizes = self._bytes = None
 
     @classmethod
     def empty(cls, blocks, kv_heads, block_tokens, head_dim, device="cuda"):
@@ -82,16 +82,21 @@ class KVCache:
         code = _tokens.dtype_code(q.dtype)
         seqs, width = self._batch(table, lengths, offsets)
         if out is None:
-            out = q.new_empty((tokens, heads, self.head_dim))
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif not (out.get_device() == self._index and out.dtype is q.dtype and out.shape == q.shape and out.is_contiguous()):
             raise ValueError("out must be a contiguous tensor of q's shape, type and device")
         if workspace is None:
-            workspace = q.new_empty(self.attention_workspace(tokens, heads, seqs, width, max_new), dtype=torch.uint8)
+            sizes = (tokens, heads, seqs, width, max_new)
+            if sizes != self._sizes:   # (a decode loop's calls have the same ones)
+                self._sizes, self._bytes = sizes, self.attention_workspace(*sizes)
+            if self._bytes:
+                workspace = q.new_empty(self._bytes, dtype=torch.uint8)
         elif not (workspace.get_device() == self._index and workspace.dtype is torch.uint8 and workspace.is_contiguous()):
             raise ValueError("workspace must be a contiguous uint8 tensor on q's device")
         check(lib().ltq_cache_attention(self._ref, q.data_ptr(), code, ld, tokens, heads, offsets.data_ptr(), lengths.data_ptr(),
                                         table.data_ptr(), seqs, width, max_new, self.head_dim ** -0.5 if scale is None else scale,
-                                        out.data_ptr(), workspace.data_ptr(), workspace.numel(), self._index, _tokens.raw_stream(self._index)))
+                                        out.data_ptr(), workspace.data_ptr() if workspace is not None else None,
+                                        workspace.numel() if workspace is not None else 0, self._index, _tokens.raw_stream(self._index)))
         return out
 
     def attention_workspace(self, tokens, q_heads, seqs, width, max_new):
@@ -100,7 +105,12 @@ class KVCache:
 
     def values(self, dtype=torch.float32):
         """Keys and values of all slots as numbers: two tensors [blocks, kv_heads, block_tokens, head_dim] of `dtype`."""
-        return tuple(_tokens.dequantize_tokens(t, p, dtype).view(self.k.shape) for t, p in self._as_rows)
+        code, shape = _tokens.dtype_code(dtype), self.k.shape
+        rows, row, stream = self.blocks * self.kv_heads, self.block_tokens * self.head_dim, _tokens.raw_stream(self._index)
+        out = self.k.new_empty(shape, dtype=dtype), self.k.new_empty(shape, dtype=dtype)
+        for o, codes, qparams in zip(out, (self.k, self.v), (self.k_qparams, self.v_qparams)) if rows else ():
+            check(lib().ltq_dequantize_tokens_u8(o.data_ptr(), code, row, codes.data_ptr(), qparams.data_ptr(), rows, row, self._index, stream))
+        return out
 
     def check(self):
         """Waits for the stream and raises if a cache call met a sequence or block id outside its bounds since the last check."""

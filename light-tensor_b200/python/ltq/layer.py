@@ -100,7 +100,7 @@ class LayerHandle:
         out = self._tokens_out(out, M, dtype, x.device)
         if M:
             check(lib().ltq_layer_forward_tokens(self._h, x.data_ptr(), qparams.data_ptr(), sums.data_ptr(), M, _tokens.dtype_code(dtype), flags,
-                                                 out.data_ptr(), out.stride(0), self._stream()))
+                                                 out.data_ptr(), out.stride(0) if M > 1 else self.N, self._stream()))
         return out
 
     def forward_float(self, x, dtype=None, flags=0, out=None):
@@ -115,7 +115,7 @@ class LayerHandle:
         if out is None:
             out, ld_out = x.new_empty((M, self.N), dtype=dtype), self.N
         else:
-            out, ld_out = self._tokens_out(out, M, dtype or x.dtype, x.device), out.stride(0)
+            out, ld_out = self._tokens_out(out, M, dtype or x.dtype, x.device), out.stride(0) if M > 1 else self.N
         if M:
             need = M * self._row_workspace
             ws = x.new_empty(need, dtype=torch.uint8)

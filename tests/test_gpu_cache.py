@@ -419,6 +419,28 @@ def test_attention_strided_queries_own_buffers_and_streams(cuda):
         assert torch.equal(other, want)
 
 
+def test_attention_workspace(cuda):
+    """None is needed for a short call, and none may be too small for a long one."""
+    import ltq
+    torch = cuda
+    b = batch(torch, 16, [(1, 40)], 16)
+    cache = random_cache(torch, ltq, 16, b["blocks"], 1, 16, 64)
+    q = torch.randn(1, 4, 64).half().cuda()
+    for width in (len(b["table"][0]), 3000):
+        table = ints(torch, [b["table"][0] + [-1] * (width - len(b["table"][0]))])
+        args = (q, table, ints(torch, b["lengths"]), ints(torch, b["offsets"]), 1)
+        need = cache.attention_workspace(1, 4, 1, width, 1)
+        want = cache.attention(*args)
+        assert (need == 0) == (width < 3000)
+        assert torch.equal(cache.attention(*args, workspace=torch.empty(need, dtype=torch.uint8, device="cuda")), want)
+        if need:
+            with pytest.raises(ltq.LtqError) as e:
+                cache.attention(*args, workspace=torch.empty(need - 1, dtype=torch.uint8, device="cuda"))
+            assert e.value.status == -1
+            with pytest.raises(ltq.LtqError):
+                cache.attention(*args, workspace=torch.empty(0, dtype=torch.uint8, device="cuda"))
+
+
 def test_long_cache_offsets_beyond_32_bits(cuda):
     """Block ids whose byte offsets pass 2^32: 140 000 blocks of 16 x 8 heads x 256."""
     import ltq

@@ -72,7 +72,7 @@ def test_attention_arguments():
     L = ltq.lib()
     assert attention(L, heads=3) == attention(L, heads=0) == attention(L, heads=4096, ld=1 << 20) == -1
     assert attention(L, scale=float("inf")) == attention(L, scale=float("nan")) == -1
-    assert attention(L, q=None) == attention(L, out=None) == attention(L, ws=None) == attention(L, ws=4104) == attention(L, q=4097) == -1
+    assert attention(L, q=None) == attention(L, out=None) == attention(L, ws=4104) == attention(L, q=4097) == -1
 
 
 def test_no_cpu_fallback():
