@@ -419,6 +419,48 @@ def test_attention_strided_queries_own_buffers_and_streams(cuda):
         assert torch.equal(other, want)
 
 
+def test_prompt_attention_captured_and_on_two_streams(cuda):
+    """A captured call follows the lengths and offsets of its replay; two calls at once do not meet."""
+    import ltq
+    torch = cuda
+    big, small = [(260, 2300), (150, 900), (257, 600)], [(40, 1100), (0, 17), (300, 302)]
+    b = batch(torch, 17, big, 16)
+    cache = random_cache(torch, ltq, 17, b["blocks"], 2, 16, 128)
+    q = torch.randn(700, 8, 128, generator=torch.Generator().manual_seed(17)).bfloat16().cuda()
+    table = ints(torch, b["table"])
+    shapes = []
+    for spans in (big, small):
+        offsets = [0]
+        for n, _ in spans:
+            offsets.append(offsets[-1] + n)
+        shapes.append((ints(torch, [length for _, length in spans]), ints(torch, offsets)))
+    want = [cache.attention(q, table, *shape, 300) for shape in shapes]
+    lengths, offsets = (t.clone() for t in shapes[0])
+    out = torch.zeros_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.attention(q, table, lengths, offsets, 300, out=out)
+    for k in (0, 1, 0):
+        lengths.copy_(shapes[k][0])
+        offsets.copy_(shapes[k][1])
+        rows = int(shapes[k][1][-1])
+        graph.replay()
+        assert torch.equal(out[:rows], want[k][:rows])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(4):
+        for k, stream in enumerate(streams):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                got[k].append(cache.attention(q, table, *shapes[k], 300))
+    for stream in streams:
+        torch.cuda.current_stream().wait_stream(stream)
+    for k in range(2):
+        rows = int(shapes[k][1][-1])
+        assert all(torch.equal(o[:rows], want[k][:rows]) for o in got[k])
+    cache.check()
+
+
 def test_attention_workspace(cuda):
     """None is needed for a short call, and none may be too small for a long one."""
     import ltq
