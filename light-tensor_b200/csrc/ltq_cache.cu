@@ -124,7 +124,7 @@ cache_append_kernel(const ltq_kv_cache cache, const CacheBatch bt, const void *_
     const bool finite = most < INFINITY && scale < INFINITY;   // false for NaN, a NaN that the block had before included
     if (threadIdx.x == 0) {
         const float stored = finite ? scale : __int_as_float(0x7FC00000);
-        if (((uintptr_t)qp & 7) == 0) *reinterpret_cast<uint2 *>(qp) = make_uint2(__float_as_uint(stored), 128u);
+        *reinterpret_cast<uint2 *>(qp) = make_uint2(__float_as_uint(stored), 128u);
     }
     const float inv = quant_row_inv(scale);
     if (finite && used && scale > old) {

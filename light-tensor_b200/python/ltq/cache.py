@@ -30,7 +30,7 @@ class KVCache:
         self._desc = KVCacheDesc(k.data_ptr(), k_qparams.data_ptr(), v.data_ptr(), v_qparams.data_ptr(), self.blocks, self.kv_heads,
                                  self.block_tokens, self.head_dim)
         self._ref = C.byref(self._desc)
-        self._sizes = self._bytes = None
+        self._last = None, 0
 
     @classmethod
     def empty(cls, blocks, kv_heads, block_tokens, head_dim, device="cuda"):
@@ -87,10 +87,11 @@ class KVCache:
             raise ValueError("out must be a contiguous tensor of q's shape, type and device")
         if workspace is None:
             sizes = (tokens, heads, seqs, width, max_new)
-            if sizes != self._sizes:   # (a decode loop's calls have the same ones)
-                self._sizes, self._bytes = sizes, self.attention_workspace(*sizes)
-            if self._bytes:
-                workspace = q.new_empty(self._bytes, dtype=torch.uint8)
+            last = self._last   # sizes and bytes of a call before: a decode loop's calls have the same ones
+            if last[0] != sizes:
+                last = self._last = sizes, self.attention_workspace(*sizes)
+            if last[1]:
+                workspace = q.new_empty(last[1], dtype=torch.uint8)
         elif not (workspace.get_device() == self._index and workspace.dtype is torch.uint8 and workspace.is_contiguous()):
             raise ValueError("workspace must be a contiguous uint8 tensor on q's device")
         check(lib().ltq_cache_attention(self._ref, q.data_ptr(), code, ld, tokens, heads, offsets.data_ptr(), lengths.data_ptr(),
