@@ -26,7 +26,9 @@
 //    permute per two codes.  Zero points come off the sums: q . (k - z) = q . k - z * sum(q), and p . (v - z) = p . v - z * sum(p)
 //    with p as rounded for the MMA;
 //  * q is scaled by a power of two per row so that halves hold it (float q: split into two halves, 22 bits, and so are
-//    the probabilities then);
+//    the probabilities then; the tensor core cuts off what does not fit a sum, always towards zero, so with float q the zero
+//    points come off the codes first, exact in halves, and every product starts from zero and is added up in float: 742
+//    new tokens of 1364 were off by 1.6e-5 otherwise, now by 3e-7);
 //  * V's block scales go into the probabilities as a ratio to the largest one so far, so that one accumulator serves all;
 //  * the running maximum is kept only approximately: the reference m moves when a score exceeds it by more than 8 (base 2), so
 //    that probabilities stay below 2^8 and almost every step does without a reduction over lanes.
@@ -192,11 +194,23 @@ struct Rows {
     int pos[NT][2];                     // position of those rows' tokens (rows that do not exist see everything, with q = 0)
     int first_pos;                      // the smallest of the warp's
     float m[NT][2], l[NT][2];
-    float o[D / 16][NT][4];             // 2^-24 * sum of probability * V scale / v_ref * code
-    float zp[NT][2];                    // sum of probability * V scale / v_ref * zero point
+    float o[D / 16][NT][4];             // 2^-24 * sum of probability * V scale / v_ref * code (float q: of code - zero point, as it is)
+    float zp[NT][2];                    // sum of probability * V scale / v_ref * zero point (float q: 0)
     float v_ref, v_inv;                 // largest V scale so far and its inverse
 };
 constexpr float CODE = 16777216.f;      // 2^24: a code's half is the code over this
+constexpr bool EXACT = TERMS == 2;      // codes as the halves code - zero point instead, see above
+
+// Two codes of a word as an operand: bytes `sel` picks of w and, above each, of what makes it a half; `zero`: 1024 + zero point, twice.
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t sel, uint32_t zero)
+{
+    if (!EXACT) return prmt(w, 0, sel);
+    const uint32_t x = prmt(w, 0x64646464u, sel);   // 1024 + code
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&x), *reinterpret_cast<const __half2 *>(&zero));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+// What the sum `o` of a row says, with its `zp`.
+__device__ __forceinline__ float sum_of(float o, float zp) { return EXACT ? o : fmaf(o, CODE, -zp); }
 
 template <int D, int NT>
 __device__ __forceinline__ void load_rows(Rows<D, NT> &r, const AttnArgs &a, const CacheSeq &s, uint32_t h, uint32_t row0, int g, int c)
@@ -301,19 +315,28 @@ __device__ __forceinline__ void take_keys(Rows<D, NT> &r, const Keys<D> &keys, i
     const float k_scale = __uint_as_float(keys.k_par.x), v_scale = __uint_as_float(keys.v_par.x);
     const float k_zero = (float)(keys.k_par.y & 0xFF), v_zero = (float)(keys.v_par.y & 0xFF);
     const bool bad = keys.bad;
-    float acc[NT][2][4];   // two chains: an MMA waits for the one before it on the same accumulator
+    const uint32_t k_zero2 = 0x64006400u + (keys.k_par.y & 0xFF) * 0x10001u, v_zero2 = 0x64006400u + (keys.v_par.y & 0xFF) * 0x10001u;
+    float acc[NT][2][4];   // two chains: an MMA waits for the one before it on the same accumulator 
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int j = 0; j < 4; j++) acc[nt][0][j] = acc[nt][1][j] = 0.f;
 #pragma unroll
     for (int w = 0; w < D / 16; w++) {
-        const uint32_t a0 = prmt(keys.k[0][w], 0, 0x4140), a2 = prmt(keys.k[0][w], 0, 0x4342);
-        const uint32_t a1 = prmt(keys.k[1][w], 0, 0x4140), a3 = prmt(keys.k[1][w], 0, 0x4342);
+        const uint32_t a0 = code_pair(keys.k[0][w], 0x4140, k_zero2), a2 = code_pair(keys.k[0][w], 0x4342, k_zero2);
+        const uint32_t a1 = code_pair(keys.k[1][w], 0x4140, k_zero2), a3 = code_pair(keys.k[1][w], 0x4342, k_zero2);
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int nt = 0; nt < NT; nt++) {
+            if (EXACT) {
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < TERMS; i++) mma16816(acc[nt][w & 1], a0, a1, a2, a3, r.q[i][nt][w][0], r.q[i][nt][w][1]);
+                for (int i = TERMS - 1; i >= 0; i--) mma16816(part, a0, a1, a2, a3, r.q[i][nt][w][0], r.q[i][nt][w][1]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[nt][w & 1][j] += part[j];
+            } else {
+                mma16816(acc[nt][w & 1], a0, a1, a2, a3, r.q[0][nt][w][0], r.q[0][nt][w][1]);
+            }
+        }
     }
 
     // t = score - m.  Of element j: row 2c + (j & 1), key g + 8 * (j >> 1).
@@ -325,8 +348,8 @@ __device__ __forceinline__ void take_keys(Rows<D, NT> &r, const Keys<D> &keys, i
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const float x = r.scale[nt][j] * k_scale;
-            sc[nt][j] = x * CODE;
-            zo[nt][j] = x * (k_zero * r.q_sum[nt][j]);
+            sc[nt][j] = EXACT ? x : x * CODE;
+            zo[nt][j] = EXACT ? 0.f : x * (k_zero * r.q_sum[nt][j]);
         }
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -415,8 +438,10 @@ __device__ __forceinline__ void take_keys(Rows<D, NT> &r, const Keys<D> &keys, i
                 b.x += d.x;
                 b.y += d.y;
             }
-            r.zp[nt][0] = fmaf(v_zero, b.x, r.zp[nt][0]);
-            r.zp[nt][1] = fmaf(v_zero, b.y, r.zp[nt][1]);
+            if (!EXACT) {
+                r.zp[nt][0] = fmaf(v_zero, b.x, r.zp[nt][0]);
+                r.zp[nt][1] = fmaf(v_zero, b.y, r.zp[nt][1]);
+            }
         }
     }
 #pragma unroll
@@ -425,11 +450,20 @@ __device__ __forceinline__ void take_keys(Rows<D, NT> &r, const Keys<D> &keys, i
         for (int half = 0; half < 2; half++) {
             const uint32_t sel = half ? 0x7362 : 0x5140;
             const uint32_t x = prmt(keys.v[0][w], keys.v[1][w], sel), y = prmt(keys.v[2][w], keys.v[3][w], sel);
-            const uint32_t a0 = prmt(x, 0, 0x4140), a1 = prmt(x, 0, 0x4342), a2 = prmt(y, 0, 0x4140), a3 = prmt(y, 0, 0x4342);
+            const uint32_t a0 = code_pair(x, 0x4140, v_zero2), a1 = code_pair(x, 0x4342, v_zero2);
+            const uint32_t a2 = code_pair(y, 0x4140, v_zero2), a3 = code_pair(y, 0x4342, v_zero2);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+            for (int nt = 0; nt < NT; nt++) {
+                if (EXACT) {
+                    float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < TERMS; i++) mma16816(r.o[2 * w + half][nt], a0, a1, a2, a3, p[i][nt][0], p[i][nt][1]);
+                    for (int i = TERMS - 1; i >= 0; i--) mma16816(part, a0, a1, a2, a3, p[i][nt][0], p[i][nt][1]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) r.o[2 * w + half][nt][j] += part[j];
+                } else {
+                    mma16816(r.o[2 * w + half][nt], a0, a1, a2, a3, p[0][nt][0], p[0][nt][1]);
+                }
+            }
         }
     }
 }
@@ -540,7 +574,7 @@ __device__ __forceinline__ void do_segment(const AttnArgs &a, uint32_t b, const 
             const float f = whole ? (l == 0.f ? 0.f : __fdiv_rn(r.v_ref, l)) : r.v_ref;   // (a row that sees nothing: zeros)
 #pragma unroll
             for (int w = 0; w < D / 32; w++) {
-                auto real = [&](float x) { return fmaf(x, CODE, -zp) * f; };
+                auto real = [&](float x) { return sum_of(x, zp) * f; };
                 const float x0 = real(r.o[2 * w][nt][j]), x1 = real(r.o[2 * w][nt][j + 2]);
                 const float x2 = real(r.o[2 * w + 1][nt][j]), x3 = real(r.o[2 * w + 1][nt][j + 2]);
                 const int d = Geo<D>::v_dim(w, g);
@@ -777,10 +811,10 @@ cache_attention_cluster_kernel(const __grid_constant__ AttnArgs a)
                     for (int i = 0; i < D / 32; i++) {
                         float4 *at = reinterpret_cast<float4 *>(&s_o[nt * 8 + 2 * c + j][Geo<D>::v_dim(i, g)]);
                         float4 v = w == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *at;
-                        v.x = fmaf(fmaf(r.o[2 * i][nt][j], CODE, -zp[nt][j]), k, v.x);
-                        v.y = fmaf(fmaf(r.o[2 * i][nt][j + 2], CODE, -zp[nt][j]), k, v.y);
-                        v.z = fmaf(fmaf(r.o[2 * i + 1][nt][j], CODE, -zp[nt][j]), k, v.z);
-                        v.w = fmaf(fmaf(r.o[2 * i + 1][nt][j + 2], CODE, -zp[nt][j]), k, v.w);
+                        v.x = fmaf(sum_of(r.o[2 * i][nt][j], zp[nt][j]), k, v.x);
+                        v.y = fmaf(sum_of(r.o[2 * i][nt][j + 2], zp[nt][j]), k, v.y);
+                        v.z = fmaf(sum_of(r.o[2 * i + 1][nt][j], zp[nt][j]), k, v.z);
+                        v.w = fmaf(sum_of(r.o[2 * i + 1][nt][j + 2], zp[nt][j]), k, v.w);
                         *at = v;
                     }
                 }

@@ -461,6 +461,23 @@ def test_prompt_attention_captured_and_on_two_streams(cuda):
     cache.check()
 
 
+@pytest.mark.parametrize("spans,heads,group,head_dim", [([(742, 1364), (300, 900)], 4, 1, 64), ([(1, 2293), (1, 73)], 8, 8, 96), ([(1, 3000)] * 9, 1, 7, 256),
+                                                        ([(25, 2123)], 2, 12, 128)])
+def test_attention_of_float_queries_is_float(cuda, spans, heads, group, head_dim):
+    """Error of the whole result, in the 2-norm.  Per probability: 2^-22 each for its two halves and its exponential; its score, of a few
+    units, some 2^-24 of itself from each sum of 16 products and of those sums: below 2^-20 together, and independent from key
+    to key, which the norm of a sum of them does not enlarge."""
+    import ltq
+    torch = cuda
+    b = batch(torch, 18, spans, 32)
+    cache = random_cache(torch, ltq, 18, b["blocks"], heads, 32, head_dim)
+    q = torch.randn(b["tokens"], heads * group, head_dim, generator=torch.Generator().manual_seed(18)).cuda()
+    scale = 1.0 / float(cache.values()[0].std() * head_dim ** 0.5)
+    got = cache.attention(q, ints(torch, b["table"]), ints(torch, b["lengths"]), ints(torch, b["offsets"]), b["max_new"], scale=scale)
+    want, _ = attention_want(torch, cache, q, b, float(np.float32(scale)))
+    assert (got.double() - want).norm() < 2.0 ** -20 * want.norm()
+
+
 def test_attention_workspace(cuda):
     """None is needed for a short call, and none may be too small for a long one."""
     import ltq
