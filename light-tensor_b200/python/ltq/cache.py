@@ -108,7 +108,7 @@ class KVCache:
         """Keys and values of all slots as numbers: two tensors [blocks, kv_heads, block_tokens, head_dim] of `dtype`."""
         code, shape = _tokens.dtype_code(dtype), self.k.shape
         rows, row, stream = self.blocks * self.kv_heads, self.block_tokens * self.head_dim, _tokens.raw_stream(self._index)
-        out = self.k.new_empty(shape, dtype=dtype), self.k.new_empty(shape, dtype=dtype)
+        out = self.k.new_empty(*shape, dtype=dtype), self.k.new_empty(*shape, dtype=dtype)
         for o, codes, qparams in zip(out, (self.k, self.v), (self.k_qparams, self.v_qparams)) if rows else ():
             check(lib().ltq_dequantize_tokens_u8(o.data_ptr(), code, row, codes.data_ptr(), qparams.data_ptr(), rows, row, self._index, stream))
         return out

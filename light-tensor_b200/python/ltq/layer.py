@@ -113,7 +113,7 @@ class LayerHandle:
         M = x.shape[0]
         out_code = code if dtype is None else _tokens.dtype_code(dtype)
         if out is None:
-            out, ld_out = x.new_empty((M, self.N), dtype=dtype), self.N
+            out, ld_out = x.new_empty(M, self.N, dtype=dtype), self.N
         else:
             out, ld_out = self._tokens_out(out, M, dtype or x.dtype, x.device), out.stride(0) if M > 1 else self.N
         if M:

@@ -50,11 +50,11 @@ def quantize_tokens(x, q=None, qparams=None, sums=None):
     M, K = x.shape
     code, ld = dtype_code(x.dtype), row_stride(x)
     if q is None:
-        q = x.new_empty((M, K), dtype=torch.uint8)
+        q = x.new_empty(M, K, dtype=torch.uint8)
     elif not (q.get_device() == dev and q.dtype is torch.uint8 and q.is_contiguous() and q.shape == x.shape):
         raise ValueError(f"q must be a contiguous uint8 CUDA tensor [{M}, {K}]")
     if qparams is None:
-        qparams = x.new_empty((M, 8), dtype=torch.uint8)
+        qparams = x.new_empty(M, 8, dtype=torch.uint8)
     else:
         check_qparams(qparams, M, dev)
     if sums is None:
@@ -76,7 +76,7 @@ def dequantize_tokens(q, qparams, dtype=torch.float32, out=None):
     check_qparams(qparams, M, dev)
     code = dtype_code(dtype)
     if out is None:
-        out, ld = q.new_empty((M, K), dtype=dtype), K
+        out, ld = q.new_empty(M, K, dtype=dtype), K
     elif not (out.get_device() == dev and out.dtype is dtype and out.shape == q.shape):
         raise ValueError(f"out must be a CUDA tensor [{M}, {K}] of {dtype}")
     else:
