@@ -9,9 +9,7 @@ Operators, all on uint8 codes with (scale, zero point) pairs, value = scale * (c
   attention  Causal attention of the newest tokens of several sequences over that cache.
 """
 import math
-import os
 import random
-import sys
 
 import torch
 
@@ -132,14 +130,6 @@ def _scale_of(p):
     return p.view(torch.float32)[..., 0]
 
 
-def _library():
-    """The library's Python package, which is used from the source tree."""
-    if "ltq" not in sys.modules:
-        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "light-tensor_b200", "python"))
-    import ltq
-    return ltq
-
-
 def prepare(case, seed):
     g = _generator(seed)
     dtype = DTYPES[case["dtype"]]
@@ -153,7 +143,10 @@ def prepare(case, seed):
             s["w_pairs"] = _pairs(0.0004 * torch.exp(0.3 * _randn(g, n)), zero)
             s["bias"] = _randn(g, n) if case["bias"] else None
             if own:
-                s["layer"] = _library().FullyConnected_t(s["w"], s["w_pairs"], s["bias"])
+                import sys
+                sys.path.insert(0, "light-tensor_b200/python") if "light-tensor_b200/python" not in sys.path else None
+                import ltq
+                s["layer"] = ltq.FullyConnected_t(s["w"], s["w_pairs"], s["bias"])
         return s
     spans = _ragged(case)
     per = [-(-length // case["block"]) for _, length in spans]
@@ -187,7 +180,10 @@ def prepare(case, seed):
     else:
         s["q"] = _randn(g, total, case["q_heads"], case["head_dim"]).to(dtype)
     if own:
-        s["cache"] = _library().KVCache(s["k"], s["k_pairs"], s["v"], s["v_pairs"])
+        import sys
+        sys.path.insert(0, "light-tensor_b200/python") if "light-tensor_b200/python" not in sys.path else None
+        import ltq
+        s["cache"] = ltq.KVCache(s["k"], s["k_pairs"], s["v"], s["v_pairs"])
     return s
 
 
@@ -280,8 +276,8 @@ def run(state):
     case = state["case"]
     op = case["op"]
     if own:
+        import ltq
         if op == "tokens":
-            ltq = _library()
             codes, pairs, _ = ltq.quantize_tokens(state["x"])
             return {"values": ltq.dequantize_tokens(codes, pairs, state["x"].dtype), "scale": _scale_of(pairs), "zero": pairs[:, 4]}
         if op == "linear":
