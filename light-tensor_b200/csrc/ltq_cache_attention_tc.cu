@@ -218,7 +218,6 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
     using G = TcGeo<D>;
     using TilePar = typename G::TilePar;
     constexpr uint32_t RT = G::RT, SB = G::SB;
-    griddep_launch_dependents();
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), sq = (raw + 1023u) & ~1023u;
     const uint32_t sk = sq + RT * G::Q_BYTES, sv = sk + 2 * G::K_BYTES;
@@ -262,6 +261,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
     if (warp == 0) {
         tmem_alloc(smem_u32(s_misc), 512);
         tmem_relinquish();
+        griddep_launch_dependents();   // not before: see there
     }
     tc_fence_before();
     __syncthreads();

@@ -194,7 +194,6 @@ __global__ void __launch_bounds__(THREADS, 1)
 conv_direct_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const DirectGeom g,
                    const Epilogue epi, void *__restrict__ out, uint32_t *status, const uint8_t *__restrict__ x_nchw)
 {
-    griddep_launch_dependents();
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw0 = smem_u32(smem_raw);
     const uint32_t ring = (raw0 + 1023u) & ~1023u;                             // [stages][planes][rows_box][P pixels][64 B]
@@ -232,6 +231,7 @@ conv_direct_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     if (warp == 1) {
         tmem_alloc(smem_u32(s_misc), TMEM_COLS);
         tmem_relinquish();
+        griddep_launch_dependents();   // not before: see there
     }
     // Where every kernel tap's window starts inside a stage: its plane's slot, then (dy * P + dx) pixel slots further on
     // (dy, dx counted from the region's first row and column).  Tabulated once: the MMA-issuing thread is the kernel's

@@ -79,7 +79,6 @@ gemm_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                   uint32_t bn, uint32_t split, uint32_t lines, uint32_t a_rows, uint32_t stages, uint32_t ring_bytes, Epilogue epi, void *__restrict__ out, uint32_t *status)
 {
     constexpr int DT = OUT - OUT_TOKENS;
-    griddep_launch_dependents();
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), ring = (raw + 1023u) & ~1023u, slice = bn / split;
     const uint32_t a_bytes = lines * a_rows * SM_BK, b_bytes = lines * bn * SM_BK, stage_bytes = a_bytes + b_bytes;
@@ -130,6 +129,7 @@ gemm_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     if (warp == 0) {
         tmem_alloc(smem_u32(s_misc), SM_ACC * SM_MAX_BN);
         tmem_relinquish();
+        griddep_launch_dependents();   // not before: see there
     }
     tc_fence_before();
     __syncthreads();

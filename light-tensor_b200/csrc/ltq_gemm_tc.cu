@@ -51,7 +51,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, uint32_t M,
                uint32_t N, uint32_t K, Epilogue epi, void *__restrict__ out, uint32_t *status)
 {
-    griddep_launch_dependents();
     using C = Cfg<BN>;
     extern __shared__ uint8_t smem_raw[];
     // 128B-swizzled tiles need a 1024-byte aligned base.
@@ -87,6 +86,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     if (warp == 1) {
         tmem_alloc(smem_u32(s_misc), C::TMEM_COLS);
         tmem_relinquish();
+        griddep_launch_dependents();   // not before: see there
     }
     tc_fence_before();
     __syncthreads();
@@ -286,7 +286,6 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     const __grid_constant__ CUtensorMap map_b3, const PairTiling tl, uint32_t M, uint32_t N, uint32_t K,
                     uint32_t stages, Epilogue epi, void *__restrict__ out, uint32_t *status)
 {
-    griddep_launch_dependents();
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;
@@ -329,6 +328,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     if (warp == 1) {
         tmem_alloc_pair(smem_u32(s_misc), 512);
         tmem_relinquish_pair();
+        griddep_launch_dependents();   // not before: see there
     }
     tc_fence_before();
     __syncthreads();

@@ -134,7 +134,6 @@ gemv_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
 {
     // By every thread, first thing: the CTA counts as released once all of them have said so, and the next launch's CTAs
     // should move in (and start fetching their weights) as early as they can.
-    griddep_launch_dependents();
     if (threadIdx.x == 0) {  // the first tensor copy waits for its descriptor: have all three on their way at once
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w_hi) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w_lo) : "memory");
@@ -233,6 +232,7 @@ gemv_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
     if (warp == 1) {
         tmem_alloc(smem_u32(misc), TMEM_COLS);
         tmem_relinquish();
+        griddep_launch_dependents();   // not before: see there
     }
     tc_fence_before();
     __syncthreads();

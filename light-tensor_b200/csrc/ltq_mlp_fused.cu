@@ -160,7 +160,6 @@ mlp_fused_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant
                  const __grid_constant__ CUtensorMap map2, const __grid_constant__ CUtensorMap map3, const MlpParams P,
                  const float *__restrict__ x, uint32_t M, float in_scale, float in_zpf, void *__restrict__ out, uint32_t *status)
 {
-    griddep_launch_dependents();
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -202,6 +201,7 @@ mlp_fused_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant
     if (warp == 2) {
         tmem_alloc(smem_u32(misc), P.tmem_cols);
         tmem_relinquish();
+        griddep_launch_dependents();   // not before: see there
     }
     tc_fence_before();
     __syncthreads();

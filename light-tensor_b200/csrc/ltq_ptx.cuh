@@ -90,7 +90,9 @@ __device__ __forceinline__ bool elect_one()
 // Programmatic dependent launch.  griddep_wait: returns once every kernel this grid programmatically depends on has
 // completed and its writes are visible (at once when the grid was launched without such a dependency).
 // griddep_launch_dependents: this CTA no longer holds back the launch of the next kernel in the stream; that kernel
-// starts when every CTA of this grid has said so or exited.
+// starts when every CTA of this grid has said so or exited.  One thread's word counts for its CTA.
+// A kernel that allocates tensor memory says so only once it has it.  Otherwise a CTA of the next kernel could come to the same SM,
+// take the columns first and then wait for this kernel's end, which waits for the columns: neither would ever go on.
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void griddep_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
