@@ -29,9 +29,13 @@
 //    the probabilities then; the tensor core cuts off what does not fit a sum, always towards zero, so with float q the zero
 //    points come off the codes first, exact in halves, and every product starts from zero and is added up in float: 742
 //    new tokens of 1364 were off by 1.6e-5 otherwise, now by 3e-7);
-//  * V's block scales go into the probabilities as a ratio to the largest one so far, so that one accumulator serves all;
-//  * the running maximum is kept only approximately: the reference m moves when a score exceeds it by more than 8 (base 2), so
-//    that probabilities stay below 2^8 and almost every step does without a reduction over lanes.
+//  * V's block scales go into the probabilities, so that one accumulator serves all.  What halves have to hold is then the weight
+//    exp2(score) * V scale, and its reference is the row's own: m + d, with m the reference of the scores (and of the sum of the
+//    probabilities) and 2^d what V's scale adds to the largest weight.  (With the largest V scale in sight as the reference, one
+//    loud block that a row gives no weight took the bits of all others: 2^22 times louder, outputs were 2 % off and more.)
+//  * both references are kept only approximately: they move when a score exceeds m, or a weight m + d, by more than 8 (base 2), so
+//    that almost every step does without a reduction over lanes.  A weight at its reference is 2^7: halves end at 2^16, and
+//    what they lose below 2^-14 lies further from the largest.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -45,9 +49,12 @@ namespace {
 constexpr int DT = LTQ_ATTN_DT;
 constexpr int TERMS = DT == LTQ_F32 ? 2 : 1;
 constexpr int WARPS = ATTN_WARPS;
-constexpr float SMALLEST_SCALE = 1.17549435e-38f;   // 2^-126
 constexpr uint32_t AHEAD = 2;     // steps beyond the one on its way into registers that are asked into L2
-constexpr float MAX_STEP = 8.f;   // how far a score may exceed the reference maximum before it moves
+constexpr float MAX_STEP = 8.f;   // how far a score or a weight may exceed its reference before that moves
+constexpr int HEAD = 7;           // a weight at its reference is 2^HEAD: with MAX_STEP above it still a half
+constexpr float LARGE = 180.f;    // factors up to this, 2^(HEAD + 0.49), need no look at the weights
+constexpr float QUIET = -118.f;   // V scales below 2^this do not lower the reference further, so that 2^(HEAD - d) stays a float
+constexpr float LOUD = 1.2676506e30f;   // 2^100: no weight's factor is larger (probabilities that reach it are below 2^-85)
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 __device__ __forceinline__ uint32_t pack2(float lo, float hi)
@@ -74,6 +81,14 @@ __device__ __forceinline__ float exp2_fast(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float log2_fast(float x)
+{
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float power2(int e) { return __int_as_float((127 + e) << 23); }        // 2^e, -126 <= e <= 127
+__device__ __forceinline__ int exponent_of(float p) { return (__float_as_int(p) >> 23) - 127; }   // of a power of two
 
 template <int D>
 struct Geo {
@@ -194,9 +209,9 @@ struct Rows {
     int pos[NT][2];                     // position of those rows' tokens (rows that do not exist see everything, with q = 0)
     int first_pos;                      // the smallest of the warp's
     float m[NT][2], l[NT][2];
-    float o[D / 16][NT][4];             // 2^-24 * sum of probability * V scale / v_ref * code (float q: of code - zero point, as it is)
-    float zp[NT][2];                    // sum of probability * V scale / v_ref * zero point (float q: 0)
-    float v_ref, v_inv;                 // largest V scale so far and its inverse
+    float o[D / 16][NT][4];             // 2^-24 * sum of weight * code (float q: of weight * (code - zero point), as it is)
+    float zp[NT][2];                    // sum of weight * zero point (float q: 0)
+    float g[NT][2];                     // 2^(HEAD - d): weight = probability * V scale * g
 };
 constexpr float CODE = 16777216.f;      // 2^24: a code's half is the code over this
 constexpr bool EXACT = TERMS == 2;      // codes as the halves code - zero point instead, see above
@@ -289,6 +304,7 @@ __device__ __forceinline__ void load_rows(Rows<D, NT> &r, const AttnArgs &a, con
             r.scale[nt][j] = __shfl_sync(0xFFFFFFFFu, sc, (2 * c + j) * 4);
             r.q_sum[nt][j] = __shfl_sync(0xFFFFFFFFu, sum, (2 * c + j) * 4);
             r.zp[nt][j] = 0.f;
+            r.g[nt][j] = power2(HEAD);
             r.pos[nt][j] = __shfl_sync(0xFFFFFFFFu, pos, (2 * c + j) * 4);
             r.m[nt][j] = -INFINITY;
             r.l[nt][j] = 0.f;
@@ -304,8 +320,6 @@ __device__ __forceinline__ void load_rows(Rows<D, NT> &r, const AttnArgs &a, con
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) first = min(first, min(r.pos[nt][0], r.pos[nt][1]));
     r.first_pos = __reduce_min_sync(0xFFFFFFFFu, first);
-    r.v_ref = SMALLEST_SCALE;
-    r.v_inv = 1.f / SMALLEST_SCALE;
 }
 
 // Scores, softmax and accumulation for 16 keys, the first at position key0.
@@ -365,11 +379,32 @@ __device__ __forceinline__ void take_keys(Rows<D, NT> &r, const Keys<D> &keys, i
                 if (bad || key0 + g + 8 * (j >> 1) > r.pos[nt][j & 1]) x[nt][j] = -INFINITY;
     };
     if (masked) mask(t);
+    // what makes a probability of a row a weight
+    float f[NT][2];
+    auto factors = [&]() {
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) f[nt][j] = fminf(v_scale * r.g[nt][j], LOUD);
+    };
+    factors();
+    float loudest = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
         for (int j = 0; j < 4; j++) top = fmaxf(top, t[nt][j]);
-    if (__any_sync(0xFFFFFFFFu, top > MAX_STEP)) {   // (also the first time: m is -inf, t +inf)
+        loudest = fmaxf(loudest, fmaxf(f[nt][0], f[nt][1]));
+    }
+    bool move = __any_sync(0xFFFFFFFFu, top > MAX_STEP || loudest > LARGE);   // (also the first time: m is -inf, t +inf)
+    if (move && __all_sync(0xFFFFFFFFu, top <= MAX_STEP)) {   // a block louder than what a row's reference stands on: do its weights reach the limit?
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) top = fmaxf(top, fmaxf(t[nt][j], t[nt][j + 2]) + (log2_fast(f[nt][j]) - (float)HEAD));
+        move = __any_sync(0xFFFFFFFFu, top > MAX_STEP);
+    }
+    if (move) {
+        const float v_log = fminf(fmaxf(log2_fast(v_scale), QUIET), 128.f);   // (NaN: QUIET)
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -379,39 +414,29 @@ __device__ __forceinline__ void take_keys(Rows<D, NT> &r, const Keys<D> &keys, i
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                float mx = fmaxf(t[nt][j], t[nt][j + 2]);
+                float here = fmaxf(t[nt][j], t[nt][j + 2]);
 #pragma unroll
-                for (int o = 4; o <= 16; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-                mx = fmaxf(mx, r.m[nt][j]);
-                const float alpha = r.m[nt][j] == mx ? 1.f : exp2_fast(r.m[nt][j] - mx);   // (both -inf: nothing there yet)
+                for (int o = 4; o <= 16; o <<= 1) here = fmaxf(here, __shfl_xor_sync(0xFFFFFFFFu, here, o));
+                const float mx = fmaxf(here, r.m[nt][j]), down = r.m[nt][j] == mx ? 0.f : r.m[nt][j] - mx;   // (both -inf: nothing there yet)
                 const float m = mx == -INFINITY ? 0.f : mx;
+                const int d = HEAD - exponent_of(r.g[nt][j]);
+                int d_new = d;
+                if (mx != -INFINITY) d_new = (int)ceilf(fmaxf(down + (float)d, here - mx + v_log));
+                const float alpha = exp2_fast(down), beta = exp2_fast(down + (float)(d - d_new));
                 t[nt][j] -= m;
                 t[nt][j + 2] -= m;
                 r.m[nt][j] = mx;
                 r.l[nt][j] *= alpha;
-                r.zp[nt][j] *= alpha;
+                r.g[nt][j] = power2(HEAD - d_new);
+                r.zp[nt][j] *= beta;
 #pragma unroll
                 for (int i = 0; i < D / 16; i++) {
-                    r.o[i][nt][j] *= alpha;
-                    r.o[i][nt][j + 2] *= alpha;
+                    r.o[i][nt][j] *= beta;
+                    r.o[i][nt][j + 2] *= beta;
                 }
             }
+        factors();
     }
-    if (v_scale > r.v_ref) {   // the same in all lanes
-        const float f = r.v_ref * __fdividef(1.f, v_scale);
-        r.v_ref = v_scale;
-        r.v_inv = __fdiv_rn(1.f, v_scale);
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-            for (int j = 0; j < 2; j++) r.zp[nt][j] *= f;
-#pragma unroll
-            for (int i = 0; i < D / 16; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) r.o[i][nt][j] *= f;
-        }
-    }
-    const float ratio = v_scale * r.v_inv;
     uint32_t p[TERMS][NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -420,10 +445,10 @@ __device__ __forceinline__ void take_keys(Rows<D, NT> &r, const Keys<D> &keys, i
             t[nt][j] = exp2_fast(t[nt][j]);
             r.l[nt][j & 1] += t[nt][j];
         }
-        float f0 = ratio, f1 = ratio;
-        if (ratio != ratio) {   // a block whose scale is NaN must not reach rows that see none of its keys (0 * NaN)
-            f0 = key0 <= r.pos[nt][0] && !bad ? ratio : 0.f;
-            f1 = key0 <= r.pos[nt][1] && !bad ? ratio : 0.f;
+        float f0 = f[nt][0], f1 = f[nt][1];
+        if (!(v_scale < INFINITY)) {   // a block whose scale is NaN reaches the rows that see one of its keys, and no others (0 * NaN)
+            f0 = key0 <= r.pos[nt][0] && !bad ? __int_as_float(0x7FC00000) : 0.f;
+            f1 = key0 <= r.pos[nt][1] && !bad ? __int_as_float(0x7FC00000) : 0.f;
         }
 #pragma unroll
         for (int i = 0; i < 2; i++) {
@@ -571,10 +596,11 @@ __device__ __forceinline__ void do_segment(const AttnArgs &a, uint32_t b, const 
             const uint32_t t = row / a.group;
             const uint64_t out_row = ((uint64_t)s.off + t) * a.q_heads + h * a.group + (row - t * a.group);
             const uint64_t place = (uint64_t)slot * 8 * NT + rr;
-            const float f = whole ? (l == 0.f ? 0.f : __fdiv_rn(r.v_ref, l)) : r.v_ref;   // (a row that sees nothing: zeros)
+            const float f = whole ? (l == 0.f ? 0.f : __fdiv_rn(1.f, l)) : 1.f;   // (a row that sees nothing: zeros)
+            const float back = power2(-exponent_of(r.g[nt][j]));
 #pragma unroll
             for (int w = 0; w < D / 32; w++) {
-                auto real = [&](float x) { return sum_of(x, zp) * f; };
+                auto real = [&](float x) { return sum_of(x, zp) * f * back; };
                 const float x0 = real(r.o[2 * w][nt][j]), x1 = real(r.o[2 * w][nt][j + 2]);
                 const float x2 = real(r.o[2 * w + 1][nt][j]), x3 = real(r.o[2 * w + 1][nt][j + 2]);
                 const int d = Geo<D>::v_dim(w, g);
@@ -806,7 +832,7 @@ cache_attention_cluster_kernel(const __grid_constant__ AttnArgs a)
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    const float k = f[nt][j] * r.v_ref;
+                    const float k = f[nt][j] * power2(-exponent_of(r.g[nt][j]));
 #pragma unroll
                     for (int i = 0; i < D / 32; i++) {
                         float4 *at = reinterpret_cast<float4 *>(&s_o[nt * 8 + 2 * c + j][Geo<D>::v_dim(i, g)]);

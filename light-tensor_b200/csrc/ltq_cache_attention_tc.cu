@@ -14,13 +14,13 @@
 //                dealt so that loads and stores spread over the banks.
 //   MMA issue    one warp per row tile, so that each goes its own way: S of a tile goes out before O of the one in front.
 //   softmax      two warpgroups per row tile take the tiles in turn, one per S buffer: thread = row = TMEM lane, so that no reduction
-//                crosses threads.  The reference maximum m moves only when a tile's probabilities add up to more than 2^12,
-//                O is hardly ever rescaled and no maximum is taken on the way.  m is an integer: what two tiles in a row, which
+//                crosses threads.  The reference m moves only when a tile's weights add up to more than 2^15, from 2^3 for the
+//                largest, O is hardly ever rescaled and no maximum is taken on the way.  m is an integer: what two tiles in a row, which
 //                two warps have at the same time, have to agree on is a power of two.  A tile with masked keys or a new
 //                maximum goes a careful way of its own, from the scores that are still in tensor memory.
 //   parameters   one warp: the scales and zero points of every 16 keys.
 //
-// Measured on 1500 and 1109 new tokens behind up to 4500, 32 query and 8 key/value heads of 128 (232 us, 109 us at the tensor cores'
+// Measured on 1500 and 1109 new tokens behind up to 4500, 32 query and 8 key/value heads of 128 (230 us, 109 us at the tensor cores'
 // measured rate).  A tile takes about 2000 cycles; its MMAs take 1300 of them (48 each for S, where Q's 4 KB per 16 of D come
 // through the shared memory port, 64 for O; nothing else slows them down, but every access to tensor memory waits about 90
 // cycles for a gap between them, whatever its width), its exponentials 1024, its instructions about 1400 issue slots.
@@ -31,9 +31,12 @@
 //  * the tiles divided evenly over persistent CTAs, with a join: 289 us (each piece of a group costs about 15 000 cycles)
 // The warps' registers are divided by need (setmaxnreg).
 //
-// Scales: K's block scale multiplies the scores, V's goes into the exponent as log2 of its ratio to a reference (at least twice
-// the largest so far, per CTA), the sum of probabilities takes it out again per 16 keys.  q is scaled by a power of two per
-// row, so that halves hold it exactly or to 11 bits (half, bfloat16 queries).
+// Scales: K's block scale multiplies the scores.  V's goes into the exponent as its logarithm, so that P holds weights, exp2(score) * V
+// scale, and m is the reference of a row's own weights (with the largest V scale in sight as the reference, one loud block that a
+// row gives no weight took the bits of all others: 2^22 times louder, outputs were 2 % off and more).  The sum of the probabilities
+// is the sum of the weights of every 16 keys over their V scale, under the same reference; where a tile's V scales are so
+// far below the loudest that such a weight could vanish and its probability not, the careful way takes the probabilities themselves.
+// q is scaled by a power of two per row, so that halves hold it exactly or to 11 bits (half, bfloat16 queries).
 //
 // Every wait is bounded, see mbar_wait.
 #include <cuda_fp16.h>
@@ -47,15 +50,18 @@ namespace ltq {
 namespace {
 
 constexpr int TC_ROWS = 128;
-constexpr float TC_MAX_SUM = 4096.f;
+constexpr float TC_MAX_SUM = 32768.f;   // a weight is below it, and a half
+constexpr float TC_HEAD = 3.f;          // a row's largest weight is 2^(TC_HEAD - 1) to 2^TC_HEAD when the reference is taken from it
 constexpr float TC_SMALLEST = 1.17549435e-38f;   // 2^-126
-constexpr float TC_MIN_RATIO = 8.6736174e-19f;   // 2^-60: a V scale below the reference by more than this adds nothing
+// Weights down to 2^-126 are floats.  The sum of probabilities is taken from them where no V scale of a tile is below the loudest
+// so far by more than 2^TC_SPREAD (what is lost then is below 2^-30 of the sum) or below 2^TC_QUIET (its inverse, 2^15 times and more,
+// has to be a float); a V scale below that one does not lower the reference further.
+constexpr float TC_SPREAD = 96.f, TC_QUIET = -100.f;
 constexpr float TC_CODE = 16777216.f;            // 2^24: a K code's half is the code over this
 
-// What the softmax needs of 16 keys: K scale times 2^24, K scale times zero point, log2 of the V scale's ratio to the reference and
-// the ratio's inverse.
+// What the softmax needs of 16 keys: K scale times 2^24, K scale times zero point, log2 of the V scale and 2^-that.
 struct GroupPar {
-    float ks, kzs, lr, inv;
+    float ks, kzs, lv, inv;
 };
 
 template <int D>
@@ -82,8 +88,8 @@ struct TcGeo {
     static constexpr int BARS = 9 + RT * 3 * SB + SW * 4 + 2 * RAW;   // k_full k_empty v_full v_empty q_full; s_full p_full pv_done; m_done; raw_full raw_empty
     struct TilePar {
         GroupPar g[GROUPS];
-        float v_ref, rescale;   // the reference, and what O so far has to be multiplied with for it
-        uint32_t bad, pad;      // bit i: group i's block does not exist
+        uint32_t bad, wide;     // bit i: group i's block does not exist; 1: V scales too far below the loudest for the common way
+        uint32_t pad[2];
     };
     static constexpr size_t SMEM = 1024 + RT * Q_BYTES + 2 * K_BYTES + 2 * V_BYTES + RAW * RAW_BYTES + 8 * sizeof(TilePar) + SW * TC_ROWS * 4 + (BARS + BARS % 2) * 8 + RAW * 16 + 16;
     static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -143,6 +149,10 @@ __device__ __forceinline__ float ex2(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ float times2(float x, float e)   // x * 2^e, where 2^e alone may not be a float
+{
+    return x * ex2(0.5f * e) * ex2(0.5f * e);
 }
 __device__ __forceinline__ float lg2(float x)
 {
@@ -405,9 +415,9 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             auto last_seen = [&](int k) { return par.bad >> k & 1 ? -1 : pos - key0 - 16 * k; };   // the last key of group k that the row sees
             uint32_t p[G::KEYS / 2];
             // The common way: everything is seen, and the reference stays.  Else the careful way, from the scores as they still are.
-            bool careful = par.bad || key0 + G::KEYS - 1 > first_pos;
+            bool careful = par.bad || par.wide || key0 + G::KEYS - 1 > first_pos;
             if (!careful) {
-                float sum = 0.f;
+                float sum = 0.f, weight = 0.f;
 #pragma unroll
                 for (int c = 0; c < G::KEYS / 32; c++) {   // 32 keys at a time
                     uint32_t x[32];
@@ -418,7 +428,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                     tmem_ld_wait();
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
-                        const float ks = row_scale * g[k].ks, base = g[k].lr - fmaf(zero_scale, g[k].kzs, m);
+                        const float ks = row_scale * g[k].ks, base = g[k].lv - fmaf(zero_scale, g[k].kzs, m);
                         const uint64_t ks2 = pair(ks, ks), base2 = pair(base, base);
                         float2 y[8];
 #pragma unroll
@@ -433,26 +443,27 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                             p[16 * c + 8 * k + i] = h2pack(y[i].x, y[i].y);
                         }
                         const float2 s2 = unpair(add2(add[0], add[1]));
+                        weight += s2.x + s2.y;
                         sum = fmaf(s2.x + s2.y, g[k].inv, sum);
                     }
                 }
-                careful = __any_sync(0xFFFFFFFFu, sum > TC_MAX_SUM);   // (with m at -inf everything is inf, and so is the sum)
+                careful = __any_sync(0xFFFFFFFFu, weight > TC_MAX_SUM);   // (with m at -inf everything is inf, and so is the sum)
                 if (!careful) l += sum;
             }
-            if (careful) {   // the maximum first
+            if (careful) {   // the largest weight first
                 float best = -INFINITY;
 #pragma unroll 1
                 for (int k = 0; k < G::GROUPS; k++) {
                     uint32_t x[16];
                     tmem_ld16(s_addr + 16 * k, x);
-                    const float ks = row_scale * par.g[k].ks, base = -zero_scale * par.g[k].kzs;
+                    const float ks = row_scale * par.g[k].ks, base = fmaxf(par.g[k].lv, TC_QUIET) - zero_scale * par.g[k].kzs;
                     const int see = last_seen(k);
                     tmem_ld_wait();
 #pragma unroll
                     for (int i = 0; i < 16; i++) best = i > see ? best : fmaxf(best, fmaf(__uint_as_float(x[i]), ks, base));
                 }
-                const float mx = fmaxf(m, ceilf(best));
-                if (m != mx) l *= ex2(m - mx);
+                const float mx = fmaxf(m, ceilf(best) - TC_HEAD);
+                if (m != mx) l = times2(l, m - mx);
                 m = mx;
             }
             // The tile in front has its reference by now: the larger one holds for both.
@@ -463,14 +474,14 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                 const float before = s_m[(wg ^ 1) * TC_ROWS + r], mx = fmaxf(m, before);
                 if (__any_sync(0xFFFFFFFFu, m < before)) {
                     const float down = m == mx ? 1.f : ex2(m - mx);
-                    l *= down;
+                    if (m != mx) l = times2(l, m - mx);
                     if (!careful) {
                         const __half2 by = __float2half2_rn(down);   // a power of two
 #pragma unroll
                         for (int i = 0; i < G::KEYS / 2; i++) *reinterpret_cast<__half2 *>(&p[i]) = __hmul2(*reinterpret_cast<__half2 *>(&p[i]), by);
                     }
                 }
-                alpha = before != mx ? par.rescale * ex2(before - mx) : par.rescale;
+                if (before != mx) alpha = ex2(before - mx);
                 m = mx;
             }
             s_m[wg * TC_ROWS + r] = m;
@@ -500,7 +511,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                     uint32_t x[16], w[8];
                     tmem_ld16(s_addr + 16 * k, x);
                     const GroupPar g = par.g[k];
-                    const float ks = row_scale * g.ks, base = g.lr - fmaf(zero_scale, g.kzs, ref);
+                    const float ks = row_scale * g.ks, score = -fmaf(zero_scale, g.kzs, ref), base = g.lv + score;
                     const int see = last_seen(k);
                     float sum = 0.f;
                     tmem_ld_wait();
@@ -511,7 +522,12 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                         sum += y0 + y1;
                         w[i] = h2pack(y0, y1);
                     }
-                    l = fmaf(sum, g.inv, l);
+                    if (!par.wide) {
+                        l = fmaf(sum, g.inv, l);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; i++) l += i > see ? 0.f : ex2(fmaf(__uint_as_float(x[i]), ks, score));
+                    }
                     tmem_st8(s_addr + 8 * k, w);
                 }
             }
@@ -521,18 +537,16 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             if (lane == 0) mbar_arrive(p_bar);
         }
         // The last tile's reference holds for all.
-        float v_ref = 1.f;
         if (ok && mine > 0) {
             const uint32_t last = mine - 1, lb = last % SB, ph = (last / SB) & 1;
             if (lb != sb) {
                 ok = __all_sync(0xFFFFFFFFu, mbar_wait(m_other, ph, abort_flag, status, 0xB20u | sb));
                 const float mx = s_m[(wg ^ 1) * TC_ROWS + r];
-                if (m != mx) l *= ex2(m - mx);
+                if (m != mx) l = times2(l, m - mx);
                 m = mx;
             }
             ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(pv_bar + 8 * lb, ph, abort_flag, status, 0xB28u | sb));
             tc_fence_after();
-            v_ref = s_par[last & 7].v_ref;
         }
         meet();
         s_m[wg * TC_ROWS + r] = l;
@@ -540,8 +554,11 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
         l += s_m[(wg ^ 1) * TC_ROWS + r];
         // this warpgroup's half of the head dimensions
         if (ok && a.splits > 1) {
+            // the join works on sums near 1: their exponent goes into the reference, and off O
             const uint64_t at = (uint64_t)(place + split) * (TC_ROWS * RT) + rt * TC_ROWS + r;
-            if (real && sb == 0) a.part_ml[at] = make_float2(m, l);
+            const int e = (int)((__float_as_uint(l) >> 23) & 0xFF) - 127, el = e < -126 ? -126 : (e > 126 ? 126 : e);
+            const float back = __uint_as_float((uint32_t)(127 - el) << 23);
+            if (real && sb == 0) a.part_ml[at] = make_float2(m + (float)el, l * back);
             float4 *dst = reinterpret_cast<float4 *>(a.part_o + at * D);
 #pragma unroll 1
             for (int d = sb * (D / 2); d < (int)(sb + 1) * (D / 2); d += 16) {
@@ -553,12 +570,12 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
                     if (real)
-                        dst[d / 4 + i] = mine > 0 ? make_float4(__uint_as_float(o[4 * i]) * v_ref, __uint_as_float(o[4 * i + 1]) * v_ref,
-                                                                __uint_as_float(o[4 * i + 2]) * v_ref, __uint_as_float(o[4 * i + 3]) * v_ref)
+                        dst[d / 4 + i] = mine > 0 ? make_float4(__uint_as_float(o[4 * i]) * back, __uint_as_float(o[4 * i + 1]) * back,
+                                                                __uint_as_float(o[4 * i + 2]) * back, __uint_as_float(o[4 * i + 3]) * back)
                                                   : make_float4(0.f, 0.f, 0.f, 0.f);
             }
         } else if (ok) {
-            const float inv = l == 0.f ? 0.f : __fdiv_rn(v_ref, l);   // a row that sees nothing: zeros
+            const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);   // a row that sees nothing: zeros
             uint16_t *dst = static_cast<uint16_t *>(a.out) + (((uint64_t)s.off + t) * a.q_heads + h * a.group + (row - t * a.group)) * D;
 #pragma unroll 1
             for (int d = sb * (D / 2); d < (int)(sb + 1) * (D / 2); d += 16) {
@@ -710,7 +727,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                     mbar_wait(raw_full + 8 * (i % G::RAW), i / G::RAW & 1, s_misc + 2, status, 0xB5Cu);
         } else if (rt == 3) {
             // what the softmax needs of every tile: lane i % GROUPS looks after its group i
-            float v_ref = TC_SMALLEST;
+            float loudest = -INFINITY;   // log2 of V's largest scale so far
             auto page_at = [&](uint32_t j) { return page_of(begin + j * G::KEYS + (lane % G::GROUPS) * 16); };
             int32_t page = tiles > 0 ? page_at(0) : 0;
             ltq_qparams kq{};
@@ -729,25 +746,28 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                 const uint32_t st = j & 1;
                 if (!__all_sync(0xFFFFFFFFu, j < 2 || mbar_wait(k_empty + 8 * st, ((j - 2) >> 1) & 1, abort_flag, status, 0xB38u | st))) break;
                 if (bad && lane < G::GROUPS) atomicCAS(status, 0u, STATUS_BAD_BLOCK);
-                float top = vs;   // (NaN is passed over)
+                // log2 of the scale, from its exponent where it has one; an infinity is as good as a NaN
+                const float mantissa = __uint_as_float((__float_as_uint(vs) & 0x7FFFFFu) | 0x3F800000u);
+                float lv = vs < TC_SMALLEST ? lg2(vs) : (float)((int)(__float_as_uint(vs) >> 23) - 127) + lg2(mantissa);
+                if (!(vs < INFINITY)) lv = __int_as_float(0x7FC00000);
+                if (bad) lv = 0.f;   // (nothing of it is seen)
+                float top = bad || lv != lv ? -INFINITY : lv, low = bad || lv != lv ? INFINITY : lv;
 #pragma unroll
-                for (int o = 1; o < G::GROUPS; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-                float rescale = 1.f;
-                if (top > v_ref) {
-                    const float next = top < 1e38f ? 2.f * top : top;
-                    rescale = v_ref * __fdividef(1.f, next);
-                    v_ref = next;
+                for (int o = 1; o < G::GROUPS; o <<= 1) {
+                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+                    low = fminf(low, __shfl_xor_sync(0xFFFFFFFFu, low, o));
                 }
-                const float ratio = __fdiv_rn(vs, v_ref), x = fmaxf(ratio, TC_MIN_RATIO);
-                const bool nan = ratio != ratio;
+                loudest = fmaxf(loudest, top);
                 const uint32_t any = __ballot_sync(0xFFFFFFFFu, bad) & ((1u << G::GROUPS) - 1);
                 TilePar &p = s_par[j & 7];
-                if (lane < G::GROUPS)
-                    p.g[lane] = GroupPar{kq.scale * TC_CODE, kq.scale * (float)kq.zero_point, nan ? ratio : lg2(x), nan ? 1.f : __fdividef(1.f, x)};
+                if (lane < G::GROUPS) {
+                    float inv;   // (as far as lv is rounded it is so on both sides; not flushed to zero, as ex2 would)
+                    asm("ex2.approx.f32 %0, %1;" : "=f"(inv) : "f"(-lv));
+                    p.g[lane] = GroupPar{kq.scale * TC_CODE, kq.scale * (float)kq.zero_point, lv, lv != lv ? 1.f : inv};
+                }
                 if (lane == 0) {
-                    p.v_ref = v_ref;
-                    p.rescale = rescale;
                     p.bad = any;
+                    p.wide = low < fmaxf(loudest - TC_SPREAD, TC_QUIET);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(k_full + 8 * st);
