@@ -23,12 +23,13 @@
 //
 // Past that the kernel is bound by instruction issue, so a step is kept short:
 //  * a code b with a zero byte above it IS a half, the subnormal b * 2^-24, which the tensor core multiplies exactly: one byte
-//    permute per two codes.  Zero points come off the sums: q . (k - z) = q . k - z * sum(q), and p . (v - z) = p . v - z * sum(p)
-//    with p as rounded for the MMA;
+//    permute per two codes of K, whose zero points come off the scores, q . (k - z) = q . k - z * sum(q);
+//  * V's zero points come off the codes first (1024 + code - (1024 + zero point), exact in halves).  The tensor core cuts off what does
+//    not fit a sum, always towards zero: O added up over thousands of steps from positive codes around 128 drifted (256 sequences
+//    of 32 000 keys, half: 1.2e-2 off, now 2.9e-4; with 18 000 steps per warp, all that the device's memory holds, 3.8e-4);
 //  * q is scaled by a power of two per row so that halves hold it (float q: split into two halves, 22 bits, and so are
-//    the probabilities then; the tensor core cuts off what does not fit a sum, always towards zero, so with float q the zero
-//    points come off the codes first, exact in halves, and every product starts from zero and is added up in float: 742
-//    new tokens of 1364 were off by 1.6e-5 otherwise, now by 3e-7);
+//    the probabilities then, K's zero points come off the codes as well, and every product starts from zero and is added up in
+//    float: 742 new tokens of 1364 were off by 1.6e-5 otherwise, now by 3e-7);
 //  * V's block scales go into the probabilities, so that one accumulator serves all.  What halves have to hold is then the weight
 //    exp2(score) * V scale, and its reference is the row's own: m + d, with m the reference of the scores (and of the sum of the
 //    probabilities) and 2^d what V's scale adds to the largest weight.  (With the largest V scale in sight as the reference, one
@@ -209,23 +210,22 @@ struct Rows {
     int pos[NT][2];                     // position of those rows' tokens (rows that do not exist see everything, with q = 0)
     int first_pos;                      // the smallest of the warp's
     float m[NT][2], l[NT][2];
-    float o[D / 16][NT][4];             // 2^-24 * sum of weight * code (float q: of weight * (code - zero point), as it is)
-    float zp[NT][2];                    // sum of weight * zero point (float q: 0)
+    float o[D / 16][NT][4];             // sum of weight * (code - zero point)
     float g[NT][2];                     // 2^(HEAD - d): weight = probability * V scale * g
 };
 constexpr float CODE = 16777216.f;      // 2^24: a code's half is the code over this
-constexpr bool EXACT = TERMS == 2;      // codes as the halves code - zero point instead, see above
+constexpr bool EXACT = TERMS == 2;      // K's codes as the halves code - zero point instead, and sums in float, see above
 
-// Two codes of a word as an operand: bytes `sel` picks of w and, above each, of what makes it a half; `zero`: 1024 + zero point, twice.
+// Two codes of a word as an operand: bytes `sel` picks of w and, above each, of what makes it a half.  OFF: without the zero point (`zero`:
+// 1024 + it, twice).
+template <bool OFF>
 __device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t sel, uint32_t zero)
 {
-    if (!EXACT) return prmt(w, 0, sel);
+    if (!OFF) return prmt(w, 0, sel);
     const uint32_t x = prmt(w, 0x64646464u, sel);   // 1024 + code
     const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&x), *reinterpret_cast<const __half2 *>(&zero));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
-// What the sum `o` of a row says, with its `zp`.
-__device__ __forceinline__ float sum_of(float o, float zp) { return EXACT ? o : fmaf(o, CODE, -zp); }
 
 template <int D, int NT>
 __device__ __forceinline__ void load_rows(Rows<D, NT> &r, const AttnArgs &a, const CacheSeq &s, uint32_t h, uint32_t row0, int g, int c)
@@ -303,7 +303,6 @@ __device__ __forceinline__ void load_rows(Rows<D, NT> &r, const AttnArgs &a, con
         for (int j = 0; j < 2; j++) {   // rows 2c + j live in lanes with g = 2c + j
             r.scale[nt][j] = __shfl_sync(0xFFFFFFFFu, sc, (2 * c + j) * 4);
             r.q_sum[nt][j] = __shfl_sync(0xFFFFFFFFu, sum, (2 * c + j) * 4);
-            r.zp[nt][j] = 0.f;
             r.g[nt][j] = power2(HEAD);
             r.pos[nt][j] = __shfl_sync(0xFFFFFFFFu, pos, (2 * c + j) * 4);
             r.m[nt][j] = -INFINITY;
@@ -327,7 +326,7 @@ template <int D, int NT>
 __device__ __forceinline__ void take_keys(Rows<D, NT> &r, const Keys<D> &keys, int key0, int g)
 {
     const float k_scale = __uint_as_float(keys.k_par.x), v_scale = __uint_as_float(keys.v_par.x);
-    const float k_zero = (float)(keys.k_par.y & 0xFF), v_zero = (float)(keys.v_par.y & 0xFF);
+    const float k_zero = (float)(keys.k_par.y & 0xFF);
     const bool bad = keys.bad;
     const uint32_t k_zero2 = 0x64006400u + (keys.k_par.y & 0xFF) * 0x10001u, v_zero2 = 0x64006400u + (keys.v_par.y & 0xFF) * 0x10001u;
     float acc[NT][2][4];   // two chains: an MMA waits for the one before it on the same accumulator 
@@ -337,8 +336,8 @@ __device__ __forceinline__ void take_keys(Rows<D, NT> &r, const Keys<D> &keys, i
         for (int j = 0; j < 4; j++) acc[nt][0][j] = acc[nt][1][j] = 0.f;
 #pragma unroll
     for (int w = 0; w < D / 16; w++) {
-        const uint32_t a0 = code_pair(keys.k[0][w], 0x4140, k_zero2), a2 = code_pair(keys.k[0][w], 0x4342, k_zero2);
-        const uint32_t a1 = code_pair(keys.k[1][w], 0x4140, k_zero2), a3 = code_pair(keys.k[1][w], 0x4342, k_zero2);
+        const uint32_t a0 = code_pair<EXACT>(keys.k[0][w], 0x4140, k_zero2), a2 = code_pair<EXACT>(keys.k[0][w], 0x4342, k_zero2);
+        const uint32_t a1 = code_pair<EXACT>(keys.k[1][w], 0x4140, k_zero2), a3 = code_pair<EXACT>(keys.k[1][w], 0x4342, k_zero2);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             if (EXACT) {
@@ -428,7 +427,6 @@ __device__ __forceinline__ void take_keys(Rows<D, NT> &r, const Keys<D> &keys, i
                 r.m[nt][j] = mx;
                 r.l[nt][j] *= alpha;
                 r.g[nt][j] = power2(HEAD - d_new);
-                r.zp[nt][j] *= beta;
 #pragma unroll
                 for (int i = 0; i < D / 16; i++) {
                     r.o[i][nt][j] *= beta;
@@ -454,18 +452,10 @@ __device__ __forceinline__ void take_keys(Rows<D, NT> &r, const Keys<D> &keys, i
         for (int i = 0; i < 2; i++) {
             const float x = t[nt][2 * i] * f0, y = t[nt][2 * i + 1] * f1;
             const uint32_t hi = pack2(x, y);
-            float2 b = unpack2(hi);
             p[0][nt][i] = movmatrix(hi);
             if (TERMS == 2) {
-                const uint32_t lo = pack2(x - b.x, y - b.y);
-                const float2 d = unpack2(lo);
-                p[TERMS - 1][nt][i] = movmatrix(lo);
-                b.x += d.x;
-                b.y += d.y;
-            }
-            if (!EXACT) {
-                r.zp[nt][0] = fmaf(v_zero, b.x, r.zp[nt][0]);
-                r.zp[nt][1] = fmaf(v_zero, b.y, r.zp[nt][1]);
+                const float2 b = unpack2(hi);
+                p[TERMS - 1][nt][i] = movmatrix(pack2(x - b.x, y - b.y));
             }
         }
     }
@@ -475,8 +465,8 @@ __device__ __forceinline__ void take_keys(Rows<D, NT> &r, const Keys<D> &keys, i
         for (int half = 0; half < 2; half++) {
             const uint32_t sel = half ? 0x7362 : 0x5140;
             const uint32_t x = prmt(keys.v[0][w], keys.v[1][w], sel), y = prmt(keys.v[2][w], keys.v[3][w], sel);
-            const uint32_t a0 = code_pair(x, 0x4140, v_zero2), a1 = code_pair(x, 0x4342, v_zero2);
-            const uint32_t a2 = code_pair(y, 0x4140, v_zero2), a3 = code_pair(y, 0x4342, v_zero2);
+            const uint32_t a0 = code_pair<true>(x, 0x4140, v_zero2), a1 = code_pair<true>(x, 0x4342, v_zero2);
+            const uint32_t a2 = code_pair<true>(y, 0x4140, v_zero2), a3 = code_pair<true>(y, 0x4342, v_zero2);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 if (EXACT) {
@@ -585,12 +575,9 @@ __device__ __forceinline__ void do_segment(const AttnArgs &a, uint32_t b, const 
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int j = 0; j < 2; j++) {   // row 2c + j of the tile: its lanes are those with the same c
-            float l = r.l[nt][j], zp = r.zp[nt][j];
+            float l = r.l[nt][j];
 #pragma unroll
-            for (int o = 4; o <= 16; o <<= 1) {
-                l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
-                zp += __shfl_xor_sync(0xFFFFFFFFu, zp, o);
-            }
+            for (int o = 4; o <= 16; o <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
             const uint32_t rr = nt * 8 + 2 * c + j, row = row0 + rr;
             if (row >= rows) continue;
             const uint32_t t = row / a.group;
@@ -600,7 +587,7 @@ __device__ __forceinline__ void do_segment(const AttnArgs &a, uint32_t b, const 
             const float back = power2(-exponent_of(r.g[nt][j]));
 #pragma unroll
             for (int w = 0; w < D / 32; w++) {
-                auto real = [&](float x) { return sum_of(x, zp) * f * back; };
+                auto real = [&](float x) { return x * f * back; };
                 const float x0 = real(r.o[2 * w][nt][j]), x1 = real(r.o[2 * w][nt][j + 2]);
                 const float x2 = real(r.o[2 * w + 1][nt][j]), x3 = real(r.o[2 * w + 1][nt][j + 2]);
                 const int d = Geo<D>::v_dim(w, g);
@@ -791,18 +778,14 @@ cache_attention_cluster_kernel(const __grid_constant__ AttnArgs a)
     Rows<D, NT> r;
     take_steps<D, NT>(r, a, b, s, h, row0, (uint32_t)((uint64_t)steps * me / parts), (uint32_t)((uint64_t)steps * (me + 1) / parts));
     // the warps' maxima and sums, then their rows one warp after the other into the CTA's
-    float l[NT][2], zp[NT][2];
+    float l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             l[nt][j] = r.l[nt][j];
-            zp[nt][j] = r.zp[nt][j];
 #pragma unroll
-            for (int o = 4; o <= 16; o <<= 1) {
-                l[nt][j] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][j], o);
-                zp[nt][j] += __shfl_xor_sync(0xFFFFFFFFu, zp[nt][j], o);
-            }
+            for (int o = 4; o <= 16; o <<= 1) l[nt][j] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][j], o);
             if (g == 0) {
                 s_part[warp][nt * 8 + 2 * c + j][0] = r.m[nt][j];
                 s_part[warp][nt * 8 + 2 * c + j][1] = l[nt][j];
@@ -837,10 +820,10 @@ cache_attention_cluster_kernel(const __grid_constant__ AttnArgs a)
                     for (int i = 0; i < D / 32; i++) {
                         float4 *at = reinterpret_cast<float4 *>(&s_o[nt * 8 + 2 * c + j][Geo<D>::v_dim(i, g)]);
                         float4 v = w == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *at;
-                        v.x = fmaf(sum_of(r.o[2 * i][nt][j], zp[nt][j]), k, v.x);
-                        v.y = fmaf(sum_of(r.o[2 * i][nt][j + 2], zp[nt][j]), k, v.y);
-                        v.z = fmaf(sum_of(r.o[2 * i + 1][nt][j], zp[nt][j]), k, v.z);
-                        v.w = fmaf(sum_of(r.o[2 * i + 1][nt][j + 2], zp[nt][j]), k, v.w);
+                        v.x = fmaf(r.o[2 * i][nt][j], k, v.x);
+                        v.y = fmaf(r.o[2 * i][nt][j + 2], k, v.y);
+                        v.z = fmaf(r.o[2 * i + 1][nt][j], k, v.z);
+                        v.w = fmaf(r.o[2 * i + 1][nt][j + 2], k, v.w);
                         *at = v;
                     }
                 }

@@ -142,3 +142,47 @@ def test_one_row_of_a_tile_does_not_take_bits_from_another(cuda, form, dtype):
     if before > 0:
         diff = (got[:before].double() - plain[:before].double()).norm() / plain[:before].double().norm()
         assert diff < 2 * BOUND[dtype]
+
+
+# ---- long runs -------------------------------------------------------------------------------------------------------------
+# A table may name a block again and again: keys of a few blocks, each with its multiplicity, make long sequences whose 64-bit softmax
+# is as quick as that of the few.
+
+LONG = {"decode": (64, 1, 32768, 128, 8, 8), "decode, more sequences": (256, 1, 32768, 128, 8, 8), "decode, 16 heads": (64, 1, 32768, 128, 8, 16),
+        "decode, 64": (256, 1, 32768, 64, 8, 4), "decode, 256": (64, 1, 32768, 256, 4, 8), "drafts": (48, 4, 32768, 128, 8, 4),
+        "prompt": (2, 300, 131072, 128, 8, 4), "prompt, 256": (2, 300, 65536, 256, 8, 4), "prompt, 64": (2, 600, 65536, 64, 8, 4)}
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("form", LONG)
+def test_long_runs_of_keys_do_not_drift(cuda, form, dtype):
+    """Nearly flat scores, hundreds to thousands of steps per accumulator: sums that lose a little towards zero at each would show."""
+    import ltq
+    torch = cuda
+    seqs, new, keys, D, heads, group = LONG[form]
+    bt, few = 64, 8
+    tail = -(-new // bt)
+    times = (keys // bt - tail) // few
+    g = torch.Generator(device="cuda").manual_seed(7)
+    cache = ltq.KVCache.empty(few + tail, heads, bt, D)
+    for n in "kv":
+        getattr(cache, n).copy_((128 + 36 * torch.randn(few + tail, heads, bt, D, generator=g, device="cuda")).round_().clamp_(0, 255).to(torch.uint8))
+        qp = getattr(cache, n + "_qparams")
+        qp.view(torch.float32)[..., 0] = 0.02
+        qp[..., 4] = 128
+    row = list(range(few)) * times + list(range(few, few + tail))
+    length, scale = len(row) * bt, float(np.float32(D ** -0.5))
+    q = (0.02 * torch.randn(seqs * new, heads * group, D, generator=g, device="cuda")).to(getattr(torch, dtype))
+    got = cache.attention(q, ints(torch, [row] * seqs), ints(torch, [length] * seqs), ints(torch, [new * i for i in range(seqs + 1)]), new, scale=scale)
+    cache.check()
+    want = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    k, v = (0.02 * (getattr(cache, n).double() - 128.0) * (float(np.float32(0.02)) / 0.02) for n in "kv")
+    behind = torch.arange((few + tail) * bt, device="cuda") - few * bt          # place of a key behind the repeated ones
+    seen = behind[None] <= (tail * bt - new + torch.arange(new, device="cuda"))[:, None]
+    often = torch.where(behind < 0, math.log(times), 0.0)
+    for h in range(heads):
+        kk, vv = k[:, h].reshape(-1, D), v[:, h].reshape(-1, D)
+        s = torch.einsum("tgd,kd->tgk", q[:, h * group:(h + 1) * group].double(), kk) * scale + often
+        s = s.view(seqs, new, group, -1).masked_fill(~seen[None, :, None], -math.inf)
+        want[:, h * group:(h + 1) * group] = torch.einsum("sngk,kd->sngd", torch.softmax(s, 3), vv).reshape(-1, group, D)
+    assert float((got.double() - want).norm() / want.norm()) < BOUND[dtype]
