@@ -492,7 +492,8 @@ int ltq_im2col_t_u8(const uint8_t *im_dev, uint64_t batches, uint64_t channels, 
                     uint64_t stride_w, uint8_t *col_t_dev, uint64_t row_pitch, int device, void *stream);
 
 /* Same check for a device without a layer at hand (the stateless entry points share the device's status word).
- * LTQ_ERR_INVALID_ARG: a cache call met a sequence or block id outside its bounds since the last check. */
+ * LTQ_ERR_INVALID_ARG: a cache call met a sequence or block id outside its bounds since the last check.  Where a wait ran out as
+ * well, that is reported first and this by the check after it.  ltq_layer_check does the same. */
 int ltq_device_check(int device, void *stream);
 
 /* Failure-path self-test, no counterpart in the reference: launches one warp that waits on a barrier nothing will

@@ -994,18 +994,19 @@ int ltq_device_check(int device, void *stream)
     DeviceState *dev;
     int rc = device_state(device, &dev);
     if (rc != LTQ_OK) return rc;
-    uint32_t code = 0;
-    LTQ_CUDA_TRY(cudaMemcpyAsync(&code, dev->status, sizeof code, cudaMemcpyDeviceToHost, (cudaStream_t)stream));
+    uint32_t words[2] = {0, 0};   // expired wait, refused argument (see GemmDevice::status)
+    LTQ_CUDA_TRY(cudaMemcpyAsync(words, dev->status, sizeof words, cudaMemcpyDeviceToHost, (cudaStream_t)stream));
     LTQ_CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
-    if (code) {
+    if (const uint32_t code = words[0]) {
         LTQ_CUDA_TRY(cudaMemsetAsync(dev->status, 0, sizeof code, (cudaStream_t)stream));
-        if (code == STATUS_BAD_SEQUENCE || code == STATUS_BAD_BLOCK) {
-            set_error(code == STATUS_BAD_BLOCK ? "a cache call met a block id outside the cache"
-                                               : "a cache call met a sequence whose offsets or length contradict its bounds");
-            return LTQ_ERR_INVALID_ARG;
-        }
         set_error("a bounded device-side wait expired (code 0x%x: role %u, slot %u)", code, code >> 8, code & 0xFF);
         return LTQ_ERR_DEVICE_TIMEOUT;
+    }
+    if (words[1]) {
+        LTQ_CUDA_TRY(cudaMemsetAsync(dev->status + 1, 0, sizeof words[1], (cudaStream_t)stream));
+        set_error(words[1] == REFUSED_BLOCK ? "a cache call met a block id outside the cache"
+                                            : "a cache call met a sequence whose offsets or length contradict its bounds");
+        return LTQ_ERR_INVALID_ARG;
     }
     return LTQ_OK;
 }

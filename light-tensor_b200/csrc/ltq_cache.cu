@@ -64,7 +64,7 @@ cache_append_kernel(const ltq_kv_cache cache, const CacheBatch bt, const void *_
     griddep_launch_dependents();
     griddep_wait();
     const CacheSeq s = cache_seq(bt, blockIdx.z);
-    if (!s.ok && threadIdx.x == 0) atomicCAS(bt.status, 0u, STATUS_BAD_SEQUENCE);
+    if (!s.ok && threadIdx.x == 0) atomicCAS(bt.refused, 0u, REFUSED_SEQUENCE);
     if (!s.ok || s.n == 0) return;
     const bool is_v = blockIdx.x & 1;
     const int bt_tokens = 1 << bt.log2_bt, start = s.len - s.n < 0 ? 0 : s.len - s.n;   // first position that is stored
@@ -75,7 +75,7 @@ cache_append_kernel(const ltq_kv_cache cache, const CacheBatch bt, const void *_
     const int end = s.len - first < bt_tokens ? (int)(s.len - first) : bt_tokens;
     const int32_t page = bt.table[(uint64_t)blockIdx.z * bt.table_width + blk];
     if ((uint32_t)page >= cache.blocks) {
-        if (threadIdx.x == 0) atomicCAS(bt.status, 0u, STATUS_BAD_BLOCK);
+        if (threadIdx.x == 0) atomicCAS(bt.refused, 0u, REFUSED_BLOCK);
         return;
     }
     constexpr int VN = Vec<DT>::N;
@@ -218,6 +218,7 @@ CacheBatch make_batch(const ltq_kv_cache *c, const int32_t *offsets, const int32
     bt.max_new = (uint32_t)max_new;
     bt.log2_bt = c->block_tokens == 16 ? 4 : (c->block_tokens == 32 ? 5 : (c->block_tokens == 64 ? 6 : 7));
     bt.status = status;
+    bt.refused = status + 1;
     return bt;
 }
 

@@ -11,7 +11,8 @@ struct CacheBatch {
     uint64_t tokens;        // rows of the row arrays
     uint32_t seqs, table_width, max_new;
     int log2_bt;            // log2 of block_tokens
-    uint32_t *status;
+    uint32_t *status;       // word for expired waits
+    uint32_t *refused;      // word for what contradicts the bounds
 };
 
 struct CacheSeq {

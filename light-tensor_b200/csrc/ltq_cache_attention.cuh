@@ -163,7 +163,7 @@ __device__ __forceinline__ void fetch_keys(Keys<D> &t, const AttnArgs &a, const 
     t.bad = (uint32_t)page >= a.cache.blocks;
     if (t.bad) {
         page = 0;
-        if (threadIdx.x % 32 == 0) atomicCAS(a.bt.status, 0u, STATUS_BAD_BLOCK);
+        if (threadIdx.x % 32 == 0) atomicCAS(a.bt.refused, 0u, REFUSED_BLOCK);
     }
     const uint64_t slot = (uint64_t)(uint32_t)page * a.cache.kv_heads + h, base = ((slot << a.bt.log2_bt) + key_in_block) * D;
     t.k_par = __ldg(reinterpret_cast<const uint2 *>(a.cache.k_qp_dev + slot));
@@ -611,7 +611,7 @@ cache_attention_kernel(const __grid_constant__ AttnArgs a)
     unsigned long long mine = 0;
     for (uint32_t b = b0; b < b0 + run && b < a.bt.seqs; b++) {
         const CacheSeq s = cache_seq(a.bt, b);
-        if (!s.ok) atomicCAS(a.bt.status, 0u, STATUS_BAD_SEQUENCE);
+        if (!s.ok) atomicCAS(a.bt.refused, 0u, REFUSED_SEQUENCE);
         mine += seq_steps(a, s, ROWS);
     }
     before[threadIdx.x] = mine;
@@ -771,7 +771,7 @@ cache_attention_cluster_kernel(const __grid_constant__ AttnArgs a)
     const uint32_t h = blockIdx.y, b = blockIdx.z, row0 = blockIdx.x / size * ROWS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const CacheSeq s = cache_seq(a.bt, b);
-    if (!s.ok && threadIdx.x == 0) atomicCAS(a.bt.status, 0u, STATUS_BAD_SEQUENCE);
+    if (!s.ok && threadIdx.x == 0) atomicCAS(a.bt.refused, 0u, REFUSED_SEQUENCE);
     const uint32_t rows = s.ok ? (uint32_t)s.n * a.group : 0u;
     if (row0 >= rows) return;   // the whole cluster
     const uint32_t steps = seen_steps(a, s, row0, ROWS), parts = size * WARPS, me = rank * WARPS + warp;

@@ -309,7 +309,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
     }
     const uint32_t row0 = group * (TC_ROWS * RT);
     const CacheSeq s = cache_seq(a.bt, b);
-    if (!s.ok && threadIdx.x == 0) atomicCAS(status, 0u, STATUS_BAD_SEQUENCE);
+    if (!s.ok && threadIdx.x == 0) atomicCAS(a.bt.refused, 0u, REFUSED_SEQUENCE);
     const uint32_t rows = s.ok ? (uint32_t)s.n * a.group : 0u;
     auto tiles_of = [&](uint32_t rt) -> uint32_t {   // key tiles that row tile rt sees
         const uint32_t first = row0 + rt * TC_ROWS;
@@ -407,7 +407,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
         bool ok = true;
         for (uint32_t j = sb; j < mine; j += SB) {
             const uint32_t ph = (j / SB) & 1;
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(s_bar, ph, abort_flag, status, 0xB00u | sb));
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(s_bar, ph, abort_flag, status, 0xE00u | sb));
             if (!ok) break;
             tc_fence_after();
             const TilePar &par = s_par[j & 7];
@@ -469,7 +469,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             // The tile in front has its reference by now: the larger one holds for both.
             float alpha = 1.f;
             if (j > 0) {
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(m_other, ((j - 1) / SB) & 1, abort_flag, status, 0xB40u | sb));
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(m_other, ((j - 1) / SB) & 1, abort_flag, status, 0xE40u | sb));
                 if (!ok) break;
                 const float before = s_m[(wg ^ 1) * TC_ROWS + r], mx = fmaxf(m, before);
                 if (__any_sync(0xFFFFFFFFu, m < before)) {
@@ -489,7 +489,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             if (lane == 0) mbar_arrive(m_bar);
             if (__any_sync(0xFFFFFFFFu, alpha != 1.f)) {
                 // O so far times alpha: once the MMA that last added to it is done (S of the tile in front is, so the one before that was)
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(pv_bar + 8 * (sb ^ 1), ((j - 1) / SB) & 1, abort_flag, status, 0xB10u | sb));
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(pv_bar + 8 * (sb ^ 1), ((j - 1) / SB) & 1, abort_flag, status, 0xE10u | sb));
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll 1
@@ -540,12 +540,12 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
         if (ok && mine > 0) {
             const uint32_t last = mine - 1, lb = last % SB, ph = (last / SB) & 1;
             if (lb != sb) {
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(m_other, ph, abort_flag, status, 0xB20u | sb));
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(m_other, ph, abort_flag, status, 0xE20u | sb));
                 const float mx = s_m[(wg ^ 1) * TC_ROWS + r];
                 if (m != mx) l = times2(l, m - mx);
                 m = mx;
             }
-            ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(pv_bar + 8 * lb, ph, abort_flag, status, 0xB28u | sb));
+            ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(pv_bar + 8 * lb, ph, abort_flag, status, 0xE28u | sb));
             tc_fence_after();
         }
         meet();
@@ -606,7 +606,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
         if constexpr (G::REGS_CONVERT < G::REGS) regs_down<G::REGS_CONVERT>();
         const int tid = threadIdx.x & 127;
         auto take = [&](uint32_t hf) {   // part hf of the codes is there
-            return __all_sync(0xFFFFFFFFu, mbar_wait(raw_full + 8 * (hf % G::RAW), hf / G::RAW & 1, abort_flag, status, 0xB50u | hf % G::RAW));
+            return __all_sync(0xFFFFFFFFu, mbar_wait(raw_full + 8 * (hf % G::RAW), hf / G::RAW & 1, abort_flag, status, 0xE50u | hf % G::RAW));
         };
         auto give = [&](uint32_t hf) {
             __syncwarp();
@@ -621,7 +621,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                 const uint32_t j = hf / G::PARTS, st = j & 1;
                 if (!take(hf)) break;
                 if (hf % G::PARTS == 0 && j >= 2 &&
-                    !__all_sync(0xFFFFFFFFu, mbar_wait(k_empty + 8 * st, ((j - 2) >> 1) & 1, abort_flag, status, 0xB30u | st))) break;
+                    !__all_sync(0xFFFFFFFFu, mbar_wait(k_empty + 8 * st, ((j - 2) >> 1) & 1, abort_flag, status, 0xE30u | st))) break;
                 const uint4 *src = reinterpret_cast<const uint4 *>(codes + hf % G::RAW * G::RAW_BYTES) + tid;
                 uint4 w[PER];
 #pragma unroll
@@ -653,7 +653,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                 const uint32_t j = hf / G::PARTS, st = j & 1;
                 if (!take(hf)) break;
                 if (hf % G::PARTS == 0 && j >= 2 &&
-                    !__all_sync(0xFFFFFFFFu, mbar_wait(v_empty + 8 * st, ((j - 2) >> 1) & 1, abort_flag, status, 0xB48u | st))) break;
+                    !__all_sync(0xFFFFFFFFu, mbar_wait(v_empty + 8 * st, ((j - 2) >> 1) & 1, abort_flag, status, 0xE48u | st))) break;
                 if (busy) {
                     const uint8_t *src = codes + hf % G::RAW * G::RAW_BYTES + G::PART * D + kg * G::V_GROUP + d0;
                     uint2 c[8];
@@ -708,7 +708,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             if (parts > 1) next = page_at(1);
             for (; hf < parts; hf++) {
                 const uint32_t st = hf % G::RAW, bar = raw_full + 8 * st;
-                if (!__all_sync(0xFFFFFFFFu, hf < (uint32_t)G::RAW || mbar_wait(raw_empty + 8 * st, (hf / G::RAW - 1) & 1, abort_flag, status, 0xB58u | st))) break;
+                if (!__all_sync(0xFFFFFFFFu, hf < (uint32_t)G::RAW || mbar_wait(raw_empty + 8 * st, (hf / G::RAW - 1) & 1, abort_flag, status, 0xE58u | st))) break;
                 if (v_lane && lane % 2 == 0) s_zero[st][(lane - 8) / 2] = zero;
                 __syncwarp();
                 if (lane == 0) mbar_expect_tx(bar, G::PART * D * 2);
@@ -724,7 +724,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             // given up: the copies still under way have to land before the block ends (a second, bounded wait)
             if (hf < parts)
                 for (uint32_t i = hf > (uint32_t)G::RAW ? hf - G::RAW : 0u; i < hf; i++)
-                    mbar_wait(raw_full + 8 * (i % G::RAW), i / G::RAW & 1, s_misc + 2, status, 0xB5Cu);
+                    mbar_wait(raw_full + 8 * (i % G::RAW), i / G::RAW & 1, s_misc + 2, status, 0xE5Cu);
         } else if (rt == 3) {
             // what the softmax needs of every tile: lane i % GROUPS looks after its group i
             float loudest = -INFINITY;   // log2 of V's largest scale so far
@@ -744,8 +744,8 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             for (uint32_t j = 0; j < tiles; j++) {
                 // in the place of tile j - 8: S of tile j - 2 is done, so P of tile j - 4 was
                 const uint32_t st = j & 1;
-                if (!__all_sync(0xFFFFFFFFu, j < 2 || mbar_wait(k_empty + 8 * st, ((j - 2) >> 1) & 1, abort_flag, status, 0xB38u | st))) break;
-                if (bad && lane < G::GROUPS) atomicCAS(status, 0u, STATUS_BAD_BLOCK);
+                if (!__all_sync(0xFFFFFFFFu, j < 2 || mbar_wait(k_empty + 8 * st, ((j - 2) >> 1) & 1, abort_flag, status, 0xE38u | st))) break;
+                if (bad && lane < G::GROUPS) atomicCAS(a.bt.refused, 0u, REFUSED_BLOCK);
                 // log2 of the scale, from its exponent where it has one; an infinity is as good as a NaN
                 const float mantissa = __uint_as_float((__float_as_uint(vs) & 0x7FFFFFu) | 0x3F800000u);
                 float lv = vs < TC_SMALLEST ? lg2(vs) : (float)((int)(__float_as_uint(vs) >> 23) - 127) + lg2(mantissa);
@@ -784,8 +784,8 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             // S of tile j; its buffer holds P of tile j - SB until the MMA that reads it is done
             auto scores = [&](uint32_t j) -> bool {
                 const uint32_t st = j & 1, sb = j % SB;
-                if (!wait(k_full + 8 * st, (j >> 1) & 1, 0xB60u | st)) return false;
-                if (j >= SB && !wait(pv_bar + 8 * sb, ((j - SB) / SB) & 1, 0xB70u | sb)) return false;
+                if (!wait(k_full + 8 * st, (j >> 1) & 1, 0xE60u | st)) return false;
+                if (j >= SB && !wait(pv_bar + 8 * sb, ((j - SB) / SB) & 1, 0xE70u | sb)) return false;
                 tc_fence_after();
                 const uint64_t kd = make_smem_desc(sk + st * G::K_BYTES);
                 if (elect_one()) {
@@ -801,7 +801,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             };
             auto output = [&](uint32_t j) -> bool {
                 const uint32_t st = j & 1, sb = j % SB;
-                if (!wait(v_full + 8 * st, (j >> 1) & 1, 0xB80u | st) || !wait(p_bar + 8 * sb, (j / SB) & 1, 0xB90u | sb)) return false;
+                if (!wait(v_full + 8 * st, (j >> 1) & 1, 0xE80u | st) || !wait(p_bar + 8 * sb, (j / SB) & 1, 0xE90u | sb)) return false;
                 tc_fence_after();
                 const uint64_t vd = make_smem_desc(sv + st * G::V_BYTES);
                 if (elect_one()) {
@@ -815,7 +815,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                 __syncwarp();
                 return true;
             };
-            bool ok = tiles > 0 && wait(q_full, 0, 0xB50u);
+            bool ok = tiles > 0 && wait(q_full, 0, 0xEC0u);
             if (SB == 1) {
                 for (uint32_t j = 0; ok && j < mine; j++) ok = scores(j) && output(j);
             } else {   // S of the next tile before O of this one
@@ -825,7 +825,7 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
             // tiles that only the other row tile sees: their stages are not held up here
             for (uint32_t j = mine; ok && j < tiles; j++) {
                 const uint32_t st = j & 1;
-                ok = wait(k_full + 8 * st, (j >> 1) & 1, 0xBA0u | st) && wait(v_full + 8 * st, (j >> 1) & 1, 0xBB0u | st);
+                ok = wait(k_full + 8 * st, (j >> 1) & 1, 0xEA0u | st) && wait(v_full + 8 * st, (j >> 1) & 1, 0xEB0u | st);
                 if (ok && lane == 0) {
                     mbar_arrive(k_empty + 8 * st);
                     mbar_arrive(v_empty + 8 * st);

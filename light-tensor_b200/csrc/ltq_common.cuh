@@ -431,8 +431,10 @@ struct GemmDevice {
     int sms;
     uint32_t *status;
 };
-// Codes of the status word that are not expired waits: what the cache kernels found in their device-side arguments.
-constexpr uint32_t STATUS_BAD_SEQUENCE = 0xA01u, STATUS_BAD_BLOCK = 0xA02u;
+// status[0]: the code of the first bounded wait that expired.  Its upper bits say which wait (a role, shared by kernels of one build: 1 to 7
+// the GEMMs and the convolution, 9 the self-test, A to D the fused chain, E the prompt attention, F the GEMM for few tiles).
+// status[1]: what a cache kernel found in its device-side arguments.  Two words, so that neither hides the other.
+constexpr uint32_t REFUSED_SEQUENCE = 1, REFUSED_BLOCK = 2;
 // Per-device constants and the status word, created on first use with that device current.
 int device_state(int device, GemmDevice **out);
 }  // namespace ltq

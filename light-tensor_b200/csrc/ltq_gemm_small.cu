@@ -142,7 +142,7 @@ gemm_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         if (lane == 0) {
             uint32_t st = 0, ph = 0;
             for (uint32_t kb = kb0 + stages; kb < kb1; kb++) {
-                if (!mbar_wait(empty0 + 8 * st, ph, abort_flag, status, 0xC00u | st)) break;
+                if (!mbar_wait(empty0 + 8 * st, ph, abort_flag, status, 0xF00u | st)) break;
                 mbar_expect_tx(full0 + 8 * st, stage_bytes);
                 load(ring + st * stage_bytes, &map_a, full0 + 8 * st, kb, m0);
                 load(ring + st * stage_bytes + a_bytes, &map_b, full0 + 8 * st, kb, n0);
@@ -156,7 +156,7 @@ gemm_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         uint32_t st = 0, ph = 0;
         bool ok = true;
         for (uint32_t kb = kb0; kb < kb1; kb++) {
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(full0 + 8 * st, ph, abort_flag, status, 0xC10u | st));
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(full0 + 8 * st, ph, abort_flag, status, 0xF10u | st));
             if (!ok) break;
             tc_fence_after();
             const uint64_t a_desc = make_smem_desc(ring + st * stage_bytes) + 2u * warp;
@@ -195,7 +195,7 @@ gemm_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             const uint32_t gj = n0 + rank * slice + j;
             s_col[j] = gj < N ? token_col(epi, gj) : make_uint4(0, 0, 0, 0);
         }
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(done, 0, abort_flag, status, 0xC20u));
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(done, 0, abort_flag, status, 0xF20u));
         if (split > 1) cluster_wait();
         if (ok) {
             tc_fence_after();
