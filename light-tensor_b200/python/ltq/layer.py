@@ -82,8 +82,9 @@ class LayerHandle:
         """Parameters per output channel: uint8 CUDA tensor [N, 8] of QParams (``quantize_tokens`` of the weight matrix gives
         one), optional float32 bias [N].  Call after set_weights, and again after every later set_weights."""
         _tokens.check_qparams(qparams, self.N, self.device_index)
-        if bias is not None and not (bias.is_cuda and bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == self.N):
-            raise ValueError("bias must be a contiguous float32 CUDA tensor with one value per output feature")
+        if bias is not None and not (bias.get_device() == self.device_index and bias.dtype == torch.float32 and bias.is_contiguous() and
+                                     bias.numel() == self.N):
+            raise ValueError(f"bias must be a contiguous float32 CUDA tensor on device {self.device_index} with one value per output feature")
         self._keep_channels = (qparams, bias)  # the library borrows these pointers
         check(lib().ltq_layer_set_channel_qparams(self._h, qparams.data_ptr(), None if bias is None else bias.data_ptr(), self._stream()))
         self._row_workspace = lib().ltq_layer_float_workspace(self._h, 1)   # bytes per token, see forward_float
@@ -91,12 +92,12 @@ class LayerHandle:
     def forward_tokens(self, x, qparams, sums, dtype=torch.float32, flags=0, out=None):
         """Product of codes x uint8 [M, K] that have parameters per token (``quantize_tokens`` returns all three) with this
         layer's weights under their parameters per channel.  Returns [M, N] of `dtype`; ``out`` may have strided rows."""
-        if not (x.is_cuda and x.dtype == torch.uint8 and x.is_contiguous() and x.dim() == 2 and x.shape[1] == self.K):
-            raise ValueError(f"x must be a contiguous uint8 CUDA tensor [tokens, {self.K}]")
+        if not (x.get_device() == self.device_index and x.dtype == torch.uint8 and x.is_contiguous() and x.dim() == 2 and x.shape[1] == self.K):
+            raise ValueError(f"x must be a contiguous uint8 CUDA tensor [tokens, {self.K}] on device {self.device_index}")
         M = x.shape[0]
         _tokens.check_qparams(qparams, M, self.device_index)
-        if not (sums.is_cuda and sums.dtype == torch.int32 and sums.is_contiguous() and sums.numel() == M):
-            raise ValueError("sums must be a contiguous int32 CUDA tensor with one value per token")
+        if not (sums.get_device() == self.device_index and sums.dtype == torch.int32 and sums.is_contiguous() and sums.numel() == M):
+            raise ValueError(f"sums must be a contiguous int32 CUDA tensor on device {self.device_index} with one value per token")
         out = self._tokens_out(out, M, dtype, x.device)
         if M:
             check(lib().ltq_layer_forward_tokens(self._h, x.data_ptr(), qparams.data_ptr(), sums.data_ptr(), M, _tokens.dtype_code(dtype), flags,
@@ -126,8 +127,8 @@ class LayerHandle:
     def _tokens_out(self, out, M, dtype, device):
         if out is None:
             return torch.empty((M, self.N), dtype=dtype, device=device)
-        if not (out.is_cuda and out.device == device and out.dtype == dtype and out.shape == (M, self.N) and (out.stride(1) == 1 or self.N == 1)):
-            raise ValueError(f"out must be a CUDA tensor [{M}, {self.N}] of {dtype} with contiguous rows")
+        if not (out.get_device() == self.device_index and out.dtype == dtype and out.shape == (M, self.N) and (out.stride(1) == 1 or self.N == 1)):
+            raise ValueError(f"out must be a tensor [{M}, {self.N}] of {dtype} with contiguous rows on device {self.device_index}")
         if M > 1 and out.stride(0) < self.N:
             raise ValueError("out's rows overlap")
         return out
