@@ -135,7 +135,7 @@ int ltq_interleave_column_blocks(const void *gathered_dev, void *out_dev, uint64
  * per-tensor calls give for it.  Where those are undefined: a range below 255 * 2^-126 (a row of zeros) gets the scale
  * 2^-126; a range that overflows gets max / 255 - min / 255; a row that holds an infinity or a NaN gets the scale NaN, zero
  * point 0 and codes 0, so that what is computed from that token is NaN and other tokens are not touched.
- * features <= 2^31 - 1. */
+ * features <= 2^31 - 1, and with sums_dev <= 8421504 (LTQ_ERR_TOO_LARGE beyond: a sum of codes might not fit). */
 int ltq_quantize_tokens_u8(const void *x_dev, int x_dtype, uint64_t tokens, uint64_t features, uint64_t ld_x, uint8_t *q_dev,
                            ltq_qparams *qp_dev, int32_t *sums_dev, int device, void *stream);
 

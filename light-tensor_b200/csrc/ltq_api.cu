@@ -228,6 +228,8 @@ int ltq_quantize_tokens_u8(const void *x_dev, int x_dtype, uint64_t tokens, uint
     LTQ_REQUIRE(features >= 1 && (ld_x >= features || tokens <= 1), LTQ_ERR_INVALID_ARG, "rows of %llu elements cannot be %llu apart",
                 (unsigned long long)features, (unsigned long long)ld_x);
     LTQ_REQUIRE(features < (1ull << 31), LTQ_ERR_TOO_LARGE, "features must be below 2^31");
+    LTQ_REQUIRE(!sums_dev || features <= 0x7FFFFFFFull / 255, LTQ_ERR_TOO_LARGE, "the code sum of %llu features may not fit 32 bits: at most %llu with sums",
+                (unsigned long long)features, 0x7FFFFFFFull / 255);
     LTQ_REQUIRE(((uintptr_t)x_dev % dtype_size(x_dtype)) == 0 && ((uintptr_t)qp_dev & 3) == 0 && ((uintptr_t)sums_dev & 3) == 0,
                 LTQ_ERR_INVALID_ARG, "misaligned array");
     if (tokens == 0) return LTQ_OK;

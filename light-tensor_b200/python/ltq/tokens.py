@@ -43,7 +43,8 @@ def raw_stream(device_index):
 def quantize_tokens(x, q=None, qparams=None, sums=None):
     """GetMinMax, ComputeQuantizationParams and Quantize of every row of x on its own.  x: float32 / float16 / bfloat16 CUDA
     [M, K], rows may be strided.  Returns (codes uint8 [M, K], parameters uint8 [M, 8] laid out as QParams, code sums
-    int32 [M]); existing tensors may be passed in for them.  A row with an infinity or NaN gets scale NaN and codes 0."""
+    int32 [M]); existing tensors may be passed in for them.  A row with an infinity or NaN gets scale NaN and codes 0.
+    K at most 8421504, so that a sum of codes fits."""
     dev = x.get_device()
     if dev < 0 or x.dim() != 2:
         raise ValueError("ltq operates on CUDA tensors only (there is no CPU path): a matrix [tokens, features] is expected")
