@@ -396,7 +396,8 @@ int ltq_layer_check(ltq_layer *layer, void *stream);
  *   lengths_dev int32 [seqs]      tokens of the sequence in all, those of this call included
  *   offsets_dev int32 [seqs + 1]  sequence b's tokens of this call are rows offsets[b] .. offsets[b+1] - 1 of the row arrays
  *   table_dev int32 [seqs][table_width]  block ids in the order of their tokens; token p is in block table[b][p / block_tokens]
- *   max_new                       host bound on offsets[b+1] - offsets[b] (sizes the launch)
+ *   max_new                       host bound on offsets[b+1] - offsets[b] (sizes the launch), at most `tokens`
+ *   table_width                   sizes the launch too: a table no wider than the sequences need gets the form that suits them
  * The n tokens of this call are the sequence's last n: positions lengths[b] - n .. lengths[b] - 1.  Tokens whose position
  * is negative (padding in front of a short sequence) are not stored, and their attention output is zero.  A sequence
  * that contradicts the bounds (offsets that fall or leave [0, tokens], more than max_new tokens, a negative length or one beyond

@@ -199,7 +199,7 @@ int check_batch(const ltq_kv_cache *c, const void *offsets, const void *lengths,
     LTQ_REQUIRE(offsets && lengths && (table || table_width == 0), LTQ_ERR_INVALID_ARG, "Invalid argument");
     LTQ_REQUIRE((((uintptr_t)offsets | (uintptr_t)lengths | (uintptr_t)table) & 3) == 0, LTQ_ERR_INVALID_ARG, "misaligned array");
     LTQ_REQUIRE(seqs <= 65535, LTQ_ERR_TOO_LARGE, "%llu sequences: at most 65535", (unsigned long long)seqs);
-    LTQ_REQUIRE(tokens < (1ull << 31) && max_new <= tokens && table_width * c->block_tokens < (1ull << 31), LTQ_ERR_INVALID_ARG,
+    LTQ_REQUIRE(tokens < (1ull << 31) && max_new <= tokens && table_width <= 0x7FFFFFFFull / c->block_tokens, LTQ_ERR_INVALID_ARG,
                 "%llu tokens, at most %llu per sequence, tables of %llu blocks", (unsigned long long)tokens, (unsigned long long)max_new,
                 (unsigned long long)table_width);
     return LTQ_OK;
@@ -315,7 +315,11 @@ int ltq_cache_append(const ltq_kv_cache *cache, const void *k_dev, const void *v
 uint64_t ltq_cache_attention_workspace(const ltq_kv_cache *cache, uint64_t tokens, uint32_t q_heads, uint64_t seqs, uint64_t table_width,
                                        uint64_t max_new, int device)
 {
-    if (check_cache(cache) != LTQ_OK || q_heads == 0 || q_heads % cache->kv_heads != 0 || tokens == 0 || seqs == 0 || max_new == 0) return 0;
+    // (0 too where the call itself would be refused for its sizes)
+    if (check_cache(cache) != LTQ_OK || q_heads == 0 || q_heads % cache->kv_heads != 0 || q_heads / cache->kv_heads > 1024 || tokens == 0 || seqs == 0 ||
+        max_new == 0 || seqs > 65535 || tokens >= (1ull << 31) || max_new > tokens || table_width > 0x7FFFFFFFull / cache->block_tokens ||
+        max_new * q_heads >= (1ull << 31))
+        return 0;
     DeviceGuard guard(device);
     GemmDevice *dev;
     if (guard.err != cudaSuccess || device_state(device, &dev) != LTQ_OK) return 0;
@@ -343,7 +347,8 @@ int ltq_cache_attention(const ltq_kv_cache *cache, const void *q_dev, int dtype,
                 (unsigned long long)ld_q);
     LTQ_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev) % dtype_size(dtype)) == 0 && ((uintptr_t)workspace_dev & 15) == 0, LTQ_ERR_INVALID_ARG,
                 "misaligned array");
-    LTQ_REQUIRE(scale - scale == 0.f, LTQ_ERR_INVALID_ARG, "the softmax scale must be finite");
+    const float scale_log2 = scale * 1.4426950408889634f;
+    LTQ_REQUIRE(scale_log2 - scale_log2 == 0.f, LTQ_ERR_INVALID_ARG, "the softmax scale must be finite, its product with log2(e) too");
     LTQ_REQUIRE(max_new * q_heads < (1ull << 31), LTQ_ERR_TOO_LARGE, "max_new * q_heads must be below 2^31");
     LTQ_ENTER_DEVICE(device);
     GemmDevice *dev;
@@ -357,7 +362,7 @@ int ltq_cache_attention(const ltq_kv_cache *cache, const void *q_dev, int dtype,
     a.ld_q = ld_q;
     a.q_heads = q_heads;
     a.group = q_heads / cache->kv_heads;
-    a.scale_log2 = scale * 1.4426950408889634f;
+    a.scale_log2 = scale_log2;
     const AttnPlan p = attn_plan(cache, dtype, q_heads, seqs, table_width, max_new, dev->sms);
     LTQ_REQUIRE(p.bytes == 0 || (workspace_dev && workspace_bytes >= p.bytes), LTQ_ERR_INVALID_ARG, "the workspace holds %llu bytes, %llu are needed",
                 (unsigned long long)workspace_bytes, (unsigned long long)p.bytes);

@@ -14,7 +14,7 @@ class KVCache:
 
     A batch of sequences is described by int32 CUDA tensors: ``lengths`` [seqs] (tokens in all, the new ones included),
     ``offsets`` [seqs + 1] (sequence b's new tokens are rows offsets[b] .. offsets[b + 1] - 1) and ``table`` [seqs, width] (block ids);
-    ``max_new`` is a host bound on the new tokens of a sequence.  The kernels read these tensors when they run, so a captured
+    ``max_new`` is a host bound on the new tokens of a sequence, at most the rows there are.  The kernels read these tensors when they run, so a captured
     call follows their contents.  A sequence or block id that contradicts the bounds is left out and makes the next
     ``check()`` raise."""
 
