@@ -193,7 +193,10 @@ typedef struct ltq_layer ltq_layer;
 
 /* FullyConnected_q::init, l-ten/fully_connected.cpp:295-320, device side.  The handle owns only derived state
  * (weight row sums, tensor maps, the activation-sum workspace that l-ten keeps in workspace_); weights and bias stay
- * the caller's. */
+ * the caller's.
+ * Threads: forwards of one layer may run in several host threads and on several streams at once, each with a workspace of its
+ * own where it takes one; those that leave the activation sums to the layer (asum_dev NULL) share its workspace and have to be
+ * ordered.  The calls that set something, and ltq_layer_destroy, run alone. */
 int ltq_layer_create(ltq_layer **layer, int device, uint64_t in_features, uint64_t out_features);
 int ltq_layer_destroy(ltq_layer *layer);
 

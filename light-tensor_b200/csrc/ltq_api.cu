@@ -280,6 +280,8 @@ int ltq::run_fc_gemm(const GemmDevice &gd, uint64_t M, uint64_t N, uint64_t K, c
     Path path;
     int rc = choose_path(M, N, K, A, B, flags, dev->sms, &path);
     if (rc != LTQ_OK) return rc;
+    std::unique_lock<std::mutex> lock;
+    if (layer) lock = std::unique_lock<std::mutex>(layer->maps);
     switch (path) {
         case PATH_SKINNY:
             // a layer's weights are fixed between ltq_layer_set_weights calls (which synchronise), so they may be streamed early
@@ -328,7 +330,15 @@ int ltq::run_fc_gemm(const GemmDevice &gd, uint64_t M, uint64_t N, uint64_t K, c
                 }
                 LTQ_CUDA_TRY(launch_gemm_tc_pair(map_a, maps, tl, M, N, K, epi, out, dev->status, dev->sms, stream));
             } else if (small) {
-                TcOperandMap *mb = layer ? &layer->map_w_small : &tmp_b[0];
+                TcOperandMap *mb = layer ? nullptr : &tmp_b[0];
+                if (layer) {
+                    for (auto &m : layer->map_w_small)
+                        if (m.matches(B, N, K, (int)plan.bn, plan.lines > 1 ? (int)plan.lines : 0)) mb = &m;
+                    if (!mb) {
+                        mb = &layer->map_w_small[layer->map_w_small_next];
+                        layer->map_w_small_next = (layer->map_w_small_next + 1) % LAYER_MAPS;
+                    }
+                }
                 er = small_maps(plan, A, M, K, &map_a, B, N, mb);
                 LTQ_REQUIRE(er == 0, LTQ_ERR_CUDA, "cuTensorMapEncodeTiled failed for an operand (CUresult %d)", er);
                 LTQ_CUDA_TRY(launch_gemm_small(map_a, *mb, plan, M, N, K, epi, out, dev->status, stream, layer != nullptr));
@@ -453,7 +463,7 @@ int ltq_layer_set_weights(ltq_layer *layer, const uint8_t *w_dev, const int32_t 
     layer->qp_channels = nullptr;   // parameters per channel belong to the weights they were given for
     for (auto &m : layer->map_w) m = TcOperandMap();
     layer->map_w_gemv = GemvWeightMaps();
-    layer->map_w_small = TcOperandMap();
+    for (auto &m : layer->map_w_small) m = TcOperandMap();
     LTQ_CUDA_TRY(launch_row_sums(w_dev, layer->N, layer->K, layer->wsum, (cudaStream_t)stream));
     LTQ_CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
     return LTQ_OK;

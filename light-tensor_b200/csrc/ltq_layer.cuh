@@ -1,6 +1,8 @@
 // The layer handle behind ltq_layer_* (include/ltq.h): what FullyConnected_q keeps between calls, device side.  Shared by
 // the entry points in ltq_api.cu and the multi-device ones in ltq_sharded.cu.
 #pragma once
+#include <mutex>
+
 #include "ltq_common.cuh"
 #include "ltq_gemm_tc.cuh"
 #include "ltq_gemv.cuh"
@@ -27,7 +29,11 @@ struct ltq_layer {
     uint64_t padded_k() const { return (K + 15) / 16 * 16; }
     ltq::TcOperandMap map_w[LAYER_MAPS];  // weight tensor maps of the tensor-core kernels, one per box height, built on demand
     int map_w_next = 0;
-    ltq::TcOperandMap map_w_small;      // weight tensor map of the kernel for few tiles, of its last plan
+    ltq::TcOperandMap map_w_small[LAYER_MAPS];  // the same for the kernel for few tiles, one per tile width and lines per box
+    int map_w_small_next = 0;
+    // Held by a forward while it finds, makes and launches with the maps here: another thread's forward of another batch size
+    // may want the slot for a map of its own.
+    std::mutex maps;
     ltq::GemvWeightMaps map_w_gemv;     // weight tensor maps of the skinny kernel
     ltq::GemvNext next;                 // weights of the layer that runs after this one (ltq_layer_set_next), with
     ltq::GemvWeightMaps map_next_gemv;  // their tensor maps as the skinny kernel of THIS layer needs them
