@@ -816,12 +816,9 @@ cache_attention_tc_kernel(const __grid_constant__ AttnArgs a)
                 return true;
             };
             bool ok = tiles > 0 && wait(q_full, 0, 0xEC0u);
-            if (SB == 1) {
-                for (uint32_t j = 0; ok && j < mine; j++) ok = scores(j) && output(j);
-            } else {   // S of the next tile before O of this one
-                if (ok && mine > 0) ok = scores(0);
-                for (uint32_t j = 0; ok && j < mine; j++) ok = (j + 1 >= mine || scores(j + 1)) && output(j);
-            }
+            // S of the next tile before O of this one
+            if (ok && mine > 0) ok = scores(0);
+            for (uint32_t j = 0; ok && j < mine; j++) ok = (j + 1 >= mine || scores(j + 1)) && output(j);
             // tiles that only the other row tile sees: their stages are not held up here
             for (uint32_t j = mine; ok && j < tiles; j++) {
                 const uint32_t st = j & 1;
