@@ -75,9 +75,9 @@ int ltq_version(void);
 const char *ltq_last_error(void);
 /* Number of kernels this library has launched since load (all threads). */
 uint64_t ltq_kernel_launches(void);
-/* Name of the GEMM kernel the calling thread launched last, with its template arguments (tile width, output type), e.g.
+/* Name of the GEMM or cache attention kernel the calling thread launched last, with its template arguments (tile width, output type), e.g.
  * "gemm_tc_pair_kernel<256,u8>"; "" before the first one.  For tests, profiling and benchmark records: it names what
- * the shape-based dispatch of ltq_layer_forward / ltq_quantized_matmul* actually chose.  No counterpart in the
+ * the shape-based dispatch of ltq_layer_forward* / ltq_quantized_matmul* / ltq_cache_attention actually chose.  No counterpart in the
  * reference. */
 const char *ltq_last_kernel(void);
 

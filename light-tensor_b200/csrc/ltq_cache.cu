@@ -380,9 +380,12 @@ int ltq_cache_attention(const ltq_kv_cache *cache, const void *q_dev, int dtype,
     cudaStream_t st = (cudaStream_t)stream;
     if (p.tc) {
         LTQ_CUDA_TRY(launch_attention_tc(a, dtype, st));
+        note_kernel("cache_attention_tc_kernel<%s,%u> (keys in %u)", dtype_name(dtype), cache->head_dim, p.splits);
         return LTQ_OK;
     }
     LTQ_CUDA_TRY(dtype == LTQ_F32 ? launch_attention_f32(a, st) : (dtype == LTQ_F16 ? launch_attention_f16(a, st) : launch_attention_bf16(a, st)));
+    if (p.cluster) note_kernel("cache_attention_cluster_kernel<%s,%u,%u> (clusters of %u)", dtype_name(dtype), cache->head_dim, p.rows_per_tile, p.cluster);
+    else note_kernel("cache_attention_kernel<%s,%u,%u>", dtype_name(dtype), cache->head_dim, p.rows_per_tile);
     return LTQ_OK;
 }
 

@@ -17,6 +17,7 @@ namespace ltq {
 constexpr int OUT_TOKENS = 3;   // Epilogue::out_mode and the kernels' OUT argument: OUT_TOKENS + ltq_dtype
 __host__ __device__ constexpr bool out_is_tokens(int out) { return out >= OUT_TOKENS; }
 inline uint64_t dtype_size(int dtype) { return dtype == LTQ_F32 ? 4 : 2; }
+inline const char *dtype_name(int dtype) { return dtype == LTQ_F32 ? "f32" : (dtype == LTQ_F16 ? "f16" : "bf16"); }
 inline bool dtype_ok(int dtype) { return dtype == LTQ_F32 || dtype == LTQ_F16 || dtype == LTQ_BF16; }
 
 // |a - za| and |w - zw| reach 255 when a zero point sits at an end of the range: up to this many terms fit an int32.
