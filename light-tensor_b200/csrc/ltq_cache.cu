@@ -371,6 +371,7 @@ int ltq_cache_attention(const ltq_kv_cache *cache, const void *q_dev, int dtype,
     a.out_vec8 = ((uintptr_t)out_dev & 15) == 0;
     a.out_vec = ((uintptr_t)out_dev % (4 * dtype_size(dtype))) == 0;
     a.cluster = p.cluster;
+    a.few_rows = 8 * (uint32_t)dev->sms;
     a.splits = p.splits;
     a.ctas = p.ctas;
     a.row_tiles = p.row_tiles;

@@ -52,11 +52,11 @@ struct AttnArgs {
     uint32_t ctas, row_tiles;      // (tensor-core form: the SMs, groups of row tiles)
     uint32_t splits;               // tensor-core form: CTAs that share one's keys
     uint32_t cluster;              // CTAs per item in the form without workspace; 0: the form with
+    uint32_t few_rows;             // up to so many rows are joined by a CTA each: eight for every SM
 };
 constexpr uint32_t ATTN_WARPS = 4;             // per CTA
 constexpr uint32_t ATTN_MIN_STEPS = 4;         // fewer 16-key steps than this are not worth a warp of their own
 constexpr uint32_t ATTN_CLUSTER_STEPS = 16;    // up to this many per warp one launch without workspace is faster
-constexpr uint64_t ATTN_FEW_ROWS = 1184;       // eight CTAs on each of 148 SMs
 // Rows of (token, head of the group) that one CTA of the attention kernel takes.
 uint32_t attn_rows_per_tile(int dtype, uint32_t head_dim, uint64_t rows);
 // CTAs of it that fit an SM at once.

@@ -858,7 +858,7 @@ cudaError_t launch_join(const AttnArgs &a, uint32_t rows_per_tile, bool dense, c
 {
     const uint64_t rows = (uint64_t)a.bt.max_new * a.q_heads;   // of one sequence
     count_launch();
-    if (rows * a.bt.seqs <= ATTN_FEW_ROWS)
+    if (rows * a.bt.seqs <= a.few_rows)
         return launch_chained(cache_attention_join_kernel<D, 8>, dim3((unsigned)rows, a.bt.seqs), dim3(256), 0, stream, a, rows_per_tile, dense);
     return launch_chained(cache_attention_join_kernel<D, 1>, dim3((unsigned)((rows + 7) / 8), a.bt.seqs), dim3(256), 0, stream, a, rows_per_tile, dense);
 }

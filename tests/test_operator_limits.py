@@ -31,3 +31,16 @@ def test_a_softmax_scale_that_wraps_in_base_two():
     L = ltq.lib()
     for scale in (3e38, -3e38, float("inf"), float("nan")):
         assert attention(L, scale=scale) == -1 and "softmax scale" in ltq.last_error()
+
+
+def test_no_number_of_sms_is_written_into_the_code():
+    """The plans ask the device for it (ten times and twenty times 148 included)."""
+    import glob
+    import os
+    import re
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    for path in glob.glob(os.path.join(root, "light-tensor_b200", "csrc", "ltq_*.cu*")):
+        if os.path.basename(path).startswith(("ltq_cache", "ltq_tokens", "ltq_gemm_small")):
+            code = re.sub(r"//[^\n]*", "", open(path).read())
+            numbers = {int(n) for n in re.findall(r"(?<![\w.])(\d+)(?:u|ull)?\b", code)}
+            assert not [n for n in numbers if n and n % 148 == 0], path
