@@ -144,6 +144,22 @@ def test_one_row_of_a_tile_does_not_take_bits_from_another(cuda, form, dtype):
         assert diff < 2 * BOUND[dtype]
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("form", FORMS)
+def test_blocks_that_were_never_written_are_zeros(cuda, form, dtype):
+    """Parameters as KVCache.empty makes them, scale 0: scores and values of zero, whatever the codes are."""
+    import ltq
+    c = Case(cuda, ltq, form, dtype)
+    for block in (1, c.blocks // 2):
+        for n in "kv":
+            getattr(c.cache, n + "_qparams")[block] = 0
+            getattr(c.cache, n)[block] = 200
+    assert c.error() < BOUND[dtype]
+    for n in "kv":
+        getattr(c.cache, n + "_qparams")[:] = 0
+    assert (c.cache.attention(c.q, *c.args, scale=c.scale) == 0).all()
+
+
 # ---- long runs -------------------------------------------------------------------------------------------------------------
 # A table may name a block again and again: keys of a few blocks, each with its multiplicity, make long sequences whose 64-bit softmax
 # is as quick as that of the few.
