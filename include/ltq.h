@@ -423,7 +423,7 @@ typedef struct ltq_kv_cache {
  * tokens of that head (at least 2^-126); in a block that already holds some, the scale grows to that where it is larger, and
  * the codes already there become Quantize(Dequantize(code)) under the new scale.  An infinity or a NaN among the new values
  * makes the block's scale NaN, for good.  Slots behind the last token keep their bytes.  Appending the same tokens again
- * changes nothing.  Two sequences of one call must not append to the same block. */
+ * changes nothing.  No block may be appended to twice in one call, by two sequences or by a table that names it twice. */
 int ltq_cache_append(const ltq_kv_cache *cache, const void *k_dev, const void *v_dev, int dtype, uint64_t ld, uint64_t tokens,
                      const int32_t *offsets_dev, const int32_t *lengths_dev, const int32_t *table_dev, uint64_t seqs, uint64_t table_width,
                      uint64_t max_new, int device, void *stream);
