@@ -435,9 +435,9 @@ int ltq_cache_append(const ltq_kv_cache *cache, const void *k_dev, const void *v
  * same call.  workspace_dev: 16-byte aligned, ltq_cache_attention_workspace bytes (none for some sizes: then it may be NULL),
  * contents meaningless before and after;
  * calls that may overlap on the GPU need workspaces of their own.  q is taken to 22 significant bits (relative to its row's
- * largest entry) and the probabilities to 11 bits - 22 for float output; sums are held in float.  The bits of a probability count
- * with its block's V scale: of each row's products of the two those far below the largest, from 2^-21 of it, have fewer (all are
- * held to 2^-28 of it, to 2^-32 for few rows), and how V scales differ among the blocks makes no difference otherwise. */
+ * largest entry) and the products of probability and V's block scale to 11 bits - 22 for float output; those far below a row's
+ * largest have fewer, all are held to 2^-27 of it (many rows of half or bfloat16), to 2^-31 (otherwise).  How V's scales differ among the
+ * blocks makes no difference beyond that.  Sums are held in float. */
 uint64_t ltq_cache_attention_workspace(const ltq_kv_cache *cache, uint64_t tokens, uint32_t q_heads, uint64_t seqs, uint64_t table_width,
                                        uint64_t max_new, int device);
 int ltq_cache_attention(const ltq_kv_cache *cache, const void *q_dev, int dtype, uint64_t ld_q, uint64_t tokens, uint32_t q_heads,

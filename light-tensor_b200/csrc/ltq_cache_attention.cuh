@@ -35,8 +35,8 @@
 //    probabilities) and 2^d what V's scale adds to the largest weight.  (With the largest V scale in sight as the reference, one
 //    loud block that a row gives no weight took the bits of all others: 2^22 times louder, outputs were 2 % off and more.)
 //  * both references are kept only approximately: they move when a score exceeds m, or a weight m + d, by more than 8 (base 2), so
-//    that almost every step does without a reduction over lanes.  A weight at its reference is 2^7: halves end at 2^16, and
-//    what they lose below 2^-14 lies further from the largest.
+//    that almost every step does without a reduction over lanes.  A row's largest weight is 2^6 or more then, not 1: halves end
+//    at 2^16, and what they lose below 2^-14 (2^-25 at most) lies further from the largest.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
